@@ -7,6 +7,7 @@
 #include "vae_wide16.hip.h"
 #include "vae_wide16pp.hip.h"
 #include "vae_wide16s.hip.h"
+#include "ctx_internal.h"
 
 #include <hipcub/hipcub.hpp>
 #include <dlfcn.h>
@@ -468,17 +469,12 @@ void fill_lstm_args(drl_ctx* c, LstmArgs& a) {
 
 }  // namespace
 
+DrlCtxView drl_ctx_view(const drl_ctx* c) { return {c->device, c->n_cu, (void*)c->stream}; }
+int drl_ctx_fail(drl_ctx* c, int code, const char* msg) { return fail(c, code, "%s", msg); }
+void drl_count_alloc() { count_alloc(); }
+
 // =================================================================================================
 extern "C" {
-
-// DRL_SRC_HASH: sha256 (first 16 hex digits) over the library's sources, passed in by csrc/Makefile; bench.py
-// and tests/test_abi.py compare it with the hash of the tree they run from, so a stale prebuilt library shows.
-#ifndef DRL_SRC_HASH
-#define DRL_SRC_HASH "unknown"
-#endif
-#define DRL_STR2(x) #x
-#define DRL_STR(x) DRL_STR2(x)
-const char* drl_version(void) { return "drlvae 0.3 (gfx950; abi " DRL_STR(DRL_ABI_REVISION) "; src " DRL_SRC_HASH ")"; }
 
 int drl_create(int device_id, drl_ctx** out) {
     if (!out) return fail(nullptr, DRL_ERR_ARG, "drl_create: out is NULL");

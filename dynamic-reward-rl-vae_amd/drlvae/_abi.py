@@ -21,6 +21,8 @@ SYMBOLS = [
     "drl_last_lstm_variant", "drl_last_lstm_kernels", "drl_last_vae_variant", "drl_last_lstm_tile", "drl_last_call_overlapped",
     "drl_comm_unique_id", "drl_comm_init", "drl_allgather_scores", "drl_comm_destroy", "drl_comm_size",
     "drl_set_knob", "drl_debug_alloc_count",
+    "drl_seq_layout_create", "drl_seq_layout_destroy", "drl_attention_workspace", "drl_attention_dev", "drl_linear_attention_workspace",
+    "drl_linear_attention_dev", "drl_linear_attention_step_dev", "drl_group_norm_workspace", "drl_group_norm_dev",
 ]
 ABI_REVISION = 2          # DRL_ABI_REVISION of include/drlvae.h
 
@@ -45,6 +47,33 @@ class ScoreOpts(C.Structure):
         ("abi_revision", C.c_int32),
     ]
 
+
+_STRIDES = [(n, C.c_int64) for n in ("q_row", "q_head", "k_row", "k_head", "v_row", "v_head", "o_row", "o_head")]
+
+
+class SeqCall(C.Structure):
+    _fields_ = [("struct_size", C.c_int32), ("abi_revision", C.c_int32), ("dtype", C.c_int32), ("on_stream", C.c_int32),
+                ("stream", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64)]
+
+
+class AttnArgs(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v", "out", "lse", "key_mask", "k_len")] + _STRIDES + [
+        ("n_heads", C.c_int32), ("n_kv_heads", C.c_int32), ("dim", C.c_int32), ("causal", C.c_int32), ("window", C.c_int32),
+        ("scale", C.c_float)]
+
+
+class LinearArgs(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v", "out", "log_decay", "state_in", "state_out")] + _STRIDES + [
+        ("n_heads", C.c_int32), ("n_kv_heads", C.c_int32), ("dim_k", C.c_int32), ("dim_v", C.c_int32), ("scale", C.c_float),
+        ("reserved", C.c_int32)]
+
+
+class NormArgs(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("x", "y", "gamma", "beta")] + [("x_row", C.c_int64), ("y_row", C.c_int64)] + [
+        ("channels", C.c_int32), ("groups", C.c_int32), ("act", C.c_int32), ("eps", C.c_float)]
+
+
+SEQ_CALL_SIZE = C.sizeof(SeqCall)
 
 _lib = None
 
@@ -126,5 +155,16 @@ def load():
     lib.drl_set_knob.argtypes = [vp, C.c_char_p, C.c_longlong]
     lib.drl_debug_alloc_count.argtypes = []
     lib.drl_debug_alloc_count.restype = C.c_longlong
+    call, attn, lin, norm = C.POINTER(SeqCall), C.POINTER(AttnArgs), C.POINTER(LinearArgs), C.POINTER(NormArgs)
+    lib.drl_seq_layout_create.argtypes = [vp, _i64p, _i64p, C.c_int, C.POINTER(vp)]
+    lib.drl_seq_layout_destroy.argtypes = [vp]
+    lib.drl_seq_layout_destroy.restype = None
+    lib.drl_attention_workspace.argtypes = [vp, vp, call, attn, _i64p]
+    lib.drl_attention_dev.argtypes = [vp, vp, call, attn]
+    lib.drl_linear_attention_workspace.argtypes = [vp, vp, call, lin, _i64p]
+    lib.drl_linear_attention_dev.argtypes = [vp, vp, call, lin]
+    lib.drl_linear_attention_step_dev.argtypes = [vp, C.c_int64, call, lin]
+    lib.drl_group_norm_workspace.argtypes = [vp, vp, C.c_int64, call, norm, _i64p]
+    lib.drl_group_norm_dev.argtypes = [vp, vp, C.c_int64, call, norm]
     _lib = lib
     return lib

@@ -11,6 +11,7 @@ from typing import Dict, Optional, Sequence
 import numpy as np
 
 from . import _abi
+from .sequence import SequenceOps
 
 _MODES = {"zeros": _abi.FLAG_ZEROS, "quirk": _abi.FLAG_QUIRK, "explicit": _abi.FLAG_EXPLICIT,
           "both": _abi.FLAG_BOTH}
@@ -25,7 +26,7 @@ def _ptr(a) -> Optional[int]:
     return None if a is None else a.ctypes.data
 
 
-class WindowScorer:
+class WindowScorer(SequenceOps):
     def __init__(self, device: int = 0):
         self._lib = _abi.load()
         h = C.c_void_p()

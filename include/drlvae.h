@@ -233,6 +233,109 @@ int drl_al_get_samples(drl_ctx* ctx, const float* series, const int64_t* seg_off
                        const drl_score_opts* opts, const int32_t* already_selected, int n_selected, int N,
                        int32_t* out_idx, int32_t* n_out, float* margin_out);
 
+/* ---- sequence operators over packed series ---------------------------------------------------- */
+
+/* The mixers a sequence network over the same packed series is built from, beside the LSTM: softmax attention,
+ * linear attention with a decaying state, and the normalisation with activation behind them.  Forward only.  They
+ * have NO counterpart in the reference.  All pointers are device memory on the context's GPU; a call enqueues on one
+ * stream and returns without synchronising, allocates nothing, keeps nothing, and may be captured into a HIP graph.
+ * Calls may overlap in time as long as they do not share a workspace or an output. */
+typedef enum drl_dtype { DRL_F32 = 0, DRL_F16 = 1, DRL_BF16 = 2 } drl_dtype;
+enum { DRL_ACT_SILU = 3 };      /* drl_group_norm_dev only: x * sigmoid(x); drl_set_vae refuses it */
+
+/* Which rows belong to which series: the plan of the calls below, made once per batch layout.  Series i owns rows
+ * q_offsets[i] .. q_offsets[i+1]-1 of q (x, out) and rows k_offsets[i] .. k_offsets[i+1]-1 of k and v; offsets are host
+ * memory, n_seg+1 entries, non-decreasing and not negative; rows outside q_offsets[0] .. q_offsets[n_seg] are neither
+ * read nor written.  k_offsets NULL: the same as q_offsets.  Fewer than 2^31 rows on each side.  Creation and
+ * destruction allocate and free device memory and may synchronise: not during a capture.  A layout is immutable, may
+ * be used from any context on the same GPU, and has to outlive the calls, and the captured graphs, that use it. */
+typedef struct drl_seq_layout drl_seq_layout;
+int drl_seq_layout_create(drl_ctx* ctx, const int64_t* q_offsets, const int64_t* k_offsets, int n_seg, drl_seq_layout** out);
+void drl_seq_layout_destroy(drl_seq_layout* layout);
+
+/* What every call says beside its operands. */
+typedef struct drl_seq_call {
+    int32_t struct_size;      /* sizeof(drl_seq_call) */
+    int32_t abi_revision;     /* DRL_ABI_REVISION */
+    int32_t dtype;            /* drl_dtype of q, k, v, x and of the output */
+    int32_t on_stream;        /* 0: the context's stream; 1: `stream`, also when that is NULL (the GPU's null stream) */
+    void* stream;
+    void* workspace;          /* 16-byte aligned device memory of at least what the operator's _workspace call says (it
+                                 may say 0); the call's own until the stream has passed it */
+    int64_t workspace_bytes;
+} drl_seq_call;
+
+/* Softmax attention with grouped heads.  Head h of a row of q attends with kv head h / (n_heads / n_kv_heads):
+ *   out_i = sum_j softmax_j(scale q_i.k_j) v_j,   lse_i = log sum_j exp(scale q_i.k_j)     over the visible keys j.
+ * In a series of nq rows and nk keys, row i sees key j when j <= i + nk - nq (causal), j > i + nk - nq - window
+ * (window > 0), and key_mask[j] != 0.  A row that sees nothing gets out = 0, lse = -inf.  What q, k or v hold behind
+ * masked keys, infinities and NaN included, has no influence.  nq = 1 is the step of a live series against its cache:
+ * k_offsets then name the cache's slots, and k_len how many of each are filled. */
+typedef struct drl_attn_args {
+    const void* q;            /* rows x n_heads x dim */
+    const void* k;            /* rows x n_kv_heads x dim */
+    const void* v;
+    void* out;                /* as q; overlaps no input */
+    float* lse;               /* [rows of q, n_heads], may be NULL */
+    const uint8_t* key_mask;  /* one byte per row of k, 0 = not there; may be NULL */
+    const int32_t* k_len;     /* keys of each series, counted from its first; values outside 0 .. its rows in the layout
+                                 are clamped to that; NULL: all of them */
+    int64_t q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head;   /* strides in elements; the last axis is dense;
+                                 multiples of 16 bytes, like every pointer */
+    int32_t n_heads, n_kv_heads;
+    int32_t dim;              /* 8 .. 128, a multiple of 8 */
+    int32_t causal, window;   /* window 0: none */
+    float scale;              /* > 0 */
+} drl_attn_args;
+int drl_attention_workspace(drl_ctx* ctx, const drl_seq_layout* layout, const drl_seq_call* call, const drl_attn_args* args,
+                            int64_t* bytes);
+int drl_attention_dev(drl_ctx* ctx, const drl_seq_layout* layout, const drl_seq_call* call, const drl_attn_args* args);
+
+/* Linear attention with an exponential decay per head, for head h of a series, from its first row to its last:
+ *   S <- exp(d_h) S + k_t v_t^T,   out_t = scale S^T q_t,      d_h = min(log_decay[h], 0)
+ * The states S are float32 [n_seg, n_heads, dim_k, dim_v]; state_in NULL: they start at 0; state_out NULL: the last
+ * ones are not kept; state_out may be state_in.  A series without rows hands its state on.  k_offsets of the layout are
+ * not used: k and v have q's rows.
+ * drl_linear_attention_step_dev: n series with one row each, state_in and state_out required. */
+typedef struct drl_linear_args {
+    const void* q;            /* rows x n_heads x dim_k */
+    const void* k;            /* rows x n_kv_heads x dim_k */
+    const void* v;            /* rows x n_kv_heads x dim_v */
+    void* out;                /* rows x n_heads x dim_v; overlaps no input */
+    const float* log_decay;   /* [n_heads] */
+    const float* state_in;
+    float* state_out;
+    int64_t q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head;   /* as in drl_attn_args */
+    int32_t n_heads, n_kv_heads;
+    int32_t dim_k;            /* 8 .. 128, a multiple of 8 */
+    int32_t dim_v;            /* 8 .. 256, a multiple of 8 */
+    float scale;              /* finite */
+    int32_t reserved;         /* 0 */
+} drl_linear_args;
+int drl_linear_attention_workspace(drl_ctx* ctx, const drl_seq_layout* layout, const drl_seq_call* call,
+                                   const drl_linear_args* args, int64_t* bytes);
+int drl_linear_attention_dev(drl_ctx* ctx, const drl_seq_layout* layout, const drl_seq_call* call, const drl_linear_args* args);
+int drl_linear_attention_step_dev(drl_ctx* ctx, int64_t n, const drl_seq_call* call, const drl_linear_args* args);
+
+/* Group normalisation with an activation, channels last: channels are cut into `groups` equal groups, and over each
+ * group's channels, in all rows of a series (layout NULL: in each of `rows` rows by itself),
+ *   y = act((x - mean) / sqrt(var + eps) * gamma + beta)          (var: the mean squared deviation)
+ * y may be x (with the same row stride). */
+typedef struct drl_norm_args {
+    const void* x;            /* rows x channels */
+    void* y;
+    const float* gamma;       /* [channels], may be NULL (1) */
+    const float* beta;        /* [channels], may be NULL (0) */
+    int64_t x_row, y_row;     /* row strides in elements, at least channels */
+    int32_t channels, groups;
+    int32_t act;              /* DRL_ACT_LINEAR, DRL_ACT_RELU, DRL_ACT_SIGMOID or DRL_ACT_SILU */
+    float eps;                /* > 0 */
+} drl_norm_args;
+int drl_group_norm_workspace(drl_ctx* ctx, const drl_seq_layout* layout, int64_t rows, const drl_seq_call* call,
+                             const drl_norm_args* args, int64_t* bytes);
+int drl_group_norm_dev(drl_ctx* ctx, const drl_seq_layout* layout, int64_t rows, const drl_seq_call* call,
+                       const drl_norm_args* args);
+
 /* ---- the only collective of the path ------------------------------------------------------------ */
 
 /* The reference is single-process; windows shard across the GPUs of a node with weights
