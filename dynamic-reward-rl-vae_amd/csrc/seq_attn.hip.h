@@ -1,4 +1,13 @@
 // Softmax attention over packed series.
+//
+//   z_ij = scale q_i.k_j,   out_i = sum_j exp(z_ij) v_j / sum_j exp(z_ij)       over the keys j that row i sees
+//
+// in one pass over the keys with a running reference m (no running maximum is needed: any m works as long as
+// exp(z - m) neither overflows nor loses the largest terms), weights p_j = exp(z_j - m), their sum l and the weighted
+// sum o; when the maximum passes m by more than 8 (in powers of two) o and l are multiplied by the ratio and m follows.
+//
+// A "row" of the products is one (row of q, head) pair: the heads that share a kv head lie side by side, so its keys
+// and values are read once for all of them, and a single new row per series still fills part of a tile.
 #pragma once
 #include "seq_common.hip.h"
 
@@ -16,6 +25,12 @@ struct AttnArgs {
     int heads, rep, dim;
     int causal, window;
     float scale;
+    // heads of one kv head are cut into `blocks` runs of `rep_b`; a tile holds `per` rows of q of one run
+    int kv_blocks, blocks, rep_b, per;
+    // the keys are cut into runs of `chunk` (splits > 1): partial results of run y, normalised, and their log-sums
+    int splits, chunk;
+    float *part_o, *part_lse;      // [splits][rows][heads][dim], [splits][rows][heads], rows from the first series' first
+    int64_t part_rows, row0;
 };
 
 // The keys [lo, hi) that row i of a series may see by position (the key mask apart).
@@ -29,10 +44,14 @@ __device__ __forceinline__ int keys_of(const AttnArgs& a, const SegInfo& s) {
     return a.k_len ? max(0, min(a.k_len[s.seg], s.nk)) : s.nk;
 }
 
-// One row and head by one wave, straight from the definition: 64 keys at a time, a lane per key for the scores, lanes
-// over the width for the sum.  Touches nothing but the visible keys' rows.
+// m and l of a row to its log-sum; l = 0 where nothing was seen.
+__device__ __forceinline__ float log_sum(float m, float l) { return l == 0.0f ? -INFINITY : m + LN2 * __builtin_amdgcn_logf(l); }
+
+// One row and head by one wave, straight from the definition, over the keys [from, to): a lane per key for the scores,
+// lanes over the width for the sum.  Touches nothing but the visible keys' rows.  Where a tile holds values that are
+// not finite and that some of its rows must not see, its rows are computed like this.
 template <typename T>
-__device__ void attn_row(const AttnArgs& a, const SegInfo& s, int nk, int i, int h) {
+__device__ __forceinline__ void attn_row(const AttnArgs& a, const SegInfo& s, int nk, int i, int h, int from, int to, int split) {
     const int lane = threadIdx.x & 63;
     const int64_t row = s.q0 + i;
     const T* q = (const T*)a.q + row * a.q_row + (int64_t)h * a.q_head;
@@ -40,6 +59,8 @@ __device__ void attn_row(const AttnArgs& a, const SegInfo& s, int nk, int i, int
     const T* vb = (const T*)a.v + s.k0 * a.v_row + (int64_t)(h / a.rep) * a.v_head;
     int lo, hi;
     visible(a, i, s.nq, nk, lo, hi);
+    lo = max(lo, from);
+    hi = min(hi, to);
     float top = -INFINITY, sum = 0.0f, o0 = 0.0f, o1 = 0.0f;
     for (int base = lo; base < hi; base += 64) {
         const int j = base + lane;
@@ -70,13 +91,309 @@ __device__ void attn_row(const AttnArgs& a, const SegInfo& s, int nk, int i, int
         }
     }
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;      // a NaN sum stays one
+    const float lse = log_sum(top == -INFINITY ? 0.0f : top, sum);
+    if (a.splits > 1) {
+        const int64_t at = ((int64_t)split * a.part_rows + row - a.row0) * a.heads + h;
+        float* o = a.part_o + at * a.dim;
+        if (lane < a.dim) o[lane] = o0 * inv;
+        if (lane + 64 < a.dim) o[lane + 64] = o1 * inv;
+        if (lane == 0) a.part_lse[at] = lse;
+        return;
+    }
     T* o = (T*)a.out + row * a.o_row + (int64_t)h * a.o_head;
     if (lane < a.dim) o[lane] = (T)(o0 * inv);
     if (lane + 64 < a.dim) o[lane + 64] = (T)(o1 * inv);
-    if (a.lse && lane == 0)
-        a.lse[row * a.heads + h] = sum == 0.0f ? -INFINITY : (top == -INFINITY ? 0.0f : top) + LN2 * __builtin_amdgcn_logf(sum);
+    if (a.lse && lane == 0) a.lse[row * a.heads + h] = lse;
 }
 
+// Which tile of which series a workgroup has: units of `per` rows, the longest series and the last rows (causal: the ones
+// with the most keys) first.  The kv head changes fastest, so that with eight of them each XCD's L2 holds one.
+struct AttnTile {
+    SegInfo s;
+    int nk, kv, head0, n_heads, i0, rows;     // rows: (row, head) pairs
+    bool any;
+};
+__device__ __forceinline__ AttnTile attn_tile(const AttnArgs& a, int64_t id) {
+    AttnTile t;
+    const int b = (int)(id % a.kv_blocks);
+    const int64_t u = id / a.kv_blocks;
+    const int slot = find_seg(a.segs, a.n_seg, u, a.per);
+    t.s = a.segs[slot];
+    t.kv = b / a.blocks;
+    const int first = (b % a.blocks) * a.rep_b;
+    t.head0 = t.kv * a.rep + first;
+    t.n_heads = min(a.rep_b, a.rep - first);
+    const int n = (t.s.nq + a.per - 1) / a.per;
+    const int k = (int)(u - (t.s.cum / a.per + slot));
+    t.any = k < n && t.n_heads > 0;
+    t.i0 = (n - 1 - k) * a.per;
+    t.rows = t.any ? min(a.per, t.s.nq - t.i0) * t.n_heads : 0;
+    t.nk = keys_of(a, t.s);
+    return t;
+}
+
+// 16-bit types.  A workgroup of four waves has 128 rows, a wave 32 of them; keys and values go through LDS in tiles of 64
+// keys, two of them in turn (64 KiB at dim 128: two workgroups per CU, one wave of each per SIMD, so that one's softmax
+// runs beside the other's products).
+// Scores are computed transposed, keys x rows: a lane then holds 32 scores of ONE row, half of the tile's keys (the lane 32
+// away has the others), the maximum is one exchange away, and the weights, rounded to the inputs' type (relative error
+// u = eps/2 each, as the result's own rounding), are as they lie in registers the second operand of values^T x weights: the
+// order of the keys inside the product is free, and the values are read with ds_read_b64_tr_b16 in the weights' order.
+template <typename T, int DT>
+__global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
+    typedef typename Vec<T>::x8 x8;
+    typedef typename Vec<T>::x4 x4;
+    constexpr int DP = DT <= 1 ? 32 : DT <= 2 ? 64 : 128;     // elements of a tile row in LDS
+    constexpr int NC = DP / 8, KS = 2 * DT, BK = 64;
+    constexpr int TILE = BK * DP * 2;                         // bytes of a tile of keys (or values)
+    constexpr int LOADS = BK * NC / 256;                      // 16-byte loads per thread and tile
+    extern __shared__ char smem[];
+    const uint32_t lds = lds_offset(smem);
+    const AttnTile t = attn_tile(a, blockIdx.x);
+    if (!t.any) return;
+    const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+
+    // this lane's row
+    const int pr = wave * 32 + col;
+    const bool row_ok = pr < t.rows;
+    const int prc = row_ok ? pr : t.rows - 1;
+    const int i = t.i0 + prc / t.n_heads, h = t.head0 + prc % t.n_heads;
+    int lo, hi;
+    visible(a, i, t.s.nq, t.nk, lo, hi);
+    int LO, HI, x0, x1;      // what any row of the workgroup sees
+    visible(a, t.i0, t.s.nq, t.nk, LO, x0);
+    visible(a, t.i0 + (t.rows - 1) / t.n_heads, t.s.nq, t.nk, x1, HI);
+    const int all_lo = x1, all_hi = x0;                        // what all of them see
+    if (a.splits > 1) {
+        LO += (int)min((int64_t)blockIdx.y * a.chunk, (int64_t)0x3fffffff);
+        HI = min(HI, LO + a.chunk);
+    }
+    const int wl = __builtin_amdgcn_readfirstlane(__shfl(lo, 0)), wh = __builtin_amdgcn_readfirstlane(__shfl(hi, 31));  // this wave's rows: they rise with the lane
+
+    x8 qf[KS];
+    {
+        const T* q = (const T*)a.q + (t.s.q0 + i) * a.q_row + (int64_t)h * a.q_head;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const int d = 16 * s + 8 * half;
+            u32x4 x = {0, 0, 0, 0};
+            if (d < a.dim) x = *(const u32x4*)(q + d);
+            qf[s] = __builtin_bit_cast(x8, x);
+        }
+    }
+
+    // staging: thread's slots of a tile, row and chunk; chunks behind the width come from zeros
+    const char* kp = (const char*)((const T*)a.k + t.s.k0 * a.k_row + (int64_t)t.kv * a.k_head);
+    const char* vp = (const char*)((const T*)a.v + t.s.k0 * a.v_row + (int64_t)t.kv * a.v_head);
+    const int64_t kr = a.k_row * 2, vr = a.v_row * 2;
+    int srow[LOADS], schunk[LOADS];
+#pragma unroll
+    for (int n = 0; n < LOADS; ++n) {
+        const int slot = n * 256 + threadIdx.x;
+        srow[n] = slot / NC;
+        schunk[n] = ((slot % NC) ^ swz<NC>(srow[n])) * 16;
+        if (schunk[n] >= a.dim * 2) schunk[n] = -1;
+    }
+    auto stage = [&](int base, int buf) {
+        const uint32_t at = lds + buf * 2 * TILE + wave * 1024;
+#pragma unroll
+        for (int n = 0; n < LOADS; ++n) {
+            const int j = min(base + srow[n], t.nk - 1);
+            const void* kg = schunk[n] >= 0 ? (const void*)(kp + j * kr + schunk[n]) : (const void*)&zero16;
+            const void* vg = schunk[n] >= 0 ? (const void*)(vp + j * vr + schunk[n]) : (const void*)&zero16;
+            load_lds16(kg, at + n * 4096);
+            load_lds16(vg, at + TILE + n * 4096);
+        }
+    };
+
+    // operand reads: keys as rows, values transposed
+    uint32_t koff[KS], voff[DT][2];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) koff[s] = col * (DP * 2) + (((2 * s + half) ^ swz<NC>(col)) * 16);
+    {
+        const int g = (lane >> 4) & 1, i4 = lane & 15;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int r = 8 * j + 4 * half + (i4 >> 2);
+                const int c = dt * 4 + g * 2 + ((i4 & 3) >> 1);
+                voff[dt][j] = r * (DP * 2) + ((c ^ swz<NC>(r)) * 16) + (i4 & 1) * 8;
+            }
+    }
+
+    const float c1 = a.scale * LOG2E;
+    float ref = -INFINITY, mc = 0.0f;        // the reference, in units of the raw score; mc = ref * c1, 0 while there is none
+    float l0 = 0.0f, l1 = 0.0f;
+    f32x16 o[DT];
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[dt][r] = 0.0f;
+
+    bool strange = false;
+    if (LO < HI) stage(LO, 0);
+    int buf = 0;
+    for (int base = LO; base < HI; base += BK, buf ^= 1) {
+        wait_loads();
+        __syncthreads();
+        if (base + BK < HI) stage(base + BK, buf ^ 1);
+        const uint32_t kt_ = lds + buf * 2 * TILE, vt_ = kt_ + TILE;
+
+        // A tile that some rows see only in part: values that are not finite must not meet the weight 0 of the rows that
+        // do not see them.  Rows that nobody sees are cleared; if others hold such values, the rows are done one by one.
+        uint64_t there = ~0ull;
+        const bool edge = a.key_mask || base < all_lo || base + BK > all_hi;
+        if (edge) {
+            const int j = base + lane;
+            there = __ballot(j < HI && (!a.key_mask || a.key_mask[t.s.k0 + j]));
+            int odd = 0;
+#pragma unroll
+            for (int n = 0; n < LOADS; ++n) {
+                const uint32_t at = vt_ + (n * 256 + threadIdx.x) * 16;
+                if (!((there >> srow[n]) & 1)) lds_write<u32x4>(at, u32x4{0, 0, 0, 0});
+                else {
+                    const u32x4 x = lds_read<u32x4>(at);
+                    constexpr uint32_t E = sizeof(T) == 2 && __is_same(T, bf16) ? 0x7f80u : 0x7c00u;
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) odd |= (x[w] & E) == E || ((x[w] >> 16) & E) == E;
+                }
+            }
+            if (__syncthreads_or(odd)) { strange = true; break; }
+        }
+        if (base >= wh || base + BK <= wl) continue;         // nothing of it for this wave
+
+        f32x16 z[2];
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) z[kt][r] = 0.0f;
+#pragma unroll
+            for (int s = 0; s < KS; ++s) z[kt] = mfma(lds_read<x8>(kt_ + koff[s] + kt * 32 * DP * 2), qf[s], z[kt]);
+        }
+        if (edge) {
+            const int from = max(lo - base, 0), to = min(hi - base, 64);
+            uint64_t see = to <= from ? 0 : there & (~0ull << from) & (~0ull >> (64 - to));
+            see >>= 4 * half;
+            const uint32_t s0 = (uint32_t)see, s1 = (uint32_t)(see >> 32);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                z[0][r] = (s0 >> acc_row(r, 0)) & 1 ? z[0][r] : -INFINITY;
+                z[1][r] = (s1 >> acc_row(r, 0)) & 1 ? z[1][r] : -INFINITY;
+            }
+        }
+        float m = fmaxf(z[0][0], z[1][0]);
+#pragma unroll
+        for (int r = 1; r < 16; ++r) m = fmaxf(m, fmaxf(z[0][r], z[1][r]));
+        m = pair_max(m);
+        if (__any((m - ref) * c1 > 8.0f)) {
+            const float now = fmaxf(m, ref);
+            const float mcn = now == -INFINITY ? 0.0f : now * c1;
+            const float f = ref == -INFINITY ? 0.0f : exp2_fast(mc - mcn);
+            ref = now;
+            mc = mcn;
+            l0 *= f;
+            l1 *= f;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[dt][r] *= f;
+        }
+        x8 p[4];
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+            for (int r = 0; r < 16; r += 2) {
+                const float w0 = exp2_fast(fmaf(z[kt][r], c1, -mc)), w1 = exp2_fast(fmaf(z[kt][r + 1], c1, -mc));
+                l0 += w0;                     // the sum takes the weights as they are: the log-sum is float32
+                l1 += w1;
+                p[2 * kt + (r >> 3)][r & 7] = (T)w0;
+                p[2 * kt + (r >> 3)][(r & 7) + 1] = (T)w1;
+            }
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+                const s16x4 v0 = lds_read_tr(vt_ + voff[dt][0] + s * 16 * DP * 2);
+                const s16x4 v1 = lds_read_tr(vt_ + voff[dt][1] + s * 16 * DP * 2);
+                typedef short s16x8 __attribute__((ext_vector_type(8)));
+                const s16x8 v = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
+                o[dt] = mfma(__builtin_bit_cast(x8, v), p[s], o[dt]);
+            }
+    }
+    if (strange) {
+        wait_loads();
+        for (int r = wave; r < t.rows; r += 4)
+            attn_row<T>(a, t.s, t.nk, t.i0 + r / t.n_heads, t.head0 + r % t.n_heads, LO, HI, blockIdx.y);
+        return;
+    }
+
+    const float l = pair_sum(l0 + l1);
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;           // a NaN sum stays one
+    const float lse = log_sum(mc * LN2, l);
+    if (!row_ok) return;
+    const int64_t row = t.s.q0 + i;
+    if (a.splits > 1) {
+        const int64_t at = ((int64_t)blockIdx.y * a.part_rows + row - a.row0) * a.heads + h;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const int d = dt * 32 + acc_row(r, half);
+                if (d < a.dim) *(f32x4*)(a.part_o + at * a.dim + d) = f32x4{o[dt][r] * inv, o[dt][r + 1] * inv, o[dt][r + 2] * inv, o[dt][r + 3] * inv};
+            }
+        if (half == 0) a.part_lse[at] = lse;
+        return;
+    }
+    T* out = (T*)a.out + row * a.o_row + (int64_t)h * a.o_head;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+            const int d = dt * 32 + acc_row(r, half);
+            const x4 w = {(T)(o[dt][r] * inv), (T)(o[dt][r + 1] * inv), (T)(o[dt][r + 2] * inv), (T)(o[dt][r + 3] * inv)};
+            if (d < a.dim) *(x4*)(out + d) = w;
+        }
+    if (a.lse && half == 0) a.lse[row * a.heads + h] = lse;
+}
+
+// Joins the runs of keys of a row and head: weights exp(lse_y - max), one wave each.
+template <typename T>
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
+    const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (id >= a.part_rows * a.heads) return;
+    const int lane = threadIdx.x & 63;
+    const int64_t stride = a.part_rows * a.heads;
+    float m = -INFINITY;
+    bool nan = false;
+    for (int y = lane; y < a.splits; y += 64) {
+        const float x = a.part_lse[y * stride + id];
+        m = fmaxf(m, x);
+        nan |= x != x;
+    }
+    m = wave_max(m);
+    if (__any(nan)) m = NAN;
+    const float mm = m == -INFINITY ? 0.0f : m;
+    float l = 0.0f, o0 = 0.0f, o1 = 0.0f;
+    for (int y = 0; y < a.splits; ++y) {
+        const float x = a.part_lse[y * stride + id];
+        if (x == -INFINITY) continue;                        // a run in which nothing is seen holds zeros
+        const float w = exp2_fast((x - mm) * LOG2E);
+        const float* o = a.part_o + (y * stride + id) * a.dim;
+        l += w;
+        if (lane < a.dim) o0 = fmaf(w, o[lane], o0);
+        if (lane + 64 < a.dim) o1 = fmaf(w, o[lane + 64], o1);
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const int64_t row = a.row0 + id / a.heads;
+    const int h = (int)(id % a.heads);
+    T* out = (T*)a.out + row * a.o_row + (int64_t)h * a.o_head;
+    if (lane < a.dim) out[lane] = (T)(o0 * inv);
+    if (lane + 64 < a.dim) out[lane + 64] = (T)(o1 * inv);
+    if (a.lse && lane == 0) a.lse[row * a.heads + h] = log_sum(mm, l);
+}
+
+// The definition, a wave per row and head.
 template <typename T>
 __global__ __launch_bounds__(256) void attn_rows_kernel(AttnArgs a) {
     const int64_t t = (int64_t)blockIdx.x;
@@ -84,7 +401,7 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnArgs a) {
     const SegInfo s = a.segs[slot];
     const int i = (int)(t - (s.cum / 4 + slot)) * 4 + (int)(threadIdx.x >> 6);
     if (i >= s.nq) return;
-    attn_row<T>(a, s, keys_of(a, s), i, blockIdx.y);
+    attn_row<T>(a, s, keys_of(a, s), i, blockIdx.y, 0, 0x7fffffff, 0);
 }
 
 }  // namespace seq

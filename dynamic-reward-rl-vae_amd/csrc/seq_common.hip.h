@@ -60,4 +60,56 @@ __device__ __forceinline__ int find_seg(const SegInfo* segs, int n_seg, int64_t 
     return __builtin_amdgcn_readfirstlane(lo);
 }
 
+// ---- tiles in LDS ------------------------------------------------------------------------------------------------
+// A tile row holds NC chunks of 16 bytes; chunk c of row r lies at place c ^ swz<NC>(r).  With it neither the reads of one
+// chunk of 16 consecutive rows (ds_read_b128, an MFMA operand's rows) nor the transposing reads of four consecutive
+// rows by 64 bytes (ds_read_b64_tr_b16) meet on a bank: LDS has 64 banks of 4 bytes, so 256 bytes go at once.
+template <int NC>
+__device__ __forceinline__ int swz(int r) {
+    if constexpr (NC == 4) return (r >> 2) & 3;
+    else if constexpr (NC == 8) return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
+    else return ((r & 3) << 2) | ((r >> 2) & 3);
+}
+
+typedef __attribute__((address_space(3))) char lds_char;
+__device__ __forceinline__ uint32_t lds_offset(const void* p) { return (uint32_t)(uintptr_t)(lds_char*)p; }
+
+// 16 bytes per lane from global memory into LDS at `lds` + 16 * lane (the same `lds` for the whole wave), without
+// registers between.  Nothing waits for it by itself: wait_loads() does, then a barrier shows it to the other waves.
+// (m0 is written: nothing else in these kernels uses it, and the compiler sets it before uses of its own.)
+__device__ __forceinline__ void load_lds16(const void* g, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(g) : "memory");
+}
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+template <typename V>
+__device__ __forceinline__ V lds_read(uint32_t at) { return *(const __attribute__((address_space(3))) V*)at; }
+template <typename V>
+__device__ __forceinline__ void lds_write(uint32_t at, V x) { *(__attribute__((address_space(3))) V*)at = x; }
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+// Lane i of a group of 16 names 8 bytes: row i / 4 of four, columns 4 (i % 4) ..; it gets column i of the four rows.
+__device__ __forceinline__ s16x4 lds_read_tr(uint32_t at) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at);
+}
+
+// The larger / the sum of a lane's value and that of the lane 32 away.
+__device__ __forceinline__ float pair_max(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
+    return fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
+}
+__device__ __forceinline__ float pair_sum(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
+    return __builtin_bit_cast(float, (uint32_t)r[0]) + __builtin_bit_cast(float, (uint32_t)r[1]);
+}
+
+// 32x32x16 product: lane l holds row (column) l & 31 of A (B), elements 8 (l >> 5) .. + 7 of the inner axis; of the result
+// column l & 31, rows (r & 3) + 8 (r >> 2) + 4 (l >> 5) in registers r = 0 .. 15.
+__device__ __forceinline__ f32x16 mfma(Vec<bf16>::x8 a, Vec<bf16>::x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x16 mfma(Vec<f16>::x8 a, Vec<f16>::x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ int acc_row(int r, int half) { return (r & 3) + 8 * (r >> 2) + 4 * half; }
+
+// Sixteen bytes of zeros: where lanes load from whose chunk lies behind a row's end.
+__device__ const u32x4 zero16 = {0, 0, 0, 0};
+
 }  // namespace seq

@@ -153,13 +153,34 @@ int drl_attention_dev(drl_ctx* c, const drl_seq_layout* l, const drl_seq_call* c
     const DrlCtxView v = drl_ctx_view(c);
     DeviceGuard guard(v.device);
     if (!guard.ok) return hip_fail(c, "drl_attention_dev", hipErrorInvalidDevice);
-    seq::AttnArgs k = {a->q, a->k, a->v, a->out, a->lse, a->key_mask, a->k_len, a->q_row, a->q_head, a->k_row, a->k_head,
-                       a->v_row, a->v_head, a->o_row, a->o_head, l->segs, l->rows.n_seg, a->n_heads, a->n_heads / a->n_kv_heads,
-                       a->dim, a->causal != 0, a->window, a->scale};
+    seq::AttnArgs k = {};
+    k.q = a->q; k.k = a->k; k.v = a->v; k.out = a->out; k.lse = a->lse; k.key_mask = a->key_mask; k.k_len = a->k_len;
+    k.q_row = a->q_row; k.q_head = a->q_head; k.k_row = a->k_row; k.k_head = a->k_head;
+    k.v_row = a->v_row; k.v_head = a->v_head; k.o_row = a->o_row; k.o_head = a->o_head;
+    k.segs = l->segs; k.n_seg = l->rows.n_seg; k.heads = a->n_heads; k.rep = a->n_heads / a->n_kv_heads; k.dim = a->dim;
+    k.causal = a->causal != 0; k.window = a->window; k.scale = a->scale;
+    k.splits = 1;
+    const hipStream_t st = stream_of(v, call);
     by_type(call->dtype, [&](auto* t) {
         typedef std::remove_pointer_t<decltype(t)> T;
-        const dim3 grid((unsigned)(l->n_q / 4 + l->rows.n_seg), a->n_heads);
-        hipLaunchKernelGGL((seq::attn_rows_kernel<T>), grid, dim3(256), 0, stream_of(v, call), k);
+        if constexpr (sizeof(T) == 2) {
+            constexpr int BM = 128;
+            k.blocks = (k.rep + BM - 1) / BM;
+            k.rep_b = (k.rep + k.blocks - 1) / k.blocks;
+            k.kv_blocks = a->n_kv_heads * k.blocks;
+            k.per = BM / k.rep_b;
+            const int64_t tiles = (l->n_q / k.per + l->rows.n_seg) * k.kv_blocks;
+            const int dt = (a->dim + 31) / 32;
+            const size_t shmem = 4 * 64 * 2 * (dt == 1 ? 32 : dt == 2 ? 64 : 128);
+            const dim3 grid((unsigned)tiles);
+            if (dt == 1) hipLaunchKernelGGL((seq::attn_tile_kernel<T, 1>), grid, dim3(256), shmem, st, k);
+            else if (dt == 2) hipLaunchKernelGGL((seq::attn_tile_kernel<T, 2>), grid, dim3(256), shmem, st, k);
+            else if (dt == 3) hipLaunchKernelGGL((seq::attn_tile_kernel<T, 3>), grid, dim3(256), shmem, st, k);
+            else hipLaunchKernelGGL((seq::attn_tile_kernel<T, 4>), grid, dim3(256), shmem, st, k);
+        } else {
+            const dim3 grid((unsigned)(l->n_q / 4 + l->rows.n_seg), a->n_heads);
+            hipLaunchKernelGGL((seq::attn_rows_kernel<T>), grid, dim3(256), 0, st, k);
+        }
     });
     return launched(c, "drl_attention_dev");
 }
