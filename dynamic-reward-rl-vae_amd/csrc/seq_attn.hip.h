@@ -139,7 +139,9 @@ __device__ __forceinline__ AttnTile attn_tile(const AttnArgs& a, int64_t id) {
 // away has the others), the maximum is one exchange away, and the weights, rounded to the inputs' type (relative error
 // u = eps/2 each, as the result's own rounding), are as they lie in registers the second operand of values^T x weights: the
 // order of the keys inside the product is free, and the values are read with ds_read_b64_tr_b16 in the weights' order.
-template <typename T, int DT>
+// FEW: at most 32 rows (steps).  One wave computes, all four load; reading the cache is what takes the time, so what the
+// weights lose by rounding goes into a second product.
+template <typename T, int DT, bool FEW>
 __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
     typedef typename Vec<T>::x8 x8;
     typedef typename Vec<T>::x4 x4;
@@ -261,7 +263,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
             }
             if (__syncthreads_or(odd)) { strange = true; break; }
         }
-        if (base >= wh || base + BK <= wl) continue;         // nothing of it for this wave
+        if (base >= wh || base + BK <= wl || wave * 32 >= t.rows) continue;         // nothing of it for this wave
 
         f32x16 z[2];
 #pragma unroll
@@ -299,7 +301,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) o[dt][r] *= f;
         }
-        x8 p[4];
+        x8 p[4], p2[FEW ? 4 : 1];
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
@@ -307,8 +309,13 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
                 const float w0 = exp2_fast(fmaf(z[kt][r], c1, -mc)), w1 = exp2_fast(fmaf(z[kt][r + 1], c1, -mc));
                 l0 += w0;                     // the sum takes the weights as they are: the log-sum is float32
                 l1 += w1;
-                p[2 * kt + (r >> 3)][r & 7] = (T)w0;
-                p[2 * kt + (r >> 3)][(r & 7) + 1] = (T)w1;
+                const int g = 2 * kt + (r >> 3);
+                p[g][r & 7] = (T)w0;
+                p[g][(r & 7) + 1] = (T)w1;
+                if constexpr (FEW) {
+                    p2[g][r & 7] = (T)(w0 - (float)p[g][r & 7]);
+                    p2[g][(r & 7) + 1] = (T)(w1 - (float)p[g][(r & 7) + 1]);
+                }
             }
 #pragma unroll
         for (int s = 0; s < 4; ++s)
@@ -319,6 +326,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
                 typedef short s16x8 __attribute__((ext_vector_type(8)));
                 const s16x8 v = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
                 o[dt] = mfma(__builtin_bit_cast(x8, v), p[s], o[dt]);
+                if constexpr (FEW) o[dt] = mfma(__builtin_bit_cast(x8, v), p2[s], o[dt]);
             }
     }
     if (strange) {
@@ -357,33 +365,50 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
     if (a.lse && half == 0) a.lse[row * a.heads + h] = lse;
 }
 
-// Joins the runs of keys of a row and head: weights exp(lse_y - max), one wave each.
+// Joins the runs of keys of a row and head: weights exp(lse_y - max), one wave each.  A run in which nothing is seen
+// (log-sum -inf) weighs nothing and its partial result is not read.
 template <typename T>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
     const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (id >= a.part_rows * a.heads) return;
     const int lane = threadIdx.x & 63;
     const int64_t stride = a.part_rows * a.heads;
-    float m = -INFINITY;
-    bool nan = false;
+    float m = -INFINITY, bad = 0.0f;
     for (int y = lane; y < a.splits; y += 64) {
         const float x = a.part_lse[y * stride + id];
         m = fmaxf(m, x);
-        nan |= x != x;
+        bad += x != x ? 1.0f : 0.0f;
     }
     m = wave_max(m);
-    if (__any(nan)) m = NAN;
+    if (wave_sum(bad) != 0.0f) m = NAN;
     const float mm = m == -INFINITY ? 0.0f : m;
     float l = 0.0f, o0 = 0.0f, o1 = 0.0f;
-    for (int y = 0; y < a.splits; ++y) {
-        const float x = a.part_lse[y * stride + id];
-        if (x == -INFINITY) continue;                        // a run in which nothing is seen holds zeros
-        const float w = exp2_fast((x - mm) * LOG2E);
-        const float* o = a.part_o + (y * stride + id) * a.dim;
+    for (int y0 = 0; y0 < a.splits; y0 += 64) {
+        const float x = y0 + lane < a.splits ? a.part_lse[(y0 + lane) * stride + id] : -INFINITY;
+        const float w = x == -INFINITY ? 0.0f : exp2_fast((x - mm) * LOG2E);
         l += w;
-        if (lane < a.dim) o0 = fmaf(w, o[lane], o0);
-        if (lane + 64 < a.dim) o1 = fmaf(w, o[lane + 64], o1);
+        uint64_t todo = __ballot(x != -INFINITY);
+        while (todo) {
+            int y[4];
+            float wy[4], p0[4], p1[4];
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {                    // four loads in flight; the last run again where there are fewer
+                y[n] = todo ? __ffsll((unsigned long long)todo) - 1 : y[n ? n - 1 : 0];
+                wy[n] = todo ? __shfl(w, y[n]) : 0.0f;
+                todo &= todo - 1;
+                const float* o = a.part_o + ((y0 + y[n]) * stride + id) * a.dim;
+                p0[n] = lane < a.dim ? o[lane] : 0.0f;
+                p1[n] = lane + 64 < a.dim ? o[lane + 64] : 0.0f;
+            }
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+                if (wy[n] != 0.0f || n == 0) {
+                    o0 = fmaf(wy[n], p0[n], o0);
+                    o1 = fmaf(wy[n], p1[n], o1);
+                }
+        }
     }
+    l = wave_sum(l);
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     const int64_t row = a.row0 + id / a.heads;
     const int h = (int)(id % a.heads);

@@ -14,6 +14,7 @@ struct drl_seq_layout {
     int device = 0;
     SeqRows rows;
     int64_t n_q = 0, n_k = 0;         // rows that belong to a series
+    int64_t q_first = 0;
     int max_q = 0, max_k = 0;
     seq::SegInfo* segs = nullptr;     // device, n_seg + 1 entries
 };
@@ -87,6 +88,7 @@ int drl_seq_layout_create(drl_ctx* c, const int64_t* qo, const int64_t* ko, int 
         l->rows.n_seg = n_seg;
         l->rows.q_end = qo[n_seg];
         l->rows.k_end = ko[n_seg];
+        l->q_first = qo[0];
         l->n_q = qo[n_seg] - qo[0];
         l->n_k = ko[n_seg] - ko[0];
         std::vector<int> order(n_seg);
@@ -137,52 +139,105 @@ static int attn_prepare(drl_ctx* c, const drl_seq_layout* l, const drl_seq_call*
     return seq_check_attention(e, &l->rows, call, a);
 }
 
+// How a call is cut: rows into tiles, and, where these do not fill the GPU, the keys into runs.
+struct AttnPlan {
+    bool tiled, few;
+    int blocks, rep_b, per, splits, chunk;
+    int64_t tiles, workspace;
+};
+static AttnPlan attn_plan(const DrlCtxView& v, const drl_seq_layout* l, const drl_seq_call* call, const drl_attn_args* a) {
+    AttnPlan p = {};
+    const int rep = a->n_heads / a->n_kv_heads, rows = 128;
+    p.tiled = call->dtype != DRL_F32;
+    p.blocks = (rep + rows - 1) / rows;
+    p.rep_b = (rep + p.blocks - 1) / p.blocks;
+    p.per = rows / p.rep_b;
+    p.few = (int64_t)std::min(l->max_q, p.per) * p.rep_b <= 32;
+    p.tiles = (l->n_q / p.per + l->rows.n_seg) * (int64_t)(a->n_kv_heads * p.blocks);
+    p.splits = 1;
+    // keys one tile can see; runs of at least 256 of them, for 8 workgroups per CU (two are resident at a time: series
+    // of different lengths then still end together)
+    const int64_t most = a->window > 0 && a->causal ? std::min<int64_t>(l->max_k, (int64_t)a->window + p.per) : l->max_k;
+    if (p.tiled && most > 512 && p.tiles < 2 * v.n_cu) {
+        const int64_t want = (8 * v.n_cu + p.tiles - 1) / p.tiles;
+        const int64_t chunk = std::max<int64_t>(256, ((most + want - 1) / want + 63) / 64 * 64);
+        p.splits = (int)((most + chunk - 1) / chunk);
+        p.chunk = (int)chunk;
+    }
+    if (p.splits > 1) p.workspace = (int64_t)p.splits * l->n_q * a->n_heads * (a->dim + 1) * 4;
+    return p;
+}
+
 int drl_attention_workspace(drl_ctx* c, const drl_seq_layout* l, const drl_seq_call* call, const drl_attn_args* a, int64_t* bytes) {
     if (!c || !bytes) return DRL_ERR_ARG;
     SeqError e;
     if (attn_prepare(c, l, call, a, e)) return fail(c, e);
-    *bytes = 0;
+    *bytes = attn_plan(drl_ctx_view(c), l, call, a).workspace;
     return DRL_OK;
 }
 
+}  // extern "C"
+
+template <typename T>
+static void attn_tiles(const AttnPlan& p, const seq::AttnArgs& k, hipStream_t st) {
+    const int dt = (k.dim + 31) / 32;
+    const size_t shmem = 4 * 64 * 2 * (dt == 1 ? 32 : dt == 2 ? 64 : 128);
+    const dim3 grid((unsigned)p.tiles, p.splits);
+    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), shmem, st, k); };
+    if (p.few) {
+        if (dt == 1) go(seq::attn_tile_kernel<T, 1, true>);
+        else if (dt == 2) go(seq::attn_tile_kernel<T, 2, true>);
+        else if (dt == 3) go(seq::attn_tile_kernel<T, 3, true>);
+        else go(seq::attn_tile_kernel<T, 4, true>);
+    } else {
+        if (dt == 1) go(seq::attn_tile_kernel<T, 1, false>);
+        else if (dt == 2) go(seq::attn_tile_kernel<T, 2, false>);
+        else if (dt == 3) go(seq::attn_tile_kernel<T, 3, false>);
+        else go(seq::attn_tile_kernel<T, 4, false>);
+    }
+    if (p.splits > 1) {
+        const dim3 jg((unsigned)((k.part_rows * k.heads + 3) / 4));
+        hipLaunchKernelGGL((seq::attn_join_kernel<T>), jg, dim3(256), 0, st, k);
+    }
+}
+
+extern "C" {
+
 int drl_attention_dev(drl_ctx* c, const drl_seq_layout* l, const drl_seq_call* call, const drl_attn_args* a) {
+    const char* who = "drl_attention_dev";
     if (!c) return DRL_ERR_ARG;
     SeqError e;
     if (attn_prepare(c, l, call, a, e)) return fail(c, e);
     if (l->n_q == 0) return DRL_OK;
     const DrlCtxView v = drl_ctx_view(c);
+    const AttnPlan p = attn_plan(v, l, call, a);
+    if (p.tiles > 0x7fffffff || l->n_q * a->n_heads > ((int64_t)1 << 32)) { e.set(DRL_ERR_UNSUPPORTED, "%s: too many rows and heads", who); return fail(c, e); }
+    if (seq_check_workspace(e, who, call, p.workspace)) return fail(c, e);
     DeviceGuard guard(v.device);
-    if (!guard.ok) return hip_fail(c, "drl_attention_dev", hipErrorInvalidDevice);
+    if (!guard.ok) return hip_fail(c, who, hipErrorInvalidDevice);
     seq::AttnArgs k = {};
     k.q = a->q; k.k = a->k; k.v = a->v; k.out = a->out; k.lse = a->lse; k.key_mask = a->key_mask; k.k_len = a->k_len;
     k.q_row = a->q_row; k.q_head = a->q_head; k.k_row = a->k_row; k.k_head = a->k_head;
     k.v_row = a->v_row; k.v_head = a->v_head; k.o_row = a->o_row; k.o_head = a->o_head;
     k.segs = l->segs; k.n_seg = l->rows.n_seg; k.heads = a->n_heads; k.rep = a->n_heads / a->n_kv_heads; k.dim = a->dim;
     k.causal = a->causal != 0; k.window = a->window; k.scale = a->scale;
-    k.splits = 1;
+    k.kv_blocks = a->n_kv_heads * p.blocks; k.blocks = p.blocks; k.rep_b = p.rep_b; k.per = p.per;
+    k.splits = p.splits; k.chunk = p.chunk;
+    k.part_rows = l->n_q; k.row0 = l->q_first;
+    if (p.splits > 1) {
+        k.part_o = (float*)call->workspace;
+        k.part_lse = k.part_o + (int64_t)p.splits * l->n_q * a->n_heads * a->dim;
+    }
     const hipStream_t st = stream_of(v, call);
     by_type(call->dtype, [&](auto* t) {
         typedef std::remove_pointer_t<decltype(t)> T;
-        if constexpr (sizeof(T) == 2) {
-            constexpr int BM = 128;
-            k.blocks = (k.rep + BM - 1) / BM;
-            k.rep_b = (k.rep + k.blocks - 1) / k.blocks;
-            k.kv_blocks = a->n_kv_heads * k.blocks;
-            k.per = BM / k.rep_b;
-            const int64_t tiles = (l->n_q / k.per + l->rows.n_seg) * k.kv_blocks;
-            const int dt = (a->dim + 31) / 32;
-            const size_t shmem = 4 * 64 * 2 * (dt == 1 ? 32 : dt == 2 ? 64 : 128);
-            const dim3 grid((unsigned)tiles);
-            if (dt == 1) hipLaunchKernelGGL((seq::attn_tile_kernel<T, 1>), grid, dim3(256), shmem, st, k);
-            else if (dt == 2) hipLaunchKernelGGL((seq::attn_tile_kernel<T, 2>), grid, dim3(256), shmem, st, k);
-            else if (dt == 3) hipLaunchKernelGGL((seq::attn_tile_kernel<T, 3>), grid, dim3(256), shmem, st, k);
-            else hipLaunchKernelGGL((seq::attn_tile_kernel<T, 4>), grid, dim3(256), shmem, st, k);
-        } else {
+        if constexpr (sizeof(T) == 2) attn_tiles<T>(p, k, st);
+        else {
             const dim3 grid((unsigned)(l->n_q / 4 + l->rows.n_seg), a->n_heads);
             hipLaunchKernelGGL((seq::attn_rows_kernel<T>), grid, dim3(256), 0, st, k);
         }
     });
-    return launched(c, "drl_attention_dev");
+    return launched(c, who);
 }
 
 // ---- linear attention ---------------------------------------------------------------------------------------------
