@@ -32,6 +32,9 @@ struct SegInfo {
     int32_t pad;
 };
 
+// A value that is the same in all lanes, into a scalar register.
+__device__ __forceinline__ float uniform(float x) { return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x))); }
+
 __device__ __forceinline__ float wave_max(float x) {
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) x = fmaxf(x, __shfl_xor(x, m));

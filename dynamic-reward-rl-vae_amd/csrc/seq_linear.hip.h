@@ -1,4 +1,9 @@
-// Linear attention with a decaying state.
+// Linear attention with a decaying state:  S <- lam S + k_t v_t^T,  out_t = scale S^T q_t,  lam = exp(d_h).
+//
+// Whole series go in chunks of C = 32 rows.  With S the state before a chunk, i and j rows of it, n its rows,
+//   out_i = scale ( lam^(i+1) S^T q_i  +  sum_{j <= i} lam^(i-j) (q_i.k_j) v_j )
+//   S'    = lam^n S + sum_j k_j (lam^(n-1-j) v_j)^T
+// four matrix products, with no power of lam above 1.
 #pragma once
 #include "seq_common.hip.h"
 
@@ -15,15 +20,40 @@ struct LinearArgs {
     int n_seg;
     int heads, rep, dk, dv;
     float scale;
+    // a series is cut into pieces of `piece` rows (a multiple of the chunk); unit u is a piece, states[u] the state
+    // before it, [heads, dk, dv] (NULL: the series are whole)
+    int piece, blocks;            // blocks: workgroups per head, over the values' width
+    float* states;
 };
 
-// d_h of the definition: a NaN stays one.
+// log2 of a head's decay per row: a growth is taken as none, a NaN stays one.
 __device__ __forceinline__ float decay_log(const LinearArgs& a, int h) {
     const float d = a.log_decay[h];
     return d > 0.0f ? 0.0f : d;
 }
+__device__ __forceinline__ float power(float ld2, int n) { return n == 0 ? 1.0f : exp2_fast(ld2 * (float)n); }
 
-// Row after row, the state's columns in registers: thread (kk, c) holds S[kk*KP .. , c] of one column c.
+struct LinearUnit {
+    SegInfo s;
+    int64_t u;
+    int first, rows;              // rows of the series in this piece
+    bool any, last;
+};
+__device__ __forceinline__ LinearUnit linear_unit(const LinearArgs& a, int64_t u) {
+    LinearUnit t;
+    t.u = u;
+    const int slot = find_seg(a.segs, a.n_seg, u, a.piece);
+    t.s = a.segs[slot];
+    const int k = (int)(u - (t.s.cum / a.piece + slot));
+    const int n = max(1, (int)(((int64_t)t.s.nq + a.piece - 1) / a.piece));
+    t.any = k < n;
+    t.last = k == n - 1;
+    t.first = k * a.piece;
+    t.rows = min(a.piece, t.s.nq - t.first);
+    return t;
+}
+
+// One step of n series, or the definition over whole ones: row after row, the state's columns in registers.
 template <typename T>
 __global__ __launch_bounds__(256) void linear_rows_kernel(LinearArgs a) {
     constexpr int KP = 32;                       // dk <= 128: four threads share a column
@@ -67,6 +97,323 @@ __global__ __launch_bounds__(256) void linear_rows_kernel(LinearArgs a) {
             const int kr = kk * KP + r;
             if (col && kr < a.dk) a.state_out[sb + (int64_t)kr * a.dv + c] = S[r];
         }
+}
+
+// 2^-e with |x| 2^-e in [2^13, 2^14), for scaling into float16's range; 1 for 0 and what is not finite.
+__device__ __forceinline__ float into_range(float x, float& back) {
+    const int e = x > 0.0f && x < INFINITY ? __builtin_amdgcn_frexp_expf(x) - 14 : 0;
+    back = __builtin_amdgcn_ldexpf(1.0f, e);
+    return __builtin_amdgcn_ldexpf(1.0f, -e);
+}
+
+// 16-bit types.  A wave keeps the state's columns of 32 value dimensions in registers, as the accumulator of the state's
+// product: rows of the key width along the registers, value dimension along the lanes.  Rounded to 16 bits it is, register
+// by register, the second operand of the product with q (the inner index may be taken in any order; q is read from LDS
+// in that order, and with it k for the scores).  Scores are computed transposed, which makes them the first operand of the
+// product with v.  k and v go through LDS once and are read as they are for the scores and transposed (ds_read_b64_tr_b16)
+// for the state.
+// Rounding: scores and the state's copy are rounded to the inputs' type (relative error eps/2, like the result's own);
+// the float32 state itself takes lam^(n-1-j) v_j as the sum of N parts of that type (24 bits of bfloat16 in three, 22 of
+// float16 in two), and loses nothing from call to call.  float16 has no range to spare: scores, state columns and
+// weighted values are scaled by powers of two before they are rounded.
+template <typename T, int KT, int NW, bool STATE>
+__global__ __launch_bounds__(NW * 64, 2) void linear_chunk_kernel(LinearArgs a) {
+    typedef typename Vec<T>::x8 x8;
+    typedef typename Vec<T>::x4 x4;
+    typedef short s16x8 __attribute__((ext_vector_type(8)));
+    constexpr bool F16 = __is_same(T, f16);
+    constexpr int C = 32, N = F16 ? 2 : 3, THREADS = NW * 64;
+    constexpr int DP = KT <= 1 ? 32 : KT <= 2 ? 64 : 128, NC = DP / 8;     // key width of an LDS row, in chunks of 8
+    constexpr int VP = 32 * NW, VC = VP / 8;
+    constexpr int QK = C * DP * 2, VB = C * VP * 2, STAGE = (STATE ? 1 : 2) * QK + VB;
+    constexpr int KL = (C * NC + THREADS - 1) / THREADS, VL = C * VC / THREADS;
+    extern __shared__ char smem[];
+    const uint32_t lds = lds_offset(smem);
+    const int h = blockIdx.x % a.heads, blk = (blockIdx.x / a.heads) % a.blocks;
+    const LinearUnit t = linear_unit(a, blockIdx.x / (a.heads * a.blocks));
+    if (!t.any || (STATE && t.last)) return;
+    const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c0 = blk * VP + wave * 32;                       // this wave's first value dimension
+    const bool on = c0 + col < a.dv;
+    const float ld2 = decay_log(a, h) * LOG2E;
+
+    // the state
+    f32x16 S[KT];
+    const float* from = nullptr;
+    if (!STATE) from = a.states ? a.states + (t.u * a.heads + h) * (int64_t)a.dk * a.dv
+                                : a.state_in ? a.state_in + ((int64_t)t.s.seg * a.heads + h) * (int64_t)a.dk * a.dv : nullptr;
+    const uint32_t lane_s = 4 * half * a.dv + c0 + col;         // state element of a register: a row of the wave's plus the lane's
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) {
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int d = kt * 32 + acc_row(r, 0);
+            S[kt][r] = from && on && d < a.dk ? (from + d * a.dv)[lane_s] : 0.0f;    // dk is a multiple of 8: d + 4 is inside too
+        }
+    }
+
+    const int64_t row0 = t.s.q0 + t.first;
+    const char* qp = (const char*)((const T*)a.q + row0 * a.q_row + (int64_t)h * a.q_head);
+    const char* kp = (const char*)((const T*)a.k + row0 * a.k_row + (int64_t)(h / a.rep) * a.k_head);
+    const char* vp = (const char*)((const T*)a.v + row0 * a.v_row + (int64_t)(h / a.rep) * a.v_head + blk * VP);
+    const int vw = (a.dv - blk * VP) * 2;                      // bytes of values from here on
+    auto stage = [&](int base, int buf) {
+        const uint32_t at = lds + buf * STAGE + wave * 1024;
+#pragma unroll
+        for (int n = 0; n < KL; ++n) {
+            if (C * NC < THREADS && wave * 64 >= C * NC) break;        // a narrow key tile: the first waves load it
+            const int slot = n * THREADS + threadIdx.x, r = slot / NC, c = ((slot % NC) ^ swz<NC>(r)) * 16;
+            const int64_t j = min(base + r, t.rows - 1);
+            const bool in = c < a.dk * 2;
+            load_lds16(in ? (const void*)(kp + j * a.k_row * 2 + c) : (const void*)&zero16, at + n * THREADS * 16);
+            if (!STATE) load_lds16(in ? (const void*)(qp + j * a.q_row * 2 + c) : (const void*)&zero16, at + QK + VB + n * THREADS * 16);
+        }
+#pragma unroll
+        for (int n = 0; n < VL; ++n) {
+            const int slot = n * THREADS + threadIdx.x, r = slot / VC, c = ((slot % VC) ^ swz<VC>(r)) * 16;
+            const int64_t j = min(base + r, t.rows - 1);
+            load_lds16(c < vw ? (const void*)(vp + j * a.v_row * 2 + c) : (const void*)&zero16, at + QK + n * THREADS * 16);
+        }
+    };
+
+    // LDS places: rows in the order of the accumulator's registers (two reads of 4), and transposed
+    const int g = (lane >> 4) & 1, i4 = lane & 15;
+    auto row_at = [&](int s, int j) { return (uint32_t)(col * (DP * 2) + (((2 * s + j) ^ swz<NC>(col)) * 16) + half * 8); };
+    auto tr_at = [&](int width, int sw_c, int r) { return (uint32_t)(r * width * 2 + sw_c * 16 + (i4 & 1) * 8); };
+    uint32_t ktr[KT][2], vtr[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int r = 8 * j + 4 * half + (i4 >> 2), cc = g * 2 + ((i4 & 3) >> 1);
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) ktr[kt][j] = tr_at(DP, (kt * 4 + cc) ^ swz<NC>(r), r);
+        vtr[j] = QK + tr_at(VP, (wave * 4 + cc) ^ swz<VC>(r), r);
+    }
+    auto read_tr = [&](uint32_t a0, uint32_t a1) {
+        return __builtin_bit_cast(x8, (s16x8)__builtin_shufflevector(lds_read_tr(a0), lds_read_tr(a1), 0, 1, 2, 3, 4, 5, 6, 7));
+    };
+    auto read_row = [&](uint32_t base, int s) {
+        const x4 x = lds_read<x4>(base + row_at(s, 0)), y = lds_read<x4>(base + row_at(s, 1));
+        return (x8)__builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+
+    // powers of lam: between a row (lane) and a key (register), of a value's row to the chunk's end, of a row from its start
+    // (the last two are a lane's part times a register's, which is the same for all lanes)
+    float inner[STATE ? 1 : 16], up[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) up[r] = uniform(power(ld2, acc_row(r, 0)));        // lam^0 .. lam^27, and back from 27
+    if constexpr (!STATE)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) inner[r] = col >= acc_row(r, half) ? a.scale * power(ld2, col - acc_row(r, half)) : 0.0f;
+    const float lane_up = a.scale * power(ld2, 4 * half + 1), lane_left = power(ld2, 4 - 4 * half);
+    float fall = expm1f(decay_log(a, h) * (float)C);           // lam^n - 1: lam^n itself, rounded, would drift over many chunks
+
+    T* op = (T*)a.out + row0 * a.o_row + (int64_t)h * a.o_head + c0;
+    if (t.rows > 0) stage(0, 0);
+    int buf = 0;
+    for (int base = 0; base < t.rows; base += C, buf ^= 1) {
+        const int n = min(C, t.rows - base);
+        wait_loads();
+        __syncthreads();
+        if (base + C < t.rows) stage(base + C, buf ^ 1);
+        if (c0 >= a.dv) continue;                              // a wave behind the values' width only loads
+        if (n < C) fall = expm1f(decay_log(a, h) * (float)n);
+        const uint32_t kb = lds + buf * STAGE, qb = kb + QK + VB;
+
+        x8 v[2];
+#pragma unroll
+        for (int s = 0; s < 2; ++s) v[s] = read_tr(kb + vtr[0] + s * 16 * VP * 2, kb + vtr[1] + s * 16 * VP * 2);
+        bool odd = false;
+        {
+            constexpr uint32_t E = F16 ? 0x7c00u : 0x7f80u;
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                const u32x4 w = __builtin_bit_cast(u32x4, v[s]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) odd |= (w[e] & E) == E || ((w[e] >> 16) & E) == E;
+            }
+        }
+        if (__any(odd)) {
+            // a value that is not finite: no row before its own may meet it, not even with weight 0.  Row after row.
+            const float lam = exp2_fast(ld2);
+            int hf = half;
+#pragma unroll 1
+            for (int j = 0; j < n; ++j) {
+                asm volatile("" : "+v"(hf));                   // 64 places per lane: not to be kept over the whole loop
+
+                const uint32_t vo = kb + QK + j * VP * 2 + (((wave * 4 + (col >> 3)) ^ swz<VC>(j)) * 16) + (col & 7) * 2;
+                const float vc = (float)lds_read<T>(vo);
+                float acc = 0.0f;
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        if (r % 4 == 0) __builtin_amdgcn_sched_barrier(0);
+                        const int d = kt * 32 + acc_row(r, hf);
+                        const uint32_t at = j * DP * 2 + (((d >> 3) ^ swz<NC>(j)) * 16) + (d & 7) * 2;
+                        S[kt][r] = fmaf((float)lds_read<T>(kb + at), vc, lam * S[kt][r]);
+                        if (kt * 32 + acc_row(r, 0) >= a.dk) S[kt][r] = 0.0f;
+                        if constexpr (!STATE) acc = fmaf((float)lds_read<T>(qb + at), S[kt][r], acc);
+                    }
+                if constexpr (!STATE) {
+                    acc = pair_sum(acc) * a.scale;
+                    if (on && half == 0) op[(int64_t)(base + j) * a.o_row + col] = (T)acc;
+                }
+            }
+            continue;
+        }
+
+        if constexpr (!STATE) {
+            f32x16 z, o;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) z[r] = o[r] = 0.0f;
+            float s_scale = 1.0f, s_back = 1.0f;
+            if constexpr (F16) {
+                float m = 0.0f;
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) m = fmaxf(m, fabsf(S[kt][r]));
+                s_scale = into_range(pair_max(m), s_back);
+            }
+#pragma unroll
+            for (int s = 0; s < 2 * KT; ++s) {
+                if (s % 2 == 0) __builtin_amdgcn_sched_barrier(0);     // two steps' reads in flight, no more: registers
+                const x8 q = read_row(qb, s), k = read_row(kb, s);
+                z = mfma(k, q, z);
+                x8 b;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) b[e] = (T)(F16 ? S[s >> 1][8 * (s & 1) + e] * s_scale : S[s >> 1][8 * (s & 1) + e]);
+                o = mfma(q, b, o);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            float p[16];
+            int apart = col - 4 * half;
+            asm volatile("" : "+v"(apart));                    // compared here: 16 lane masks are more than there are registers for
+#pragma unroll
+            for (int r = 0; r < 16; ++r) p[r] = apart >= acc_row(r, 0) ? z[r] * inner[r] : 0.0f;
+            float p_scale = 1.0f, p_back = 1.0f;
+            f32x16 w = o;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[r] *= F16 ? lane_up * up[r] * s_back : lane_up * up[r];
+            if constexpr (F16) {
+                float m = 0.0f;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    m = fmaxf(m, fabsf(p[r]));
+                    w[r] = 0.0f;
+                }
+                p_scale = into_range(wave_max(m), p_back);
+            } else w = o;
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                x8 b;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) b[e] = (T)(F16 ? p[8 * s + e] * p_scale : p[8 * s + e]);
+                w = mfma(b, v[s], w);
+            }
+            if constexpr (F16)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) w[r] = fmaf(w[r], p_back, o[r]);
+            // rows of 64 bytes through this wave's corner of LDS, then 16 bytes per lane
+            const uint32_t ob = lds + 2 * STAGE + wave * (C * 64);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) lds_write<T>(ob + acc_row(r, half) * 64 + col * 2, (T)w[r]);
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+                const int j = m * 16 + (lane >> 2);
+                const u32x4 y = lds_read<u32x4>(ob + m * 1024 + lane * 16);
+                if (j < n && c0 + (lane & 3) * 8 < a.dv) *(u32x4*)(op + (int64_t)(base + j) * a.o_row + (lane & 3) * 8) = y;
+            }
+        }
+
+        __builtin_amdgcn_sched_barrier(0);
+        float x[16], v_scale = 1.0f, v_back = 1.0f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[e] = (float)v[e >> 3][e & 7];
+        if (n == C) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[e] *= lane_left * up[15 - e];             // 31 - row = (4 - 4 half) + (27 - the register's part)
+        } else {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int j = acc_row(e, half);
+                x[e] = j < n ? x[e] * power(ld2, n - 1 - j) : 0.0f;
+            }
+        }
+        if constexpr (F16) {
+            float m = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) m = fmaxf(m, fabsf(x[e]));
+            v_scale = into_range(pair_max(m), v_back);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[e] *= v_scale;
+        }
+        x8 y[2][N];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            float r = x[e];
+#pragma unroll
+            for (int m = 0; m < N; ++m) {
+                y[e >> 3][m][e & 7] = (T)r;
+                r -= (float)y[e >> 3][m][e & 7];
+            }
+        }
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) {
+            __builtin_amdgcn_sched_barrier(0);
+            f32x16 acc;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                S[kt][r] = fmaf(S[kt][r], fall, S[kt][r]);
+                acc[r] = F16 ? 0.0f : S[kt][r];
+            }
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                const x8 k = read_tr(kb + ktr[kt][0] + s * 16 * DP * 2, kb + ktr[kt][1] + s * 16 * DP * 2);
+#pragma unroll
+                for (int m = 0; m < N; ++m) acc = mfma(k, y[s][m], acc);
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) S[kt][r] = F16 ? fmaf(acc[r], v_back, S[kt][r]) : acc[r];
+        }
+    }
+
+    float* to = nullptr;
+    if (STATE) to = a.states + ((t.u + 1) * a.heads + h) * (int64_t)a.dk * a.dv;       // the next piece's unit
+    else if (t.last && a.state_out) to = a.state_out + ((int64_t)t.s.seg * a.heads + h) * (int64_t)a.dk * a.dv;
+    if (to && on)
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int d = kt * 32 + acc_row(r, 0);
+                if (d < a.dk) (to + d * a.dv)[lane_s] = S[kt][r];
+            }
+}
+
+// The states before each piece: a unit holds what its predecessor added, from a state of 0.
+static __global__ __launch_bounds__(256) void linear_scan_kernel(LinearArgs a) {
+    const int slot = blockIdx.x, h = blockIdx.y;
+    const int64_t size = (int64_t)a.dk * a.dv, e = ((int64_t)blockIdx.z * 256 + threadIdx.x) * 4;
+    if (e >= size) return;
+    const SegInfo s = a.segs[slot];
+    const int n = max(1, (int)(((int64_t)s.nq + a.piece - 1) / a.piece));
+    const float fall = expm1f(decay_log(a, h) * (float)a.piece);
+    f32x4 S = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (a.state_in) S = *(const f32x4*)(a.state_in + ((int64_t)s.seg * a.heads + h) * size + e);
+    float* at = a.states + ((s.cum / a.piece + slot) * a.heads + h) * size + e;
+    const int64_t next = a.heads * size;
+    *(f32x4*)at = S;
+    f32x4 add = n > 1 ? *(const f32x4*)(at + next) : S;
+    for (int k = 1; k < n; ++k) {
+        at += next;
+        const f32x4 mine = add;
+        if (k + 1 < n) add = *(const f32x4*)(at + next);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) S[c] = fmaf(S[c], fall, S[c]) + mine[c];
+        *(f32x4*)at = S;
+    }
 }
 
 }  // namespace seq

@@ -242,19 +242,82 @@ int drl_attention_dev(drl_ctx* c, const drl_seq_layout* l, const drl_seq_call* c
 
 // ---- linear attention ---------------------------------------------------------------------------------------------
 
+// How a call is cut: value widths into workgroups, and, where series and heads do not fill the GPU, the rows into pieces.
+struct LinearPlan {
+    bool chunked;
+    int waves, blocks, piece;
+    int64_t units, workspace;
+};
+static LinearPlan linear_plan(const DrlCtxView& v, const drl_seq_layout* l, const drl_seq_call* call, const drl_linear_args* a) {
+    LinearPlan p = {};
+    p.chunked = call->dtype != DRL_F32;
+    const int tiles = (a->dim_v + 31) / 32;
+    p.waves = tiles <= 2 ? 2 : 4;
+    p.blocks = (tiles + p.waves - 1) / p.waves;
+    p.piece = 0x7fffffff;
+    p.units = l->rows.n_seg;
+    // Pieces cost a second reading of k and v and the states between them: only where workgroups are fewer than two per
+    // CU, and then as many as make that, of 256 rows at least.
+    const int64_t groups = (int64_t)a->n_heads * p.blocks, want = 2 * v.n_cu;
+    if (p.chunked && groups * l->rows.n_seg < want && l->max_q > 512) {
+        const int64_t rows = l->n_q * groups / want;
+        p.piece = (int)std::max<int64_t>(256, (rows + 31) / 32 * 32);
+        if (p.piece >= l->max_q) p.piece = 0x7fffffff;
+        else {
+            p.units = l->n_q / p.piece + l->rows.n_seg;
+            p.workspace = p.units * a->n_heads * a->dim_k * a->dim_v * 4;
+        }
+    }
+    return p;
+}
+
 int drl_linear_attention_workspace(drl_ctx* c, const drl_seq_layout* l, const drl_seq_call* call, const drl_linear_args* a, int64_t* bytes) {
     if (!c || !bytes) return DRL_ERR_ARG;
     SeqError e;
     if (check_layout(e, "drl_linear_attention_dev", drl_ctx_view(c), l) ||
         seq_check_linear(e, "drl_linear_attention_dev", l->rows.q_end, call, a, false)) return fail(c, e);
-    *bytes = 0;
+    *bytes = linear_plan(drl_ctx_view(c), l, call, a).workspace;
     return DRL_OK;
 }
 
 static seq::LinearArgs linear_args(const drl_linear_args* a, const seq::SegInfo* segs, int n_seg) {
-    return {a->q, a->k, a->v, a->out, a->log_decay, a->state_in, a->state_out, a->q_row, a->q_head, a->k_row, a->k_head,
-            a->v_row, a->v_head, a->o_row, a->o_head, segs, n_seg, a->n_heads, a->n_heads / a->n_kv_heads, a->dim_k, a->dim_v, a->scale};
+    seq::LinearArgs k = {};
+    k.q = a->q; k.k = a->k; k.v = a->v; k.out = a->out; k.log_decay = a->log_decay; k.state_in = a->state_in; k.state_out = a->state_out;
+    k.q_row = a->q_row; k.q_head = a->q_head; k.k_row = a->k_row; k.k_head = a->k_head;
+    k.v_row = a->v_row; k.v_head = a->v_head; k.o_row = a->o_row; k.o_head = a->o_head;
+    k.segs = segs; k.n_seg = n_seg; k.heads = a->n_heads; k.rep = a->n_heads / a->n_kv_heads; k.dk = a->dim_k; k.dv = a->dim_v;
+    k.scale = a->scale;
+    return k;
 }
+
+}  // extern "C"
+
+template <typename T, int KT, int NW>
+static void linear_chunks(const LinearPlan& p, const seq::LinearArgs& k, hipStream_t st) {
+    constexpr int DP = KT <= 1 ? 32 : KT <= 2 ? 64 : 128;
+    constexpr size_t qk = 32 * DP * 2, vb = 32 * 32 * NW * 2;
+    const dim3 grid((unsigned)(p.units * k.heads * p.blocks));
+    if (k.states) {
+        hipLaunchKernelGGL((seq::linear_chunk_kernel<T, KT, NW, true>), grid, dim3(NW * 64), 2 * (qk + vb), st, k);
+        const dim3 sg(k.n_seg, k.heads, (k.dk * k.dv / 4 + 255) / 256);
+        hipLaunchKernelGGL(seq::linear_scan_kernel, sg, dim3(256), 0, st, k);
+    }
+    hipLaunchKernelGGL((seq::linear_chunk_kernel<T, KT, NW, false>), grid, dim3(NW * 64), 2 * (2 * qk + vb) + NW * 2048, st, k);
+}
+
+template <typename T>
+static void linear_series(const LinearPlan& p, const seq::LinearArgs& k, hipStream_t st) {
+    auto by_waves = [&](auto kt) {
+        constexpr int KT = decltype(kt)::value;
+        if (p.waves == 2) linear_chunks<T, KT, 2>(p, k, st);
+        else linear_chunks<T, KT, 4>(p, k, st);
+    };
+    if (k.dk <= 32) by_waves(std::integral_constant<int, 1>());
+    else if (k.dk <= 64) by_waves(std::integral_constant<int, 2>());
+    else by_waves(std::integral_constant<int, 4>());
+}
+
+extern "C" {
 
 int drl_linear_attention_dev(drl_ctx* c, const drl_seq_layout* l, const drl_seq_call* call, const drl_linear_args* a) {
     const char* who = "drl_linear_attention_dev";
@@ -263,13 +326,23 @@ int drl_linear_attention_dev(drl_ctx* c, const drl_seq_layout* l, const drl_seq_
     const DrlCtxView v = drl_ctx_view(c);
     if (check_layout(e, who, v, l) || seq_check_linear(e, who, l->rows.q_end, call, a, false)) return fail(c, e);
     if (l->rows.n_seg == 0) return DRL_OK;
+    const LinearPlan p = linear_plan(v, l, call, a);
+    if (p.units * a->n_heads * p.blocks > 0x7fffffff) { e.set(DRL_ERR_UNSUPPORTED, "%s: too many series and heads", who); return fail(c, e); }
+    if (seq_check_workspace(e, who, call, p.workspace)) return fail(c, e);
     DeviceGuard guard(v.device);
     if (!guard.ok) return hip_fail(c, who, hipErrorInvalidDevice);
-    const seq::LinearArgs k = linear_args(a, l->segs, l->rows.n_seg);
+    seq::LinearArgs k = linear_args(a, l->segs, l->rows.n_seg);
+    k.piece = p.piece;
+    k.blocks = p.blocks;
+    if (p.workspace) k.states = (float*)call->workspace;
+    const hipStream_t st = stream_of(v, call);
     by_type(call->dtype, [&](auto* t) {
         typedef std::remove_pointer_t<decltype(t)> T;
-        const dim3 grid(l->rows.n_seg, a->n_heads, (a->dim_v + 63) / 64);
-        hipLaunchKernelGGL((seq::linear_rows_kernel<T>), grid, dim3(256), 0, stream_of(v, call), k);
+        if constexpr (sizeof(T) == 2) linear_series<T>(p, k, st);
+        else {
+            const dim3 grid(l->rows.n_seg, a->n_heads, (a->dim_v + 63) / 64);
+            hipLaunchKernelGGL((seq::linear_rows_kernel<T>), grid, dim3(256), 0, st, k);
+        }
     });
     return launched(c, who);
 }

@@ -242,16 +242,22 @@ def log_decay(gen, H, kind="memory"):
     return torch.tensor(([0.0, -math.inf, 0.7, -0.01, -30.0] * H)[:H]).cuda()
 
 
-def check_linear(sc, dt, q, k, v, ld, o, state=None, scale=None, **kw):
-    scale = q.shape[2] ** -0.5 if scale is None else scale
-    out, final = sc.linear_attention(q, k, v, ld, sc.seq_layout(o), scale=scale, state=state, **kw)
-    torch.cuda.synchronize()
+def linear_bounds(dt, q, k, v, ld, o, scale, state=None):
+    """(out, its tolerance, last states, their tolerance) from the definition."""
     want, S, oa, sa = orc.linear_attention(q, k, v, ld, o, scale=scale, state=state)
     T = max([0] + [b - a for a, b in zip(o, o[1:])])
     E = (q.shape[2] + 512 + T / 64) * U
     u = half(dt)
-    within(out, want, (3 * (u if dt != "f32" else 0) + E) * oa + u * want.abs() + torch.finfo(DT[dt]).tiny, "out")
-    within(final, S, E * sa + 1e-37, "final state")
+    return want, (3 * (u if dt != "f32" else 0) + E) * oa + u * want.abs() + torch.finfo(DT[dt]).tiny, S, E * sa + 1e-37
+
+
+def check_linear(sc, dt, q, k, v, ld, o, state=None, scale=None, **kw):
+    scale = q.shape[2] ** -0.5 if scale is None else scale
+    out, final = sc.linear_attention(q, k, v, ld, sc.seq_layout(o), scale=scale, state=state, **kw)
+    torch.cuda.synchronize()
+    want, tol, S, stol = linear_bounds(dt, q, k, v, ld, o, scale, state)
+    within(out, want, tol, "out")
+    within(final, S, stol, "final state")
     return out, final
 
 
@@ -325,16 +331,22 @@ def test_linear_values_that_are_not_finite_reach_only_what_follows(sc, dt, what)
     o = offs([150, 100])
     q, k, v = (normal(g, (250, 2, 32), dt) for _ in range(3))
     ld = log_decay(g, 2)
-    clean, cs = sc.linear_attention(q, k, v, ld, sc.seq_layout(o))
+    clean, tol, cs, stol = linear_bounds(dt, q, k, v, ld, o, 32 ** -0.5)
     for at, value in ((75, float("nan")), (97, float("inf"))):
         y = {"q": q, "k": k, "v": v}[what].clone()
         y[at, 0, 3] = value
         args = {"q": q, "k": k, "v": v, what: y}
         out, state = sc.linear_attention(args["q"], args["k"], args["v"], ld, sc.seq_layout(o))
-        assert torch.equal(out[:at], clean[:at]) and torch.equal(out[150:], clean[150:]) and torch.equal(out[:, 1], clean[:, 1])
-        assert torch.equal(state[1], cs[1]) and torch.equal(state[:, 1], cs[:, 1])
+        # what comes before, or belongs to another series or head, is what it is without the value, each within its
+        # bound: it may have been summed in another order
+        free = torch.ones(250, 2, dtype=torch.bool)
+        free[at:at + 1 if what == "q" else 150, 0] = False
+        within(out[free.cuda()], clean[free], tol[free], f"{what} {at} {value}")
+        within(state[1], cs[1], stol[1], "state of the other series")
+        within(state[:, 1], cs[:, 1], stol[:, 1], "state of the other head")
         if what == "q":
-            assert not torch.isfinite(out[at, 0].float()).any() and torch.equal(out[at + 1:], clean[at + 1:]) and torch.equal(state, cs)
+            assert not torch.isfinite(out[at, 0].float()).any()
+            within(state, cs, stol, "state")
         else:
             hit = state[0, 0, :, 3] if what == "v" else state[0, 0, 3]
             assert not torch.isfinite(hit).any()
