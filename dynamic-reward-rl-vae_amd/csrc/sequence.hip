@@ -372,13 +372,82 @@ static int norm_prepare(drl_ctx* c, const drl_seq_layout* l, int64_t rows, const
     return seq_check_norm(e, l ? l->rows.q_end : rows, call, a);
 }
 
+// How a call is cut: packs of channels, and rows into units.
+struct NormPlan {
+    int pack, lanes, count, slice, slices, piece;
+    int64_t units, blocks, workspace;
+};
+static NormPlan norm_plan(const DrlCtxView& v, const drl_seq_layout* l, int64_t rows, const drl_seq_call* call, const drl_norm_args* a) {
+    NormPlan p = {};
+    const int size = call->dtype == DRL_F32 ? 4 : 2, cg = a->channels / a->groups;
+    // the widest pack that a group is made of and that everything is aligned to
+    for (p.pack = 16 / size; p.pack > 1; p.pack /= 2) {
+        const int64_t bytes = p.pack * size;
+        if (cg % p.pack == 0 && (uintptr_t)a->x % bytes == 0 && (uintptr_t)a->y % bytes == 0 && a->x_row % p.pack == 0 && a->y_row % p.pack == 0) break;
+    }
+    const int packs = cg / p.pack;
+    p.lanes = 1;
+    if (!l) {
+        // two packs per lane hide more latency than one and still leave a group's lanes side by side in memory
+        while (p.lanes < 64 && p.lanes * 2 < packs) p.lanes *= 2;
+        p.count = (packs + p.lanes - 1) / p.lanes;
+        const int per_wave = 64 / p.lanes;
+        const int64_t sets = (a->groups + per_wave - 1) / per_wave;
+        // waves: a multiple of the sets and of four; eight workgroups per CU, or one row each where that is fewer
+        const int64_t want = std::min<int64_t>(rows * sets, (int64_t)8 * 4 * v.n_cu);
+        const int64_t unit = sets % 4 == 0 ? sets : sets % 2 == 0 ? sets * 2 : sets * 4;
+        p.blocks = std::max<int64_t>(1, (want + unit - 1) / unit) * unit / 4;
+        return p;
+    }
+    p.slice = std::max(1, std::min(a->groups, 256 / std::min(packs, 256)));
+    p.slices = (a->groups + p.slice - 1) / p.slice;
+    const int share = std::min(packs, 256), rl = 256 / std::min(p.slice * packs, 256);
+    while (p.lanes < 64 && p.lanes < share * rl) p.lanes *= 2;
+    // four workgroups per CU, of at least 8 rows per thread, at most 256 units to a series (each of which reads the
+    // moments of all)
+    const int64_t fill = (l->n_q * p.slices + 4 * v.n_cu - 1) / (4 * v.n_cu);
+    p.piece = (int)std::max({fill, (int64_t)8 * rl, (int64_t)(l->max_q + 255) / 256});
+    p.units = l->n_q / p.piece + l->rows.n_seg;
+    if (l->max_q > p.piece) p.workspace = p.units * a->groups * 2 * 4;
+    return p;
+}
+
 int drl_group_norm_workspace(drl_ctx* c, const drl_seq_layout* l, int64_t rows, const drl_seq_call* call, const drl_norm_args* a, int64_t* bytes) {
     if (!c || !bytes) return DRL_ERR_ARG;
     SeqError e;
     if (norm_prepare(c, l, rows, call, a, e)) return fail(c, e);
-    *bytes = 0;
+    *bytes = norm_plan(drl_ctx_view(c), l, rows, call, a).workspace;
     return DRL_OK;
 }
+
+}  // extern "C"
+
+template <typename T, int V>
+static void norm_launch(const NormPlan& p, const seq::NormArgs& k, hipStream_t st) {
+    auto go = [&](auto kernel, dim3 grid) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, k); };
+    if (k.segs) {
+        const dim3 grid((unsigned)p.units, p.slices);
+        if (k.part) go(seq::norm_series_kernel<T, V, true>, grid);
+        go(seq::norm_series_kernel<T, V, false>, grid);
+        return;
+    }
+    const dim3 grid((unsigned)p.blocks);
+    if (p.count <= 1) go(seq::norm_rows_kernel<T, V, 1>, grid);
+    else if (p.count <= 2) go(seq::norm_rows_kernel<T, V, 2>, grid);
+    else if (p.count <= 4) go(seq::norm_rows_kernel<T, V, 4>, grid);
+    else go(seq::norm_rows_kernel<T, V, 0>, grid);
+}
+
+template <typename T>
+static void norm_packs(const NormPlan& p, const seq::NormArgs& k, hipStream_t st) {
+    if constexpr (sizeof(T) == 2)
+        if (p.pack == 8) return norm_launch<T, 8>(p, k, st);
+    if (p.pack == 4) norm_launch<T, 4>(p, k, st);
+    else if (p.pack == 2) norm_launch<T, 2>(p, k, st);
+    else norm_launch<T, 1>(p, k, st);
+}
+
+extern "C" {
 
 int drl_group_norm_dev(drl_ctx* c, const drl_seq_layout* l, int64_t rows, const drl_seq_call* call, const drl_norm_args* a) {
     const char* who = "drl_group_norm_dev";
@@ -387,14 +456,18 @@ int drl_group_norm_dev(drl_ctx* c, const drl_seq_layout* l, int64_t rows, const 
     if (norm_prepare(c, l, rows, call, a, e)) return fail(c, e);
     if ((l ? l->n_q : rows) == 0) return DRL_OK;
     const DrlCtxView v = drl_ctx_view(c);
+    const NormPlan p = norm_plan(v, l, rows, call, a);
+    if (seq_check_workspace(e, who, call, p.workspace)) return fail(c, e);
     DeviceGuard guard(v.device);
     if (!guard.ok) return hip_fail(c, who, hipErrorInvalidDevice);
-    const seq::NormArgs k = {a->x, a->y, a->gamma, a->beta, a->x_row, a->y_row, l ? l->segs : nullptr, a->channels, a->groups, a->act, a->eps};
-    by_type(call->dtype, [&](auto* t) {
-        typedef std::remove_pointer_t<decltype(t)> T;
-        const dim3 grid((unsigned)(l ? l->rows.n_seg : rows), a->groups);
-        hipLaunchKernelGGL((seq::norm_group_kernel<T>), grid, dim3(256), 0, stream_of(v, call), k);
-    });
+    seq::NormArgs k = {};
+    k.x = a->x; k.y = a->y; k.gamma = a->gamma; k.beta = a->beta; k.x_row = a->x_row; k.y_row = a->y_row; k.rows = rows;
+    k.segs = l ? l->segs : nullptr; k.n_seg = l ? l->rows.n_seg : 0;
+    k.channels = a->channels; k.groups = a->groups; k.act = a->act; k.eps = a->eps;
+    k.lanes = p.lanes; k.piece = p.piece; k.slice = p.slice;
+    if (p.workspace) k.part = (float*)call->workspace;
+    const hipStream_t st = stream_of(v, call);
+    by_type(call->dtype, [&](auto* t) { norm_packs<std::remove_pointer_t<decltype(t)>>(p, k, st); });
     return launched(c, who);
 }
 
