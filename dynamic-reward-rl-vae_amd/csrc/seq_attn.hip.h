@@ -132,6 +132,38 @@ __device__ __forceinline__ AttnTile attn_tile(const AttnArgs& a, int64_t id) {
     return t;
 }
 
+// A wave's rows: o and l as they were summed, m the reference in natural units.
+template <typename T, int DT>
+__device__ __forceinline__ void attn_store(const AttnArgs& a, const AttnTile& t, const f32x16 (&o)[DT], float l, float m, int i, int h, bool row_ok, int half) {
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;           // a NaN sum stays one
+    const float lse = log_sum(m, l);
+    if (!row_ok) return;
+    const int64_t row = t.s.q0 + i;
+    if (a.splits > 1) {
+        const int64_t at = ((int64_t)blockIdx.y * a.part_rows + row - a.row0) * a.heads + h;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const int d = dt * 32 + acc_row(r, half);
+                if (d < a.dim) *(f32x4*)(a.part_o + at * a.dim + d) = f32x4{o[dt][r] * inv, o[dt][r + 1] * inv, o[dt][r + 2] * inv, o[dt][r + 3] * inv};
+            }
+        if (half == 0) a.part_lse[at] = lse;
+        return;
+    }
+    T* out = (T*)a.out + row * a.o_row + (int64_t)h * a.o_head;
+    struct alignas(4 * sizeof(T)) Four { T e[4]; };
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+            const int d = dt * 32 + acc_row(r, half);
+            const Four w = {{(T)(o[dt][r] * inv), (T)(o[dt][r + 1] * inv), (T)(o[dt][r + 2] * inv), (T)(o[dt][r + 3] * inv)}};
+            if (d < a.dim) *(Four*)(out + d) = w;
+        }
+    if (a.lse && half == 0) a.lse[row * a.heads + h] = lse;
+}
+
 // 16-bit types.  A workgroup of four waves has 128 rows, a wave 32 of them; keys and values go through LDS in tiles of 64
 // keys, two of them in turn (64 KiB at dim 128: two workgroups per CU, one wave of each per SIMD, so that one's softmax
 // runs beside the other's products).
@@ -336,33 +368,150 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
         return;
     }
 
-    const float l = pair_sum(l0 + l1);
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;           // a NaN sum stays one
-    const float lse = log_sum(mc * LN2, l);
-    if (!row_ok) return;
-    const int64_t row = t.s.q0 + i;
+    attn_store<T, DT>(a, t, o, pair_sum(l0 + l1), mc * LN2, i, h, row_ok, half);
+}
+
+// float32.  The same on 32x32x2 products, with tiles of 32 keys: the matrix pipe is 16 times slower, and what it does takes
+// most of the time.  Here a score register is at once an operand of values^T x weights, and nothing is rounded.
+template <int DT>
+__global__ __launch_bounds__(256, 2) void attn_tile32_kernel(AttnArgs a) {
+    constexpr int DP = DT <= 1 ? 32 : DT <= 2 ? 64 : 128, NC = DP / 4, KS = 4 * DT, BK = 32;
+    constexpr int TILE = BK * DP * 4, LOADS = BK * NC / 256;
+    extern __shared__ char smem[];
+    const uint32_t lds = lds_offset(smem);
+    const AttnTile t = attn_tile(a, blockIdx.x);
+    if (!t.any) return;
+    const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int pr = wave * 32 + col;
+    const bool row_ok = pr < t.rows;
+    const int prc = row_ok ? pr : t.rows - 1;
+    const int i = t.i0 + prc / t.n_heads, h = t.head0 + prc % t.n_heads;
+    int lo, hi, LO, HI, all_lo, all_hi;
+    visible(a, i, t.s.nq, t.nk, lo, hi);
+    visible(a, t.i0, t.s.nq, t.nk, LO, all_hi);
+    visible(a, t.i0 + (t.rows - 1) / t.n_heads, t.s.nq, t.nk, all_lo, HI);
     if (a.splits > 1) {
-        const int64_t at = ((int64_t)blockIdx.y * a.part_rows + row - a.row0) * a.heads + h;
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-            for (int r = 0; r < 16; r += 4) {
-                const int d = dt * 32 + acc_row(r, half);
-                if (d < a.dim) *(f32x4*)(a.part_o + at * a.dim + d) = f32x4{o[dt][r] * inv, o[dt][r + 1] * inv, o[dt][r + 2] * inv, o[dt][r + 3] * inv};
-            }
-        if (half == 0) a.part_lse[at] = lse;
-        return;
+        LO += (int)min((int64_t)blockIdx.y * a.chunk, (int64_t)0x3fffffff);
+        HI = min(HI, LO + a.chunk);
     }
-    T* out = (T*)a.out + row * a.o_row + (int64_t)h * a.o_head;
+    const int wl = __builtin_amdgcn_readfirstlane(__shfl(lo, 0)), wh = __builtin_amdgcn_readfirstlane(__shfl(hi, 31));
+
+    f32x4 qf[KS];                            // elements 8 s + 4 half .. of this lane's row
+    {
+        const float* q = (const float*)a.q + (t.s.q0 + i) * a.q_row + (int64_t)h * a.q_head;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const int d = 8 * s + 4 * half;
+            qf[s] = d < a.dim ? *(const f32x4*)(q + d) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+    }
+    const char* kp = (const char*)((const float*)a.k + t.s.k0 * a.k_row + (int64_t)t.kv * a.k_head);
+    const char* vp = (const char*)((const float*)a.v + t.s.k0 * a.v_row + (int64_t)t.kv * a.v_head);
+    const int64_t kr = a.k_row * 4, vr = a.v_row * 4;
+    int srow[LOADS], schunk[LOADS];
+#pragma unroll
+    for (int n = 0; n < LOADS; ++n) {
+        const int slot = n * 256 + threadIdx.x;
+        srow[n] = slot / NC;
+        schunk[n] = ((slot % NC) ^ swz32<NC>(srow[n])) * 16;
+        if (schunk[n] >= a.dim * 4) schunk[n] = -1;
+    }
+    auto stage = [&](int base, int buf) {
+        const uint32_t at = lds + buf * 2 * TILE + wave * 1024;
+#pragma unroll
+        for (int n = 0; n < LOADS; ++n) {
+            const int j = min(base + srow[n], t.nk - 1);
+            load_lds16(schunk[n] >= 0 ? (const void*)(kp + j * kr + schunk[n]) : (const void*)&zero16, at + n * 4096);
+            load_lds16(schunk[n] >= 0 ? (const void*)(vp + j * vr + schunk[n]) : (const void*)&zero16, at + TILE + n * 4096);
+        }
+    };
+    const float c1 = a.scale * LOG2E;
+    float ref = -INFINITY, mc = 0.0f, l = 0.0f;
+    f32x16 o[DT];
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-        for (int r = 0; r < 16; r += 4) {
-            const int d = dt * 32 + acc_row(r, half);
-            const x4 w = {(T)(o[dt][r] * inv), (T)(o[dt][r + 1] * inv), (T)(o[dt][r + 2] * inv), (T)(o[dt][r + 3] * inv)};
-            if (d < a.dim) *(x4*)(out + d) = w;
+        for (int r = 0; r < 16; ++r) o[dt][r] = 0.0f;
+
+    bool strange = false;
+    if (LO < HI) stage(LO, 0);
+    int buf = 0;
+    for (int base = LO; base < HI; base += BK, buf ^= 1) {
+        wait_loads();
+        __syncthreads();
+        if (base + BK < HI) stage(base + BK, buf ^ 1);
+        const uint32_t kt_ = lds + buf * 2 * TILE, vt_ = kt_ + TILE;
+        uint32_t there = ~0u;
+        const bool edge = a.key_mask || base < all_lo || base + BK > all_hi;
+        if (edge) {
+            const int j = base + col;
+            there = (uint32_t)__ballot(j < HI && (!a.key_mask || a.key_mask[t.s.k0 + j]));
+            int odd = 0;
+#pragma unroll
+            for (int n = 0; n < LOADS; ++n) {
+                const uint32_t at = vt_ + (n * 256 + threadIdx.x) * 16;
+                if (!((there >> srow[n]) & 1)) lds_write<u32x4>(at, u32x4{0, 0, 0, 0});
+                else {
+                    const u32x4 x = lds_read<u32x4>(at);
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) odd |= (x[w] & 0x7f800000u) == 0x7f800000u;
+                }
+            }
+            if (__syncthreads_or(odd)) { strange = true; break; }
         }
-    if (a.lse && half == 0) a.lse[row * a.heads + h] = lse;
+        if (base >= wh || base + BK <= wl || wave * 32 >= t.rows) continue;
+
+        f32x16 z;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) z[r] = 0.0f;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const f32x4 k = lds_read<f32x4>(kt_ + col * (DP * 4) + (((2 * s + half) ^ swz32<NC>(col)) * 16));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) z = mfma(k[e], qf[s][e], z);
+        }
+        if (edge) {
+            const int from = max(lo - base, 0), to = min(hi - base, 32);
+            const uint32_t see = (to <= from ? 0 : there & (~0u << from) & (~0u >> (32 - to))) >> (4 * half);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) z[r] = (see >> acc_row(r, 0)) & 1 ? z[r] : -INFINITY;
+        }
+        float m = z[0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r) m = fmaxf(m, z[r]);
+        m = pair_max(m);
+        if (__any((m - ref) * c1 > 8.0f)) {
+            const float now = fmaxf(m, ref);
+            const float mcn = now == -INFINITY ? 0.0f : now * c1;
+            const float f = ref == -INFINITY ? 0.0f : exp2_fast(mc - mcn);
+            ref = now;
+            mc = mcn;
+            l *= f;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[dt][r] *= f;
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            z[r] = exp2_fast(fmaf(z[r], c1, -mc));
+            l += z[r];
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int row = acc_row(r, half);
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+                o[dt] = mfma(lds_read<float>(vt_ + row * (DP * 4) + (((dt * 8 + (col >> 2)) ^ swz32<NC>(row)) * 16) + (col & 3) * 4), z[r], o[dt]);
+        }
+    }
+    if (strange) {
+        wait_loads();
+        for (int r = wave; r < t.rows; r += 4)
+            attn_row<float>(a, t.s, t.nk, t.i0 + r / t.n_heads, t.head0 + r % t.n_heads, LO, HI, blockIdx.y);
+        return;
+    }
+    attn_store<float, DT>(a, t, o, pair_sum(l), mc * LN2, i, h, row_ok, half);
 }
 
 // Joins the runs of keys of a row and head: weights exp(lse_y - max), one wave each.  A run in which nothing is seen
@@ -416,17 +565,6 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
     if (lane < a.dim) out[lane] = (T)(o0 * inv);
     if (lane + 64 < a.dim) out[lane + 64] = (T)(o1 * inv);
     if (a.lse && lane == 0) a.lse[row * a.heads + h] = log_sum(mm, l);
-}
-
-// The definition, a wave per row and head.
-template <typename T>
-__global__ __launch_bounds__(256) void attn_rows_kernel(AttnArgs a) {
-    const int64_t t = (int64_t)blockIdx.x;
-    const int slot = find_seg(a.segs, a.n_seg, t, 4);
-    const SegInfo s = a.segs[slot];
-    const int i = (int)(t - (s.cum / 4 + slot)) * 4 + (int)(threadIdx.x >> 6);
-    if (i >= s.nq) return;
-    attn_row<T>(a, s, keys_of(a, s), i, blockIdx.y, 0, 0x7fffffff, 0);
 }
 
 }  // namespace seq

@@ -74,6 +74,13 @@ __device__ __forceinline__ int swz(int r) {
     else return ((r & 3) << 2) | ((r >> 2) & 3);
 }
 
+// The same for float32, chunks of 4: reads of one chunk of 16 consecutive rows.
+template <int NC>
+__device__ __forceinline__ int swz32(int r) {
+    if constexpr (NC == 8) return (r >> 1) & 7;
+    else return r & 15;
+}
+
 typedef __attribute__((address_space(3))) char lds_char;
 __device__ __forceinline__ uint32_t lds_offset(const void* p) { return (uint32_t)(uintptr_t)(lds_char*)p; }
 
@@ -110,6 +117,8 @@ __device__ __forceinline__ float pair_sum(float x) {
 // column l & 31, rows (r & 3) + 8 (r >> 2) + 4 (l >> 5) in registers r = 0 .. 15.
 __device__ __forceinline__ f32x16 mfma(Vec<bf16>::x8 a, Vec<bf16>::x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f32x16 mfma(Vec<f16>::x8 a, Vec<f16>::x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+// 32x32x2 product: one element of the inner axis per lane half.
+__device__ __forceinline__ f32x16 mfma(float a, float b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ int acc_row(int r, int half) { return (r & 3) + 8 * (r >> 2) + 4 * half; }
 
 // Sixteen bytes of zeros: where lanes load from whose chunk lies behind a row's end.

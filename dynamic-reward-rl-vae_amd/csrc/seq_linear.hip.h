@@ -53,50 +53,65 @@ __device__ __forceinline__ LinearUnit linear_unit(const LinearArgs& a, int64_t u
     return t;
 }
 
-// One step of n series, or the definition over whole ones: row after row, the state's columns in registers.
+// One row of each of n series.  Bound by reading and writing the states once, 8 bytes per element: a wave has 4 columns per
+// lane of as many state rows as fit side by side (64 lanes over dv / 4 quads), a workgroup all dk rows of a column block
+// of one series and head, and joins what the rows add to the output through LDS.
 template <typename T>
-__global__ __launch_bounds__(256) void linear_rows_kernel(LinearArgs a) {
-    constexpr int KP = 32;                       // dk <= 128: four threads share a column
-    __shared__ float part[4][64];
-    SegInfo s = {(int64_t)blockIdx.x, 0, 0, 1, 1, (int)blockIdx.x, 0};       // a step: one row each
-    if (a.segs) s = a.segs[blockIdx.x];
-    const int h = blockIdx.y, c = blockIdx.z * 64 + (threadIdx.x & 63), kk = threadIdx.x >> 6;
-    const bool col = c < a.dv;
-    const float lam = exp2_fast(decay_log(a, h) * LOG2E);
-    const int64_t sb = ((int64_t)s.seg * a.heads + h) * a.dk * a.dv;
-    float S[KP];
-#pragma unroll
-    for (int r = 0; r < KP; ++r) {
-        const int kr = kk * KP + r;
-        S[r] = a.state_in && col && kr < a.dk ? a.state_in[sb + (int64_t)kr * a.dv + c] : 0.0f;
+__global__ __launch_bounds__(256) void linear_step_kernel(LinearArgs a) {
+    __shared__ float part[4 * 256];
+    __shared__ float kq[2][128];
+    const int h = blockIdx.x % a.heads;
+    const int64_t row = blockIdx.x / a.heads;
+    const int quads = a.dv / 4, across = min(quads, 64);               // lanes of a workgroup row: quads of columns
+    const int down = 256 / across;                                     // state rows at a time
+    const int x = threadIdx.x % across, y = threadIdx.x / across;
+    const bool on = y < down;
+    if (threadIdx.x < a.dk) {
+        kq[0][threadIdx.x] = (float)((const T*)a.k + row * a.k_row + (int64_t)(h / a.rep) * a.k_head)[threadIdx.x];
+        kq[1][threadIdx.x] = (float)((const T*)a.q + row * a.q_row + (int64_t)h * a.q_head)[threadIdx.x];
     }
-    const T* q = (const T*)a.q + (int64_t)h * a.q_head;
-    const T* k = (const T*)a.k + (int64_t)(h / a.rep) * a.k_head;
-    const T* v = (const T*)a.v + (int64_t)(h / a.rep) * a.v_head;
-    T* o = (T*)a.out + (int64_t)h * a.o_head;
-    for (int t = 0; t < s.nq; ++t) {
-        const int64_t row = s.q0 + t;
-        const float vc = col ? (float)v[row * a.v_row + c] : 0.0f;
-        float acc = 0.0f;
+    const T* v = (const T*)a.v + row * a.v_row + (int64_t)(h / a.rep) * a.v_head + x * 4;
+    f32x4 vc = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (on)
 #pragma unroll
-        for (int r = 0; r < KP; ++r) {
-            const int kr = kk * KP + r;
-            if (kr < a.dk) {
-                S[r] = fmaf((float)k[row * a.k_row + kr], vc, lam * S[r]);
-                acc = fmaf((float)q[row * a.q_row + kr], S[r], acc);
+        for (int e = 0; e < 4; ++e) vc[e] = (float)v[e];
+    const float lam = exp2_fast(decay_log(a, h) * LOG2E);
+    const int64_t sb = (row * a.heads + h) * (int64_t)a.dk * a.dv + x * 4;
+    const float* in = a.state_in + sb;
+    float* out = a.state_out + sb;
+    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    __syncthreads();
+    if (on) {
+        constexpr int U = 8;                                           // rows in flight
+        for (int r0 = y; r0 < a.dk; r0 += U * down) {
+            f32x4 S[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int r = r0 + u * down;
+                if (r < a.dk) S[u] = *(const f32x4*)(in + (int64_t)r * a.dv);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int r = r0 + u * down;
+                if (r < a.dk) {
+                    const float kk = kq[0][r], qq = kq[1][r];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        S[u][e] = fmaf(kk, vc[e], lam * S[u][e]);
+                        acc[e] = fmaf(qq, S[u][e], acc[e]);
+                    }
+                    *(f32x4*)(out + (int64_t)r * a.dv) = S[u];
+                }
             }
         }
-        part[kk][threadIdx.x & 63] = acc;
-        __syncthreads();
-        if (kk == 0 && col) o[row * a.o_row + c] = (T)((part[0][threadIdx.x] + part[1][threadIdx.x] + part[2][threadIdx.x] + part[3][threadIdx.x]) * a.scale);
-        __syncthreads();
     }
-    if (a.state_out)
-#pragma unroll
-        for (int r = 0; r < KP; ++r) {
-            const int kr = kk * KP + r;
-            if (col && kr < a.dk) a.state_out[sb + (int64_t)kr * a.dv + c] = S[r];
-        }
+    if (on) *(f32x4*)&part[(y * across + x) * 4] = acc;
+    __syncthreads();
+    if (threadIdx.x < a.dv) {
+        float s = 0.0f;
+        for (int i = 0; i < down; ++i) s += part[i * across * 4 + threadIdx.x];
+        ((T*)a.out + row * a.o_row + (int64_t)h * a.o_head)[threadIdx.x] = (T)(s * a.scale);
+    }
 }
 
 // 2^-e with |x| 2^-e in [2^13, 2^14), for scaling into float16's range; 1 for 0 and what is not finite.
@@ -381,6 +396,169 @@ __global__ __launch_bounds__(NW * 64, 2) void linear_chunk_kernel(LinearArgs a) 
 
     float* to = nullptr;
     if (STATE) to = a.states + ((t.u + 1) * a.heads + h) * (int64_t)a.dk * a.dv;       // the next piece's unit
+    else if (t.last && a.state_out) to = a.state_out + ((int64_t)t.s.seg * a.heads + h) * (int64_t)a.dk * a.dv;
+    if (to && on)
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int d = kt * 32 + acc_row(r, 0);
+                if (d < a.dk) (to + d * a.dv)[lane_s] = S[kt][r];
+            }
+}
+
+// float32: the same on 32x32x2 products; a register of the state or of the scores is an operand as it is, and nothing is
+// rounded or split.
+template <int KT, int NW, bool STATE>
+__global__ __launch_bounds__(NW * 64) void linear_chunk32_kernel(LinearArgs a) {
+    constexpr int C = 32, THREADS = NW * 64;
+    constexpr int DP = KT <= 1 ? 32 : KT <= 2 ? 64 : 128, NC = DP / 4;
+    constexpr int VP = 32 * NW, VC = VP / 4;
+    constexpr int QK = C * DP * 4, VB = C * VP * 4, STAGE = (STATE ? 1 : 2) * QK + VB;
+    constexpr int KL = C * NC / THREADS, VL = C * VC / THREADS;
+    static_assert(KL >= 1 && VL >= 1, "a load per thread at least");
+    extern __shared__ char smem[];
+    const uint32_t lds = lds_offset(smem);
+    const int h = blockIdx.x % a.heads, blk = (blockIdx.x / a.heads) % a.blocks;
+    const LinearUnit t = linear_unit(a, blockIdx.x / (a.heads * a.blocks));
+    if (!t.any || (STATE && t.last)) return;
+    const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c0 = blk * VP + wave * 32;
+    const bool on = c0 + col < a.dv;
+    const float ld2 = decay_log(a, h) * LOG2E;
+    f32x16 S[KT];
+    const float* from = nullptr;
+    if (!STATE) from = a.states ? a.states + (t.u * a.heads + h) * (int64_t)a.dk * a.dv
+                                : a.state_in ? a.state_in + ((int64_t)t.s.seg * a.heads + h) * (int64_t)a.dk * a.dv : nullptr;
+    const uint32_t lane_s = 4 * half * a.dv + c0 + col;
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int d = kt * 32 + acc_row(r, 0);
+            S[kt][r] = from && on && d < a.dk ? (from + d * a.dv)[lane_s] : 0.0f;
+        }
+    const int64_t row0 = t.s.q0 + t.first;
+    const char* qp = (const char*)((const float*)a.q + row0 * a.q_row + (int64_t)h * a.q_head);
+    const char* kp = (const char*)((const float*)a.k + row0 * a.k_row + (int64_t)(h / a.rep) * a.k_head);
+    const char* vp = (const char*)((const float*)a.v + row0 * a.v_row + (int64_t)(h / a.rep) * a.v_head + blk * VP);
+    const int vw = (a.dv - blk * VP) * 4;
+    auto stage = [&](int base, int buf) {
+        const uint32_t at = lds + buf * STAGE + wave * 1024;
+#pragma unroll
+        for (int n = 0; n < KL; ++n) {
+            const int slot = n * THREADS + threadIdx.x, r = slot / NC, c = ((slot % NC) ^ swz32<NC>(r)) * 16;
+            const int64_t j = min(base + r, t.rows - 1);
+            const bool in = c < a.dk * 4;
+            load_lds16(in ? (const void*)(kp + j * a.k_row * 4 + c) : (const void*)&zero16, at + n * THREADS * 16);
+            if (!STATE) load_lds16(in ? (const void*)(qp + j * a.q_row * 4 + c) : (const void*)&zero16, at + QK + VB + n * THREADS * 16);
+        }
+#pragma unroll
+        for (int n = 0; n < VL; ++n) {
+            const int slot = n * THREADS + threadIdx.x, r = slot / VC, c = ((slot % VC) ^ swz32<VC>(r)) * 16;
+            const int64_t j = min(base + r, t.rows - 1);
+            load_lds16(c < vw ? (const void*)(vp + j * a.v_row * 4 + c) : (const void*)&zero16, at + QK + n * THREADS * 16);
+        }
+    };
+    float up[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) up[r] = uniform(power(ld2, acc_row(r, 0)));
+    const float lane_up = a.scale * power(ld2, 4 * half + 1), lane_left = power(ld2, 4 - 4 * half);
+    float fall = expm1f(decay_log(a, h) * (float)C);
+    float* op = (float*)a.out + row0 * a.o_row + (int64_t)h * a.o_head;
+    if (t.rows > 0) stage(0, 0);
+    int buf = 0;
+    for (int base = 0; base < t.rows; base += C, buf ^= 1) {
+        const int n = min(C, t.rows - base);
+        wait_loads();
+        __syncthreads();
+        if (base + C < t.rows) stage(base + C, buf ^ 1);
+        if (c0 >= a.dv) continue;
+        if (n < C) fall = expm1f(decay_log(a, h) * (float)n);
+        const uint32_t kb = lds + buf * STAGE, vb = kb + QK, qb = vb + VB;
+        float v[16];
+        bool odd = false;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int j = acc_row(r, half);
+            v[r] = lds_read<float>(vb + j * VP * 4 + (((wave * 8 + (col >> 2)) ^ swz32<VC>(j)) * 16) + (col & 3) * 4);
+            odd |= !(fabsf(v[r]) < INFINITY);
+        }
+        if (__any(odd)) {
+            // a value that is not finite: row after row, as for the 16-bit types
+            const float lam = exp2_fast(ld2);
+            int hf = half;
+#pragma unroll 1
+            for (int j = 0; j < n; ++j) {
+                asm volatile("" : "+v"(hf));
+                const float vc = lds_read<float>(vb + j * VP * 4 + (((wave * 8 + (col >> 2)) ^ swz32<VC>(j)) * 16) + (col & 3) * 4);
+                float acc = 0.0f;
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        if (r % 4 == 0) __builtin_amdgcn_sched_barrier(0);
+                        const int d = kt * 32 + acc_row(r, hf);
+                        const uint32_t at = j * DP * 4 + (((d >> 2) ^ swz32<NC>(j)) * 16) + (d & 3) * 4;
+                        S[kt][r] = fmaf(lds_read<float>(kb + at), vc, lam * S[kt][r]);
+                        if (kt * 32 + acc_row(r, 0) >= a.dk) S[kt][r] = 0.0f;
+                        if constexpr (!STATE) acc = fmaf(lds_read<float>(qb + at), S[kt][r], acc);
+                    }
+                if constexpr (!STATE) {
+                    acc = pair_sum(acc) * a.scale;
+                    if (on && half == 0) op[(int64_t)(base + j) * a.o_row + c0 + col] = acc;
+                }
+            }
+            continue;
+        }
+        if constexpr (!STATE) {
+            f32x16 z, o;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) z[r] = o[r] = 0.0f;
+#pragma unroll
+            for (int s = 0; s < 4 * KT; ++s) {
+                const uint32_t at = col * (DP * 4) + (((2 * s + half) ^ swz32<NC>(col)) * 16);
+                const f32x4 q = lds_read<f32x4>(qb + at), k = lds_read<f32x4>(kb + at);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    z = mfma(k[e], q[e], z);
+                    o = mfma(q[e], S[s >> 2][4 * (s & 3) + e], o);
+                }
+            }
+            int apart = col - 4 * half;
+            asm volatile("" : "+v"(apart));
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[r] *= lane_up * up[r];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int d = apart - acc_row(r, 0);
+                o = mfma(d >= 0 ? z[r] * a.scale * power(ld2, d) : 0.0f, v[r], o);
+            }
+            if (on)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int j = acc_row(r, half);
+                    if (j < n) op[(int64_t)(base + j) * a.o_row + c0 + col] = o[r];
+                }
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int j = acc_row(r, half);
+            v[r] *= n == C ? lane_left * up[15 - r] : j < n ? power(ld2, n - 1 - j) : 0.0f;
+        }
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) S[kt][r] = fmaf(S[kt][r], fall, S[kt][r]);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int j = acc_row(r, half);
+                S[kt] = mfma(lds_read<float>(kb + j * DP * 4 + (((kt * 8 + (col >> 2)) ^ swz32<NC>(j)) * 16) + (col & 3) * 4), v[r], S[kt]);
+            }
+        }
+    }
+    float* to = nullptr;
+    if (STATE) to = a.states + ((t.u + 1) * a.heads + h) * (int64_t)a.dk * a.dv;
     else if (t.last && a.state_out) to = a.state_out + ((int64_t)t.s.seg * a.heads + h) * (int64_t)a.dk * a.dv;
     if (to && on)
 #pragma unroll

@@ -27,7 +27,7 @@ __device__ __forceinline__ float activate(float x, int act) {
     if (act == 1) return x < 0.0f ? 0.0f : x;                       // a NaN stays one
     if (act == 0) return x;
     const float s = __builtin_amdgcn_rcpf(1.0f + exp2_fast(-LOG2E * x));
-    return act == 2 ? s : (x == -INFINITY ? x * 0.0f : x * s);
+    return act == 2 ? s : x * s;
 }
 
 template <typename T, int V> struct alignas(V * sizeof(T)) Pack { T e[V]; };

@@ -141,14 +141,13 @@ static int attn_prepare(drl_ctx* c, const drl_seq_layout* l, const drl_seq_call*
 
 // How a call is cut: rows into tiles, and, where these do not fill the GPU, the keys into runs.
 struct AttnPlan {
-    bool tiled, few;
+    bool few;
     int blocks, rep_b, per, splits, chunk;
     int64_t tiles, workspace;
 };
 static AttnPlan attn_plan(const DrlCtxView& v, const drl_seq_layout* l, const drl_seq_call* call, const drl_attn_args* a) {
     AttnPlan p = {};
     const int rep = a->n_heads / a->n_kv_heads, rows = 128;
-    p.tiled = call->dtype != DRL_F32;
     p.blocks = (rep + rows - 1) / rows;
     p.rep_b = (rep + p.blocks - 1) / p.blocks;
     p.per = rows / p.rep_b;
@@ -158,7 +157,7 @@ static AttnPlan attn_plan(const DrlCtxView& v, const drl_seq_layout* l, const dr
     // keys one tile can see; runs of at least 256 of them, for 8 workgroups per CU (two are resident at a time: series
     // of different lengths then still end together)
     const int64_t most = a->window > 0 && a->causal ? std::min<int64_t>(l->max_k, (int64_t)a->window + p.per) : l->max_k;
-    if (p.tiled && most > 512 && p.tiles < 2 * v.n_cu) {
+    if (most > 512 && p.tiles < 2 * v.n_cu) {
         const int64_t want = (8 * v.n_cu + p.tiles - 1) / p.tiles;
         const int64_t chunk = std::max<int64_t>(256, ((most + want - 1) / want + 63) / 64 * 64);
         p.splits = (int)((most + chunk - 1) / chunk);
@@ -178,23 +177,27 @@ int drl_attention_workspace(drl_ctx* c, const drl_seq_layout* l, const drl_seq_c
 
 }  // extern "C"
 
+// Runs f with the constant n, 1 .. 4.
+template <typename F>
+static void by_count(int n, F f) {
+    if (n == 1) f(std::integral_constant<int, 1>());
+    else if (n == 2) f(std::integral_constant<int, 2>());
+    else if (n == 3) f(std::integral_constant<int, 3>());
+    else f(std::integral_constant<int, 4>());
+}
+
 template <typename T>
 static void attn_tiles(const AttnPlan& p, const seq::AttnArgs& k, hipStream_t st) {
     const int dt = (k.dim + 31) / 32;
-    const size_t shmem = 4 * 64 * 2 * (dt == 1 ? 32 : dt == 2 ? 64 : 128);
+    const size_t shmem = 4 * 128 * 64 * (dt == 1 ? 1 : dt == 2 ? 2 : 4) / 2;      // two tiles of keys and of values
     const dim3 grid((unsigned)p.tiles, p.splits);
     auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), shmem, st, k); };
-    if (p.few) {
-        if (dt == 1) go(seq::attn_tile_kernel<T, 1, true>);
-        else if (dt == 2) go(seq::attn_tile_kernel<T, 2, true>);
-        else if (dt == 3) go(seq::attn_tile_kernel<T, 3, true>);
-        else go(seq::attn_tile_kernel<T, 4, true>);
-    } else {
-        if (dt == 1) go(seq::attn_tile_kernel<T, 1, false>);
-        else if (dt == 2) go(seq::attn_tile_kernel<T, 2, false>);
-        else if (dt == 3) go(seq::attn_tile_kernel<T, 3, false>);
-        else go(seq::attn_tile_kernel<T, 4, false>);
-    }
+    by_count(dt, [&](auto d) {
+        constexpr int DT = decltype(d)::value;
+        if constexpr (sizeof(T) == 4) go(seq::attn_tile32_kernel<DT>);
+        else if (p.few) go(seq::attn_tile_kernel<T, DT, true>);
+        else go(seq::attn_tile_kernel<T, DT, false>);
+    });
     if (p.splits > 1) {
         const dim3 jg((unsigned)((k.part_rows * k.heads + 3) / 4));
         hipLaunchKernelGGL((seq::attn_join_kernel<T>), jg, dim3(256), 0, st, k);
@@ -229,14 +232,7 @@ int drl_attention_dev(drl_ctx* c, const drl_seq_layout* l, const drl_seq_call* c
         k.part_lse = k.part_o + (int64_t)p.splits * l->n_q * a->n_heads * a->dim;
     }
     const hipStream_t st = stream_of(v, call);
-    by_type(call->dtype, [&](auto* t) {
-        typedef std::remove_pointer_t<decltype(t)> T;
-        if constexpr (sizeof(T) == 2) attn_tiles<T>(p, k, st);
-        else {
-            const dim3 grid((unsigned)(l->n_q / 4 + l->rows.n_seg), a->n_heads);
-            hipLaunchKernelGGL((seq::attn_rows_kernel<T>), grid, dim3(256), 0, st, k);
-        }
-    });
+    by_type(call->dtype, [&](auto* t) { attn_tiles<std::remove_pointer_t<decltype(t)>>(p, k, st); });
     return launched(c, who);
 }
 
@@ -244,13 +240,11 @@ int drl_attention_dev(drl_ctx* c, const drl_seq_layout* l, const drl_seq_call* c
 
 // How a call is cut: value widths into workgroups, and, where series and heads do not fill the GPU, the rows into pieces.
 struct LinearPlan {
-    bool chunked;
     int waves, blocks, piece;
     int64_t units, workspace;
 };
 static LinearPlan linear_plan(const DrlCtxView& v, const drl_seq_layout* l, const drl_seq_call* call, const drl_linear_args* a) {
     LinearPlan p = {};
-    p.chunked = call->dtype != DRL_F32;
     const int tiles = (a->dim_v + 31) / 32;
     p.waves = tiles <= 2 ? 2 : 4;
     p.blocks = (tiles + p.waves - 1) / p.waves;
@@ -259,7 +253,7 @@ static LinearPlan linear_plan(const DrlCtxView& v, const drl_seq_layout* l, cons
     // Pieces cost a second reading of k and v and the states between them: only where workgroups are fewer than two per
     // CU, and then as many as make that, of 256 rows at least.
     const int64_t groups = (int64_t)a->n_heads * p.blocks, want = 2 * v.n_cu;
-    if (p.chunked && groups * l->rows.n_seg < want && l->max_q > 512) {
+    if (groups * l->rows.n_seg < want && l->max_q > 512) {
         const int64_t rows = l->n_q * groups / want;
         p.piece = (int)std::max<int64_t>(256, (rows + 31) / 32 * 32);
         if (p.piece >= l->max_q) p.piece = 0x7fffffff;
@@ -292,29 +286,39 @@ static seq::LinearArgs linear_args(const drl_linear_args* a, const seq::SegInfo*
 
 }  // extern "C"
 
-template <typename T, int KT, int NW>
+template <typename T, int KT, int NW, bool STATE>
 static void linear_chunks(const LinearPlan& p, const seq::LinearArgs& k, hipStream_t st) {
     constexpr int DP = KT <= 1 ? 32 : KT <= 2 ? 64 : 128;
-    constexpr size_t qk = 32 * DP * 2, vb = 32 * 32 * NW * 2;
+    constexpr int stage = 32 * sizeof(T) * ((STATE ? 1 : 2) * DP + 32 * NW), out = sizeof(T) == 2 && !STATE ? NW * 2048 : 0;
     const dim3 grid((unsigned)(p.units * k.heads * p.blocks));
-    if (k.states) {
-        hipLaunchKernelGGL((seq::linear_chunk_kernel<T, KT, NW, true>), grid, dim3(NW * 64), 2 * (qk + vb), st, k);
-        const dim3 sg(k.n_seg, k.heads, (k.dk * k.dv / 4 + 255) / 256);
-        hipLaunchKernelGGL(seq::linear_scan_kernel, sg, dim3(256), 0, st, k);
-    }
-    hipLaunchKernelGGL((seq::linear_chunk_kernel<T, KT, NW, false>), grid, dim3(NW * 64), 2 * (2 * qk + vb) + NW * 2048, st, k);
+    auto go = [&](auto kernel) {
+        // more LDS than a kernel gets unasked
+        if (2 * stage + out > 64 * 1024) (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 2 * stage + out);
+        hipLaunchKernelGGL(kernel, grid, dim3(NW * 64), 2 * stage + out, st, k);
+    };
+    if constexpr (sizeof(T) == 2) go(seq::linear_chunk_kernel<T, KT, NW, STATE>);
+    else go(seq::linear_chunk32_kernel<KT, NW, STATE>);
 }
 
 template <typename T>
 static void linear_series(const LinearPlan& p, const seq::LinearArgs& k, hipStream_t st) {
-    auto by_waves = [&](auto kt) {
-        constexpr int KT = decltype(kt)::value;
-        if (p.waves == 2) linear_chunks<T, KT, 2>(p, k, st);
-        else linear_chunks<T, KT, 4>(p, k, st);
+    auto all = [&](auto state) {
+        constexpr bool STATE = decltype(state)::value;
+        auto by_waves = [&](auto kt) {
+            constexpr int KT = decltype(kt)::value;
+            if (p.waves == 2) linear_chunks<T, KT, 2, STATE>(p, k, st);
+            else linear_chunks<T, KT, 4, STATE>(p, k, st);
+        };
+        if (k.dk <= 32) by_waves(std::integral_constant<int, 1>());
+        else if (k.dk <= 64) by_waves(std::integral_constant<int, 2>());
+        else by_waves(std::integral_constant<int, 4>());
     };
-    if (k.dk <= 32) by_waves(std::integral_constant<int, 1>());
-    else if (k.dk <= 64) by_waves(std::integral_constant<int, 2>());
-    else by_waves(std::integral_constant<int, 4>());
+    if (k.states) {
+        all(std::true_type());
+        const dim3 grid(k.n_seg, k.heads, (k.dk * k.dv / 4 + 255) / 256);
+        hipLaunchKernelGGL(seq::linear_scan_kernel, grid, dim3(256), 0, st, k);
+    }
+    all(std::false_type());
 }
 
 extern "C" {
@@ -336,14 +340,7 @@ int drl_linear_attention_dev(drl_ctx* c, const drl_seq_layout* l, const drl_seq_
     k.blocks = p.blocks;
     if (p.workspace) k.states = (float*)call->workspace;
     const hipStream_t st = stream_of(v, call);
-    by_type(call->dtype, [&](auto* t) {
-        typedef std::remove_pointer_t<decltype(t)> T;
-        if constexpr (sizeof(T) == 2) linear_series<T>(p, k, st);
-        else {
-            const dim3 grid(l->rows.n_seg, a->n_heads, (a->dim_v + 63) / 64);
-            hipLaunchKernelGGL((seq::linear_rows_kernel<T>), grid, dim3(256), 0, st, k);
-        }
-    });
+    by_type(call->dtype, [&](auto* t) { linear_series<std::remove_pointer_t<decltype(t)>>(p, k, st); });
     return launched(c, who);
 }
 
@@ -353,14 +350,14 @@ int drl_linear_attention_step_dev(drl_ctx* c, int64_t n, const drl_seq_call* cal
     SeqError e;
     if (seq_check_linear(e, who, n, call, a, true)) return fail(c, e);
     if (n == 0) return DRL_OK;
+    if (n * a->n_heads > 0x7fffffff) { e.set(DRL_ERR_UNSUPPORTED, "%s: too many series and heads", who); return fail(c, e); }
     const DrlCtxView v = drl_ctx_view(c);
     DeviceGuard guard(v.device);
     if (!guard.ok) return hip_fail(c, who, hipErrorInvalidDevice);
     const seq::LinearArgs k = linear_args(a, nullptr, 0);
     by_type(call->dtype, [&](auto* t) {
         typedef std::remove_pointer_t<decltype(t)> T;
-        const dim3 grid((unsigned)n, a->n_heads, (a->dim_v + 63) / 64);
-        hipLaunchKernelGGL((seq::linear_rows_kernel<T>), grid, dim3(256), 0, stream_of(v, call), k);
+        hipLaunchKernelGGL((seq::linear_step_kernel<T>), dim3((unsigned)(n * a->n_heads)), dim3(256), 0, stream_of(v, call), k);
     });
     return launched(c, who);
 }
