@@ -134,7 +134,7 @@ __device__ __forceinline__ AttnTile attn_tile(const AttnArgs& a, int64_t id) {
 
 // A wave's rows: o and l as they were summed, m the reference in natural units.
 template <typename T, int DT>
-__device__ __forceinline__ void attn_store(const AttnArgs& a, const AttnTile& t, const f32x16 (&o)[DT], float l, float m, int i, int h, bool row_ok, int half) {
+__device__ __forceinline__ void attn_store(const AttnArgs& a, const AttnTile& t, const f32x16 (&o)[DT], float l, float m, int i, int h, bool row_ok, int half, int first = 0) {
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;           // a NaN sum stays one
     const float lse = log_sum(m, l);
     if (!row_ok) return;
@@ -145,10 +145,10 @@ __device__ __forceinline__ void attn_store(const AttnArgs& a, const AttnTile& t,
         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
             for (int r = 0; r < 16; r += 4) {
-                const int d = dt * 32 + acc_row(r, half);
+                const int d = (first + dt) * 32 + acc_row(r, half);
                 if (d < a.dim) *(f32x4*)(a.part_o + at * a.dim + d) = f32x4{o[dt][r] * inv, o[dt][r + 1] * inv, o[dt][r + 2] * inv, o[dt][r + 3] * inv};
             }
-        if (half == 0) a.part_lse[at] = lse;
+        if (half == 0 && first == 0) a.part_lse[at] = lse;
         return;
     }
     T* out = (T*)a.out + row * a.o_row + (int64_t)h * a.o_head;
@@ -157,11 +157,11 @@ __device__ __forceinline__ void attn_store(const AttnArgs& a, const AttnTile& t,
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
         for (int r = 0; r < 16; r += 4) {
-            const int d = dt * 32 + acc_row(r, half);
+            const int d = (first + dt) * 32 + acc_row(r, half);
             const Four w = {{(T)(o[dt][r] * inv), (T)(o[dt][r + 1] * inv), (T)(o[dt][r + 2] * inv), (T)(o[dt][r + 3] * inv)}};
             if (d < a.dim) *(Four*)(out + d) = w;
         }
-    if (a.lse && half == 0) a.lse[row * a.heads + h] = lse;
+    if (a.lse && half == 0 && first == 0) a.lse[row * a.heads + h] = lse;
 }
 
 // 16-bit types.  A workgroup of four waves has 128 rows, a wave 32 of them; keys and values go through LDS in tiles of 64
@@ -171,9 +171,7 @@ __device__ __forceinline__ void attn_store(const AttnArgs& a, const AttnTile& t,
 // away has the others), the maximum is one exchange away, and the weights, rounded to the inputs' type (relative error
 // u = eps/2 each, as the result's own rounding), are as they lie in registers the second operand of values^T x weights: the
 // order of the keys inside the product is free, and the values are read with ds_read_b64_tr_b16 in the weights' order.
-// FEW: at most 32 rows (steps).  One wave computes, all four load; reading the cache is what takes the time, so what the
-// weights lose by rounding goes into a second product.
-template <typename T, int DT, bool FEW>
+template <typename T, int DT>
 __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
     typedef typename Vec<T>::x8 x8;
     typedef typename Vec<T>::x4 x4;
@@ -286,12 +284,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
             for (int n = 0; n < LOADS; ++n) {
                 const uint32_t at = vt_ + (n * 256 + threadIdx.x) * 16;
                 if (!((there >> srow[n]) & 1)) lds_write<u32x4>(at, u32x4{0, 0, 0, 0});
-                else {
-                    const u32x4 x = lds_read<u32x4>(at);
-                    constexpr uint32_t E = sizeof(T) == 2 && __is_same(T, bf16) ? 0x7f80u : 0x7c00u;
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) odd |= (x[w] & E) == E || ((x[w] >> 16) & E) == E;
-                }
+                else odd |= not_finite<T>(lds_read<u32x4>(at));
             }
             if (__syncthreads_or(odd)) { strange = true; break; }
         }
@@ -333,7 +326,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) o[dt][r] *= f;
         }
-        x8 p[4], p2[FEW ? 4 : 1];
+        x8 p[4];
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
@@ -344,10 +337,6 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
                 const int g = 2 * kt + (r >> 3);
                 p[g][r & 7] = (T)w0;
                 p[g][(r & 7) + 1] = (T)w1;
-                if constexpr (FEW) {
-                    p2[g][r & 7] = (T)(w0 - (float)p[g][r & 7]);
-                    p2[g][(r & 7) + 1] = (T)(w1 - (float)p[g][(r & 7) + 1]);
-                }
             }
 #pragma unroll
         for (int s = 0; s < 4; ++s)
@@ -358,7 +347,6 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
                 typedef short s16x8 __attribute__((ext_vector_type(8)));
                 const s16x8 v = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
                 o[dt] = mfma(__builtin_bit_cast(x8, v), p[s], o[dt]);
-                if constexpr (FEW) o[dt] = mfma(__builtin_bit_cast(x8, v), p2[s], o[dt]);
             }
     }
     if (strange) {
@@ -451,11 +439,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile32_kernel(AttnArgs a) {
             for (int n = 0; n < LOADS; ++n) {
                 const uint32_t at = vt_ + (n * 256 + threadIdx.x) * 16;
                 if (!((there >> srow[n]) & 1)) lds_write<u32x4>(at, u32x4{0, 0, 0, 0});
-                else {
-                    const u32x4 x = lds_read<u32x4>(at);
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) odd |= (x[w] & 0x7f800000u) == 0x7f800000u;
-                }
+                else odd |= not_finite<float>(lds_read<u32x4>(at));
             }
             if (__syncthreads_or(odd)) { strange = true; break; }
         }
@@ -512,6 +496,209 @@ __global__ __launch_bounds__(256, 2) void attn_tile32_kernel(AttnArgs a) {
         return;
     }
     attn_store<float, DT>(a, t, o, pair_sum(l), mc * LN2, i, h, row_ok, half);
+}
+
+// At most 32 rows per kv head (steps).  Reading the cache is what takes the time: every wave has tiles of 32 keys of its own,
+// every NW-th, in two LDS buffers of its own, and waits for nothing but its own loads; at the end the waves' sums are
+// joined through LDS.  With 16-bit types, what the weights lose by rounding goes into a second product: it is free here.
+template <typename T, int DT, int NW>
+__global__ __launch_bounds__(NW * 64) void attn_step_kernel(AttnArgs a) {
+    constexpr bool F32 = sizeof(T) == 4;
+    constexpr int E = 16 / sizeof(T);                          // elements of a chunk
+    constexpr int DP = DT <= 1 ? 32 : DT <= 2 ? 64 : 128, NC = DP / E, KS = F32 ? 4 * DT : 2 * DT, BK = 32;
+    constexpr int ROW = DP * sizeof(T), TILE = BK * ROW, LOADS = BK * NC / 64;
+    extern __shared__ char smem[];
+    const uint32_t lds = lds_offset(smem);
+    const AttnTile t = attn_tile(a, blockIdx.x);
+    if (!t.any) return;
+    const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const bool row_ok = col < t.rows;
+    const int prc = row_ok ? col : t.rows - 1;
+    const int i = t.i0 + prc / t.n_heads, h = t.head0 + prc % t.n_heads;
+    int lo, hi, LO, HI, all_lo, all_hi;
+    visible(a, i, t.s.nq, t.nk, lo, hi);
+    visible(a, t.i0, t.s.nq, t.nk, LO, all_hi);
+    visible(a, t.i0 + (t.rows - 1) / t.n_heads, t.s.nq, t.nk, all_lo, HI);
+    if (a.splits > 1) {
+        LO += (int)min((int64_t)blockIdx.y * a.chunk, (int64_t)0x3fffffff);
+        HI = min(HI, LO + a.chunk);
+    }
+    auto sw = [](int r) { return F32 ? swz32<NC>(r) : swz<NC>(r); };
+
+    u32x4 qf[KS];
+    {
+        const T* q = (const T*)a.q + (t.s.q0 + i) * a.q_row + (int64_t)h * a.q_head;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const int d = E * (2 * s + half);
+            qf[s] = d < a.dim ? *(const u32x4*)(q + d) : u32x4{0, 0, 0, 0};
+        }
+    }
+    const char* kp = (const char*)((const T*)a.k + t.s.k0 * a.k_row + (int64_t)t.kv * a.k_head);
+    const char* vp = (const char*)((const T*)a.v + t.s.k0 * a.v_row + (int64_t)t.kv * a.v_head);
+    const int64_t kr = a.k_row * sizeof(T), vr = a.v_row * sizeof(T);
+    const uint32_t mine = lds + wave * 4 * TILE;
+    auto stage = [&](int base, int buf) {
+        const uint32_t at = mine + buf * 2 * TILE;
+#pragma unroll
+        for (int n = 0; n < LOADS; ++n) {
+            const int slot = n * 64 + lane, r = slot / NC, c = ((slot % NC) ^ sw(r)) * 16;
+            const int64_t j = min(base + r, t.nk - 1);
+            load_lds16(c < a.dim * (int)sizeof(T) ? (const void*)(kp + j * kr + c) : (const void*)&zero16, at + n * 1024);
+        }
+#pragma unroll
+        for (int n = 0; n < LOADS; ++n) {
+            const int slot = n * 64 + lane, r = slot / NC, c = ((slot % NC) ^ sw(r)) * 16;
+            const int64_t j = min(base + r, t.nk - 1);
+            load_lds16(c < a.dim * (int)sizeof(T) ? (const void*)(vp + j * vr + c) : (const void*)&zero16, at + TILE + n * 1024);
+        }
+    };
+    const float c1 = a.scale * LOG2E;
+    float ref = -INFINITY, mc = 0.0f, l = 0.0f;
+    f32x16 o[DT];
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[dt][r] = 0.0f;
+    int odd = 0;
+    const int first = LO + wave * BK, stride = NW * BK;
+    if (first < HI) stage(first, 0);
+    if (first + stride < HI) stage(first + stride, 1);
+    int buf = 0;
+    for (int base = first; base < HI; base += stride, buf ^= 1) {
+        // this tile's loads, not the next one's
+        if (base + stride < HI) wait_loads_but<2 * LOADS>();
+        else wait_loads();
+        const uint32_t kt_ = mine + buf * 2 * TILE, vt_ = kt_ + TILE;
+        uint32_t there = ~0u;
+        const bool edge = a.key_mask || base < all_lo || base + BK > all_hi || base + BK > HI;
+        if (edge) {
+            const int j = base + col;
+            there = (uint32_t)__ballot(j < HI && (!a.key_mask || a.key_mask[t.s.k0 + j]));
+#pragma unroll
+            for (int n = 0; n < LOADS; ++n) {
+                const uint32_t at = vt_ + (n * 64 + lane) * 16;
+                if (!((there >> ((n * 64 + lane) / NC)) & 1)) lds_write<u32x4>(at, u32x4{0, 0, 0, 0});
+                else odd |= not_finite<T>(lds_read<u32x4>(at));
+            }
+        }
+        f32x16 z;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) z[r] = 0.0f;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const u32x4 k = lds_read<u32x4>(kt_ + col * ROW + (((2 * s + half) ^ sw(col)) * 16));
+            if constexpr (F32) {
+                const f32x4 kf = __builtin_bit_cast(f32x4, k), q = __builtin_bit_cast(f32x4, qf[s]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) z = mfma(kf[e], q[e], z);
+            } else z = mfma(__builtin_bit_cast(typename Vec<T>::x8, k), __builtin_bit_cast(typename Vec<T>::x8, qf[s]), z);
+        }
+        if (edge) {
+            const int from = max(lo - base, 0), to = min(hi - base, 32);
+            const uint32_t see = (to <= from ? 0 : there & (~0u << from) & (~0u >> (32 - to))) >> (4 * half);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) z[r] = (see >> acc_row(r, 0)) & 1 ? z[r] : -INFINITY;
+        }
+        float m = z[0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r) m = fmaxf(m, z[r]);
+        m = pair_max(m);
+        if (__any((m - ref) * c1 > 8.0f)) {
+            const float now = fmaxf(m, ref);
+            const float mcn = now == -INFINITY ? 0.0f : now * c1;
+            const float f = ref == -INFINITY ? 0.0f : exp2_fast(mc - mcn);
+            ref = now;
+            mc = mcn;
+            l *= f;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[dt][r] *= f;
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            z[r] = exp2_fast(fmaf(z[r], c1, -mc));
+            l += z[r];
+        }
+        if constexpr (F32) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int row = acc_row(r, half);
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt)
+                    o[dt] = mfma(lds_read<float>(vt_ + row * ROW + (((dt * 8 + (col >> 2)) ^ sw(row)) * 16) + (col & 3) * 4), z[r], o[dt]);
+            }
+        } else {
+            typedef typename Vec<T>::x8 x8;
+            typedef short s16x8 __attribute__((ext_vector_type(8)));
+            const int g = (lane >> 4) & 1, i4 = lane & 15;
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                x8 p, p2;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    p[e] = (T)z[8 * s + e];
+                    p2[e] = (T)(z[8 * s + e] - (float)p[e]);
+                }
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) {
+                    s16x4 v[2];
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const int r = 8 * j + 4 * half + (i4 >> 2), c = dt * 4 + g * 2 + ((i4 & 3) >> 1);
+                        v[j] = lds_read_tr(vt_ + (16 * s + r) * ROW + ((c ^ sw(r)) * 16) + (i4 & 1) * 8);
+                    }
+                    const x8 vv = __builtin_bit_cast(x8, (s16x8)__builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7));
+                    o[dt] = mfma(vv, p, o[dt]);
+                    o[dt] = mfma(vv, p2, o[dt]);
+                }
+            }
+        }
+        // the tile is read: its place may be loaded again
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if (base + 2 * stride < HI) stage(base + 2 * stride, buf);
+    }
+    l = pair_sum(l);
+    if (__syncthreads_or(odd)) {
+        for (int r = wave; r < t.rows; r += NW)
+            attn_row<T>(a, t.s, t.nk, t.i0 + r / t.n_heads, t.head0 + r % t.n_heads, LO, HI, blockIdx.y);
+        return;
+    }
+
+    // sums of the waves, in units of 2^(m_w - M); a wave takes a 32-wide part of the result (two, where they are fewer)
+    float* all = (float*)smem;                               // [NW][DT][16][64], then m and l [NW][2][32]
+    float* ml = all + NW * DT * 1024;
+    const float m = ref == -INFINITY ? -INFINITY : mc;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) all[((wave * DT + dt) * 16 + r) * 64 + lane] = o[dt][r];
+    if (half == 0) {
+        ml[wave * 64 + col] = m;
+        ml[wave * 64 + 32 + col] = l;
+    }
+    __syncthreads();
+    float M = -INFINITY, f[NW];
+#pragma unroll
+    for (int w = 0; w < NW; ++w) M = fmaxf(M, ml[w * 64 + col]);
+    const float MM = M == -INFINITY ? 0.0f : M;
+    l = 0.0f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+        f[w] = exp2_fast(ml[w * 64 + col] - MM);
+        l = fmaf(f[w], ml[w * 64 + 32 + col], l);
+    }
+    for (int dt = wave; dt < DT; dt += NW) {
+        f32x16 x[1];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            x[0][r] = 0.0f;
+#pragma unroll
+            for (int w = 0; w < NW; ++w) x[0][r] = fmaf(f[w], all[((w * DT + dt) * 16 + r) * 64 + lane], x[0][r]);
+        }
+        attn_store<T, 1>(a, t, x, l, MM * LN2, i, h, row_ok, half, dt);
+    }
 }
 
 // Joins the runs of keys of a row and head: weights exp(lse_y - max), one wave each.  A run in which nothing is seen

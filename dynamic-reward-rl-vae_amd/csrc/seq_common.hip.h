@@ -92,6 +92,20 @@ __device__ __forceinline__ void load_lds16(const void* g, uint32_t lds) {
 }
 __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
+// All but the last N loads.
+template <int N>
+__device__ __forceinline__ void wait_loads_but() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+
+// Whether 16 bytes hold an infinity or NaN.
+template <typename T>
+__device__ __forceinline__ int not_finite(u32x4 x) {
+    constexpr uint32_t E = sizeof(T) == 4 ? 0x7f800000u : __is_same(T, bf16) ? 0x7f80u : 0x7c00u;
+    int odd = 0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) odd |= (x[w] & E) == E || (sizeof(T) == 2 && ((x[w] >> 16) & E) == E);
+    return odd;
+}
+
 template <typename V>
 __device__ __forceinline__ V lds_read(uint32_t at) { return *(const __attribute__((address_space(3))) V*)at; }
 template <typename V>

@@ -189,14 +189,18 @@ static void by_count(int n, F f) {
 template <typename T>
 static void attn_tiles(const AttnPlan& p, const seq::AttnArgs& k, hipStream_t st) {
     const int dt = (k.dim + 31) / 32;
-    const size_t shmem = 4 * 128 * 64 * (dt == 1 ? 1 : dt == 2 ? 2 : 4) / 2;      // two tiles of keys and of values
+    const size_t tile = 64 * sizeof(T) * (dt == 1 ? 1 : dt == 2 ? 2 : 4) * 16;    // 32 keys (or values)
     const dim3 grid((unsigned)p.tiles, p.splits);
-    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), shmem, st, k); };
+    auto go = [&](auto kernel, int waves, size_t shmem) {
+        if (shmem > 64 * 1024) (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)shmem);
+        hipLaunchKernelGGL(kernel, grid, dim3(waves * 64), shmem, st, k);
+    };
     by_count(dt, [&](auto d) {
         constexpr int DT = decltype(d)::value;
-        if constexpr (sizeof(T) == 4) go(seq::attn_tile32_kernel<DT>);
-        else if (p.few) go(seq::attn_tile_kernel<T, DT, true>);
-        else go(seq::attn_tile_kernel<T, DT, false>);
+        constexpr int NW = sizeof(T) == 4 && DT > 2 ? 2 : 4;
+        if (p.few) go(seq::attn_step_kernel<T, DT, NW>, NW, std::max(NW * 4 * tile, (size_t)NW * (DT * 4096 + 256)));
+        else if constexpr (sizeof(T) == 4) go(seq::attn_tile32_kernel<DT>, 4, 4 * tile);
+        else go(seq::attn_tile_kernel<T, DT>, 4, 8 * tile);
     });
     if (p.splits > 1) {
         const dim3 jg((unsigned)((k.part_rows * k.heads + 3) / 4));

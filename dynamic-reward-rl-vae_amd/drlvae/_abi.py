@@ -4,6 +4,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # DRLVAE_LIB points experiments (ablation builds) at another build of the same library
@@ -74,6 +75,17 @@ class NormArgs(C.Structure):
 
 
 SEQ_CALL_SIZE = C.sizeof(SeqCall)
+
+
+def _packer(cls):
+    """struct.Struct with a ctypes structure's layout, native sizes and alignment."""
+    code = {C.c_void_p: "P", C.c_int64: "q", C.c_int32: "i", C.c_float: "f"}
+    p = struct.Struct("@" + "".join(code[t] for _, t in cls._fields_))
+    assert p.size <= C.sizeof(cls) and C.sizeof(cls) - p.size < 8
+    return struct.Struct("@" + "".join(code[t] for _, t in cls._fields_) + "0P")      # the end padded as the structure's
+
+
+pack_call, pack_attn, pack_linear, pack_norm = (_packer(c).pack for c in (SeqCall, AttnArgs, LinearArgs, NormArgs))
 
 _lib = None
 
@@ -155,7 +167,7 @@ def load():
     lib.drl_set_knob.argtypes = [vp, C.c_char_p, C.c_longlong]
     lib.drl_debug_alloc_count.argtypes = []
     lib.drl_debug_alloc_count.restype = C.c_longlong
-    call, attn, lin, norm = C.POINTER(SeqCall), C.POINTER(AttnArgs), C.POINTER(LinearArgs), C.POINTER(NormArgs)
+    call = attn = lin = norm = vp          # the structs below, or their bytes (sequence.py packs them: it is quicker)
     lib.drl_seq_layout_create.argtypes = [vp, _i64p, _i64p, C.c_int, C.POINTER(vp)]
     lib.drl_seq_layout_destroy.argtypes = [vp]
     lib.drl_seq_layout_destroy.restype = None

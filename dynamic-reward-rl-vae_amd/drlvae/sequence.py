@@ -19,11 +19,15 @@ _torch = None
 _dtypes = {}
 
 
+_stream = None
+
+
 def _t():
-    global _torch
+    global _torch, _stream
     if _torch is None:
         import torch
         _dtypes.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
+        _stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda d: torch.cuda.current_stream(d).cuda_stream)
         _torch = torch
     return _torch
 
@@ -43,6 +47,7 @@ class SeqLayout:
         scorer._check(self._lib.drl_seq_layout_create(scorer._h, q.ctypes.data_as(p64), None if k_offsets is None else k.ctypes.data_as(p64),
                                                       len(q) - 1, C.byref(h)), "drl_seq_layout_create")
         self._h = h
+        self._plans = {}              # scratch bytes that calls of given sizes need
         self.device = scorer.device
         self.n_seg = len(q) - 1
         self.q_first, self.q_rows = int(q[0]), int(q[-1])
@@ -70,27 +75,32 @@ class SequenceOps:
 
     # ------------------------------------------------------------------ checks and plumbing
     def _tensor(self, name, x, dtype, ndim):
-        torch = _t()
-        if not isinstance(x, torch.Tensor) or x.dim() != ndim or (dtype is not None and x.dtype != dtype):
+        """x as a tensor of that many axes on this scorer's GPU; its shape."""
+        torch = _torch or _t()
+        if not isinstance(x, torch.Tensor) or (dtype is not None and x.dtype != dtype):
             raise ValueError(f"{name} must be a {ndim}-dimensional tensor" + (f" of {dtype}" if dtype is not None else ""))
+        shape = x.shape
+        if len(shape) != ndim:
+            raise ValueError(f"{name} must be a {ndim}-dimensional tensor, not of shape {tuple(shape)}")
         if not x.is_cuda or x.get_device() != self.device:
             raise ValueError(f"{name} is on {x.device}, the scorer on GPU {self.device}")
         if x.requires_grad and torch.is_grad_enabled():
             raise ValueError(f"{name} requires a gradient: the sequence operators are forward only (use torch.no_grad())")
-        return x
+        return shape
 
     def _rows(self, name, x, dtype, rows, heads=None, dim=None):
-        self._tensor(name, x, dtype, 3)
-        s = x.shape
+        """(shape, strides) of a tensor of rows x heads x dim."""
+        s = self._tensor(name, x, dtype, 3)
         if s[0] < rows or (heads is not None and s[1] != heads) or (dim is not None and s[2] != dim):
             raise ValueError(f"{name} has shape {tuple(s)}, expected at least {rows} rows x {heads or s[1]} heads x {dim or s[2]}")
-        if x.stride(2) != 1 and s[2] != 1:
+        st = x.stride()
+        if st[2] != 1 and s[2] != 1:
             raise ValueError(f"the last axis of {name} must be dense")
-        return x
+        return s, st
 
     def _flat(self, name, x, dtype, n):
-        self._tensor(name, x, dtype, 1)
-        if x.shape[0] != n or not x.is_contiguous():
+        s = self._tensor(name, x, dtype, 1)
+        if s[0] != n or (n > 1 and x.stride(0) != 1):
             raise ValueError(f"{name} must hold {n} dense values")
         return x.data_ptr()
 
@@ -102,82 +112,77 @@ class SequenceOps:
         return layout
 
     def _output(self, out, like, shape, covered):
-        """The output tensor: the caller's, or a new one, zero where no series writes."""
-        torch = _t()
+        """(output tensor, its strides): the caller's, or a new one, zero where no series writes."""
         if out is None:
-            return torch.empty(shape, dtype=like.dtype, device=like.device) if covered else torch.zeros(shape, dtype=like.dtype, device=like.device)
-        self._rows("out", out, like.dtype, 0, shape[1], shape[2])
-        if out.shape[0] != shape[0]:
-            raise ValueError(f"out has {out.shape[0]} rows, q {shape[0]}")
-        return out
+            out = like.new_empty(shape) if covered else like.new_zeros(shape)
+            return out, out.stride()
+        s, st = self._rows("out", out, like.dtype, 0, shape[1], shape[2])
+        if s[0] != shape[0]:
+            raise ValueError(f"out has {s[0]} rows, q {shape[0]}")
+        return out, st
 
-    def _call(self, dtype):
-        try:
-            code = _dtypes[dtype]
-        except KeyError:
-            raise ValueError(f"dtype {dtype}: float32, float16 or bfloat16") from None
-        return _abi.SeqCall(_abi.SEQ_CALL_SIZE, _abi.ABI_REVISION, code, 1, _torch.cuda.current_stream(self.device).cuda_stream, None, 0)
-
-    def _workspace(self, fn, head, call, args, device):
-        """Asks how much scratch the call needs and takes it from torch; returns the tensor that keeps it alive."""
-        n = C.c_int64(0)
-        self._check(fn(self._h, *head, C.byref(call), C.byref(args), C.byref(n)), fn.__name__)
-        if n.value == 0:
-            return None
-        ws = _torch.empty(n.value, dtype=_torch.uint8, device=device)
-        call.workspace, call.workspace_bytes = ws.data_ptr(), n.value
-        return ws
+    def _run(self, name, dtype, like, head, args, plan):
+        """One call on torch's current stream.  ``plan``, a dictionary of the layout's (or None: no scratch), keeps how much
+        scratch calls of these sizes need; the scratch itself is torch's, new for each call."""
+        code = _dtypes.get(dtype)
+        if code is None:
+            raise ValueError(f"dtype {dtype}: float32, float16 or bfloat16")
+        lib, stream = self._lib, _stream(self.device)
+        need, ws = 0, None
+        if plan is not None:
+            need = plan[0].get(plan[1])
+            if need is None:
+                n = C.c_int64(0)
+                call = _abi.pack_call(_abi.SEQ_CALL_SIZE, _abi.ABI_REVISION, code, 1, stream, 0, 0)
+                self._check(getattr(lib, f"drl_{name}_workspace")(self._h, *head, call, args, C.byref(n)), f"drl_{name}_workspace")
+                need = plan[0][plan[1]] = n.value
+        if need:
+            ws = like.new_empty(need, dtype=_torch.uint8)
+            call = _abi.pack_call(_abi.SEQ_CALL_SIZE, _abi.ABI_REVISION, code, 1, stream, ws.data_ptr(), need)
+        else:
+            call = _abi.pack_call(_abi.SEQ_CALL_SIZE, _abi.ABI_REVISION, code, 1, stream, 0, 0)
+        rc = getattr(lib, f"drl_{name}_dev")(self._h, *head, call, args)
+        if rc:
+            self._check(rc, f"drl_{name}_dev")
 
     # ------------------------------------------------------------------ attention
     def attention(self, q, k, v, layout: SeqLayout, *, scale: Optional[float] = None, causal: bool = True, window: int = 0,
                   key_mask=None, k_len=None, out=None, return_lse: bool = False):
         """Softmax attention over the layout's series: q [rows, heads, dim], k and v [rows, kv_heads, dim] (any row and
-        head strides; float32, float16 or bfloat16), heads a multiple of kv_heads, dim a multiple of 8 up to 128.
+        head strides of 16 bytes; float32, float16 or bfloat16), heads a multiple of kv_heads, dim a multiple of 8 up to 128.
 
         Row i of a series with nq rows and nk keys sees key j when j <= i + nk - nq (``causal``), j > i + nk - nq -
         window (``window`` > 0) and ``key_mask``[j] (bool, one per row of k).  ``k_len`` (int32, one per series): how
         many of its rows of k are filled; values outside them are clamped.  A row that sees nothing gets 0 and a
         log-sum of -inf.  Returns out, or (out, lse [rows, heads] float32)."""
-        torch = _t()
         layout = self._layout(layout)
-        self._rows("q", q, None, layout.q_rows)
-        rows, heads, dim = q.shape
-        self._rows("k", k, q.dtype, layout.k_rows, None, dim)
-        self._rows("v", v, q.dtype, layout.k_rows, k.shape[1], dim)
+        (rows, heads, dim), qs = self._rows("q", q, None, layout.q_rows)
+        dtype = q.dtype
+        (k_rows, kv, _), ks = self._rows("k", k, dtype, layout.k_rows, None, dim)
+        _, vs = self._rows("v", v, dtype, layout.k_rows, kv, dim)
         covered = layout.q_first == 0 and layout.q_rows == rows
-        out = self._output(out, q, (rows, heads, dim), covered)
-        lse = None
+        out, os_ = self._output(out, q, (rows, heads, dim), covered)
+        lse, mask, klen = None, 0, 0
         if return_lse:
-            lse = torch.empty((rows, heads), dtype=torch.float32, device=q.device) if covered else torch.zeros((rows, heads), dtype=torch.float32, device=q.device)
-        mask = None
+            lse = (q.new_empty if covered else q.new_zeros)((rows, heads), dtype=_torch.float32)
         if key_mask is not None:
-            if key_mask.dtype not in (torch.bool, torch.uint8):
+            if key_mask.dtype not in (_torch.bool, _torch.uint8):
                 raise ValueError("key_mask must be bool or uint8")
-            mask = self._flat("key_mask", key_mask, None, k.shape[0])
-        klen = None if k_len is None else self._flat("k_len", k_len, torch.int32, layout.n_seg)
-        call = self._call(q.dtype)
-        qs, ks, vs, os_ = q.stride(), k.stride(), v.stride(), out.stride()
-        a = _abi.AttnArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(), mask, klen,
-                          qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os_[0], os_[1], heads, k.shape[1], dim, 1 if causal else 0, int(window),
-                          dim ** -0.5 if scale is None else float(scale))
-        ws = self._workspace(self._lib.drl_attention_workspace, (layout._h,), call, a, q.device)
-        self._check(self._lib.drl_attention_dev(self._h, layout._h, C.byref(call), C.byref(a)), "drl_attention_dev")
-        del ws
-        return (out, lse) if return_lse else out
+            mask = self._flat("key_mask", key_mask, None, k_rows)
+        if k_len is not None:
+            klen = self._flat("k_len", k_len, _torch.int32, layout.n_seg)
+        window = int(window)
+        args = _abi.pack_attn(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(), mask, klen,
+                              qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os_[0], os_[1], heads, kv, dim, 1 if causal else 0, window,
+                              dim ** -0.5 if scale is None else scale)
+        self._run("attention", dtype, q, (layout._h,), args, (layout._plans, (0, dtype, heads, kv, dim, causal, window)))
+        return out if lse is None else (out, lse)
 
     # ------------------------------------------------------------------ linear attention
-    def _linear_args(self, q, k, v, log_decay, out, state_in, state_out, scale):
-        qs, ks, vs, os_ = q.stride(), k.stride(), v.stride(), out.stride()
-        return _abi.LinearArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), self._flat("log_decay", log_decay, _torch.float32, q.shape[1]),
-                               None if state_in is None else state_in.data_ptr(), None if state_out is None else state_out.data_ptr(),
-                               qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os_[0], os_[1], q.shape[1], k.shape[1], q.shape[2], v.shape[2],
-                               q.shape[2] ** -0.5 if scale is None else float(scale), 0)
-
     def _state(self, name, x, shape):
-        self._tensor(name, x, _torch.float32, 4)
-        if tuple(x.shape) != shape or not x.is_contiguous():
+        if self._tensor(name, x, _torch.float32, 4) != shape or not x.is_contiguous():
             raise ValueError(f"{name} must be a dense tensor of shape {shape}")
-        return x
+        return x.data_ptr()
 
     def linear_attention(self, q, k, v, log_decay, layout: SeqLayout, *, scale: Optional[float] = None, state=None, out=None,
                          final_state=None):
@@ -186,41 +191,38 @@ class SequenceOps:
         q [rows, heads, dim_k], k [rows, kv_heads, dim_k], v [rows, kv_heads, dim_v]; the states are float32
         [n_seg, heads, dim_k, dim_v]: ``state`` the first ones (None: zeros), the last ones are returned, in
         ``final_state`` if given (it may be ``state``).  Returns (out [rows, heads, dim_v], final_state)."""
-        torch = _t()
         layout = self._layout(layout)
-        self._rows("q", q, None, layout.q_rows)
-        rows, heads, dk = q.shape
-        self._rows("k", k, q.dtype, layout.q_rows, None, dk)
-        self._rows("v", v, q.dtype, layout.q_rows, k.shape[1])
-        dv = v.shape[2]
-        out = self._output(out, q, (rows, heads, dv), layout.q_first == 0 and layout.q_rows == rows)
+        (rows, heads, dk), qs = self._rows("q", q, None, layout.q_rows)
+        dtype = q.dtype
+        (_, kv, _), ks = self._rows("k", k, dtype, layout.q_rows, None, dk)
+        (_, _, dv), vs = self._rows("v", v, dtype, layout.q_rows, kv)
+        out, os_ = self._output(out, q, (rows, heads, dv), layout.q_first == 0 and layout.q_rows == rows)
         shape = (layout.n_seg, heads, dk, dv)
-        if state is not None:
-            self._state("state", state, shape)
+        first = 0 if state is None else self._state("state", state, shape)
         if final_state is None:
-            final_state = torch.empty(shape, dtype=torch.float32, device=q.device)
+            final_state = q.new_empty(shape, dtype=_torch.float32)
+            last = final_state.data_ptr()
         else:
-            self._state("final_state", final_state, shape)
-        call = self._call(q.dtype)
-        a = self._linear_args(q, k, v, log_decay, out, state, final_state, scale)
-        ws = self._workspace(self._lib.drl_linear_attention_workspace, (layout._h,), call, a, q.device)
-        self._check(self._lib.drl_linear_attention_dev(self._h, layout._h, C.byref(call), C.byref(a)), "drl_linear_attention_dev")
-        del ws
+            last = self._state("final_state", final_state, shape)
+        args = _abi.pack_linear(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), self._flat("log_decay", log_decay, _torch.float32, heads),
+                                first, last, qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os_[0], os_[1], heads, kv, dk, dv,
+                                dk ** -0.5 if scale is None else scale, 0)
+        self._run("linear_attention", dtype, q, (layout._h,), args, (layout._plans, (1, dtype, heads, kv, dk, dv)))
         return out, final_state
 
     def linear_attention_step(self, q, k, v, log_decay, state, *, scale: Optional[float] = None, out=None):
         """One new row of each of n series: q [n, heads, dim_k], k [n, kv_heads, dim_k], v [n, kv_heads, dim_v]; ``state``
         [n, heads, dim_k, dim_v] is updated in place.  Returns out [n, heads, dim_v]."""
-        _t()
-        self._rows("q", q, None, 0)
-        n, heads, dk = q.shape
-        self._rows("k", k, q.dtype, n, None, dk)
-        self._rows("v", v, q.dtype, n, k.shape[1])
-        out = self._output(out, q, (n, heads, v.shape[2]), True)
-        self._state("state", state, (n, heads, dk, v.shape[2]))
-        call = self._call(q.dtype)
-        a = self._linear_args(q, k, v, log_decay, out, state, state, scale)
-        self._check(self._lib.drl_linear_attention_step_dev(self._h, n, C.byref(call), C.byref(a)), "drl_linear_attention_step_dev")
+        (n, heads, dk), qs = self._rows("q", q, None, 0)
+        dtype = q.dtype
+        (_, kv, _), ks = self._rows("k", k, dtype, n, None, dk)
+        (_, _, dv), vs = self._rows("v", v, dtype, n, kv)
+        out, os_ = self._output(out, q, (n, heads, dv), True)
+        st = self._state("state", state, (n, heads, dk, dv))
+        args = _abi.pack_linear(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), self._flat("log_decay", log_decay, _torch.float32, heads),
+                                st, st, qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os_[0], os_[1], heads, kv, dk, dv,
+                                dk ** -0.5 if scale is None else scale, 0)
+        self._run("linear_attention_step", dtype, q, (n,), args, None)
         return out
 
     # ------------------------------------------------------------------ group norm
@@ -229,28 +231,30 @@ class SequenceOps:
         """Group normalisation and an activation ("linear", "relu", "sigmoid", "silu") of x [rows, channels]: statistics
         over each group's channels in all rows of a series, or, without a layout, in each row.  gamma and beta are
         float32 [channels].  ``out`` may be x."""
-        torch = _t()
-        self._tensor("x", x, None, 2)
-        rows, c = x.shape
-        if x.stride(1) != 1 and c != 1:
+        rows, c = self._tensor("x", x, None, 2)
+        xs = x.stride()
+        if xs[1] != 1 and c != 1:
             raise ValueError("the last axis of x must be dense")
         if layout is not None and self._layout(layout).q_rows > rows:
             raise ValueError(f"x has {rows} rows, the layout {layout.q_rows}")
         if out is None:
-            covered = layout is None or (layout.q_first == 0 and layout.q_rows == rows)
-            out = (torch.empty if covered else torch.zeros)((rows, c), dtype=x.dtype, device=x.device)
+            out = (x.new_empty if layout is None or (layout.q_first == 0 and layout.q_rows == rows) else x.new_zeros)((rows, c))
+            ys = (c, 1)
         else:
-            self._tensor("out", out, x.dtype, 2)
-            if out.shape != x.shape or (out.stride(1) != 1 and c != 1):
+            if self._tensor("out", out, x.dtype, 2) != x.shape or (out.stride(1) != 1 and c != 1):
                 raise ValueError("out must have x's shape and a dense last axis")
-        if activation not in _ACTS:
+            ys = out.stride()
+        act = _ACTS.get(activation)
+        if act is None:
             raise ValueError(f"activation {activation!r}: one of {', '.join(_ACTS)}")
-        call = self._call(x.dtype)
-        a = _abi.NormArgs(x.data_ptr(), out.data_ptr(), None if gamma is None else self._flat("gamma", gamma, torch.float32, c),
-                          None if beta is None else self._flat("beta", beta, torch.float32, c),
-                          x.stride(0) if rows > 1 else c, out.stride(0) if rows > 1 else c, c, int(groups), _ACTS[activation], float(eps))
-        h = None if layout is None else layout._h
-        ws = self._workspace(self._lib.drl_group_norm_workspace, (h, rows), call, a, x.device)
-        self._check(self._lib.drl_group_norm_dev(self._h, h, rows, C.byref(call), C.byref(a)), "drl_group_norm_dev")
-        del ws
+        xp, yp = x.data_ptr(), out.data_ptr()
+        xr, yr = (xs[0], ys[0]) if rows > 1 else (c, c)
+        args = _abi.pack_norm(xp, yp, 0 if gamma is None else self._flat("gamma", gamma, _torch.float32, c),
+                              0 if beta is None else self._flat("beta", beta, _torch.float32, c), xr, yr, c, int(groups), act, eps)
+        if layout is None:
+            self._run("group_norm", x.dtype, x, (None, rows), args, None)
+        else:
+            # the plan goes by what x and out are aligned to as well
+            self._run("group_norm", x.dtype, x, (layout._h, rows), args,
+                      (layout._plans, (2, x.dtype, c, groups, (xp | yp | xr * 16 | yr * 16) & 255)))
         return out
