@@ -96,14 +96,21 @@ __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)"
 template <int N>
 __device__ __forceinline__ void wait_loads_but() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 
-// Whether 16 bytes hold an infinity or NaN.
-template <typename T>
-__device__ __forceinline__ int not_finite(u32x4 x) {
-    constexpr uint32_t E = sizeof(T) == 4 ? 0x7f800000u : __is_same(T, bf16) ? 0x7f80u : 0x7c00u;
-    int odd = 0;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) odd |= (x[w] & E) == E || (sizeof(T) == 2 && ((x[w] >> 16) & E) == E);
-    return odd;
+// Whether 16 (or 32) bytes hold an infinity or NaN: the largest exponent of all.
+template <typename T, typename... X>
+__device__ __forceinline__ bool not_finite(X... x) {
+    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+    if constexpr (sizeof(T) == 4) {
+        uint32_t top = 0;
+        ((top = max(max(top, x[0] & 0x7fffffffu), max(x[1] & 0x7fffffffu, max(x[2] & 0x7fffffffu, x[3] & 0x7fffffffu)))), ...);
+        return top >= 0x7f800000u;
+    } else {
+        constexpr unsigned short E = __is_same(T, bf16) ? 0x7f80 : 0x7c00;
+        u16x2 top = {0, 0};
+        auto one = [&](uint32_t w) { top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, w & 0x7fff7fffu)); };
+        ((one(x[0]), one(x[1]), one(x[2]), one(x[3])), ...);
+        return max(top[0], top[1]) >= E;
+    }
 }
 
 template <typename V>

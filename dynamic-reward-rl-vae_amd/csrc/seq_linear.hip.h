@@ -238,44 +238,20 @@ __global__ __launch_bounds__(NW * 64, 2) void linear_chunk_kernel(LinearArgs a) 
         x8 v[2];
 #pragma unroll
         for (int s = 0; s < 2; ++s) v[s] = read_tr(kb + vtr[0] + s * 16 * VP * 2, kb + vtr[1] + s * 16 * VP * 2);
-        bool odd = false;
-        {
-            constexpr uint32_t E = F16 ? 0x7c00u : 0x7f80u;
+        // A value that is not finite must not meet the rows before its own, not even with weight 0: it is taken out, and its
+        // column is set to NaN from its row on.
+        int bad;
+        const bool odd = __any(not_finite<T>(__builtin_bit_cast(u32x4, v[0]), __builtin_bit_cast(u32x4, v[1])));
+        if (odd) {
+            bad = C;
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                const u32x4 w = __builtin_bit_cast(u32x4, v[s]);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) odd |= (w[e] & E) == E || ((w[e] >> 16) & E) == E;
-            }
-        }
-        if (__any(odd)) {
-            // a value that is not finite: no row before its own may meet it, not even with weight 0.  Row after row.
-            const float lam = exp2_fast(ld2);
-            int hf = half;
-#pragma unroll 1
-            for (int j = 0; j < n; ++j) {
-                asm volatile("" : "+v"(hf));                   // 64 places per lane: not to be kept over the whole loop
-
-                const uint32_t vo = kb + QK + j * VP * 2 + (((wave * 4 + (col >> 3)) ^ swz<VC>(j)) * 16) + (col & 7) * 2;
-                const float vc = (float)lds_read<T>(vo);
-                float acc = 0.0f;
-#pragma unroll
-                for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        if (r % 4 == 0) __builtin_amdgcn_sched_barrier(0);
-                        const int d = kt * 32 + acc_row(r, hf);
-                        const uint32_t at = j * DP * 2 + (((d >> 3) ^ swz<NC>(j)) * 16) + (d & 7) * 2;
-                        S[kt][r] = fmaf((float)lds_read<T>(kb + at), vc, lam * S[kt][r]);
-                        if (kt * 32 + acc_row(r, 0) >= a.dk) S[kt][r] = 0.0f;
-                        if constexpr (!STATE) acc = fmaf((float)lds_read<T>(qb + at), S[kt][r], acc);
-                    }
-                if constexpr (!STATE) {
-                    acc = pair_sum(acc) * a.scale;
-                    if (on && half == 0) op[(int64_t)(base + j) * a.o_row + col] = (T)acc;
+            for (int e = 15; e >= 0; --e)
+                if (!(fabsf((float)v[e >> 3][e & 7]) < INFINITY)) {
+                    bad = acc_row(e, half);
+                    v[e >> 3][e & 7] = (T)0.0f;
                 }
-            }
-            continue;
+            bad = min(bad, __shfl_xor(bad, 32));
+            if (bad >= n) bad = C;                             // rows behind the series' last are its last again
         }
 
         if constexpr (!STATE) {
@@ -330,6 +306,9 @@ __global__ __launch_bounds__(NW * 64, 2) void linear_chunk_kernel(LinearArgs a) 
             if constexpr (F16)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) w[r] = fmaf(w[r], p_back, o[r]);
+            if (odd)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) w[r] = acc_row(r, half) >= bad ? NAN : w[r];
             // rows of 64 bytes through this wave's corner of LDS, then 16 bytes per lane
             const uint32_t ob = lds + 2 * STAGE + wave * (C * 64);
 #pragma unroll
@@ -366,12 +345,15 @@ __global__ __launch_bounds__(NW * 64, 2) void linear_chunk_kernel(LinearArgs a) 
         }
         x8 y[2][N];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            float r = x[e];
+        for (int e = 0; e < 16; e += 2) {
+            f32x2 r = {x[e], x[e + 1]};
 #pragma unroll
             for (int m = 0; m < N; ++m) {
-                y[e >> 3][m][e & 7] = (T)r;
-                r -= (float)y[e >> 3][m][e & 7];
+                const typename Vec<T>::x2 c = __builtin_convertvector(r, typename Vec<T>::x2);
+                y[e >> 3][m][e & 7] = c[0];
+                y[e >> 3][m][(e & 7) + 1] = c[1];
+                r[0] -= (float)c[0];
+                r[1] -= (float)c[1];
             }
         }
 #pragma unroll
@@ -392,6 +374,11 @@ __global__ __launch_bounds__(NW * 64, 2) void linear_chunk_kernel(LinearArgs a) 
 #pragma unroll
             for (int r = 0; r < 16; ++r) S[kt][r] = F16 ? fmaf(acc[r], v_back, S[kt][r]) : acc[r];
         }
+        if (odd && bad < C)
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) S[kt][r] = NAN;
     }
 
     float* to = nullptr;
@@ -484,32 +471,17 @@ __global__ __launch_bounds__(NW * 64) void linear_chunk32_kernel(LinearArgs a) {
             v[r] = lds_read<float>(vb + j * VP * 4 + (((wave * 8 + (col >> 2)) ^ swz32<VC>(j)) * 16) + (col & 3) * 4);
             odd |= !(fabsf(v[r]) < INFINITY);
         }
-        if (__any(odd)) {
-            // a value that is not finite: row after row, as for the 16-bit types
-            const float lam = exp2_fast(ld2);
-            int hf = half;
-#pragma unroll 1
-            for (int j = 0; j < n; ++j) {
-                asm volatile("" : "+v"(hf));
-                const float vc = lds_read<float>(vb + j * VP * 4 + (((wave * 8 + (col >> 2)) ^ swz32<VC>(j)) * 16) + (col & 3) * 4);
-                float acc = 0.0f;
+        int bad = C;                                           // as for the 16-bit types
+        odd = __any(odd);
+        if (odd) {
 #pragma unroll
-                for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        if (r % 4 == 0) __builtin_amdgcn_sched_barrier(0);
-                        const int d = kt * 32 + acc_row(r, hf);
-                        const uint32_t at = j * DP * 4 + (((d >> 2) ^ swz32<NC>(j)) * 16) + (d & 3) * 4;
-                        S[kt][r] = fmaf(lds_read<float>(kb + at), vc, lam * S[kt][r]);
-                        if (kt * 32 + acc_row(r, 0) >= a.dk) S[kt][r] = 0.0f;
-                        if constexpr (!STATE) acc = fmaf(lds_read<float>(qb + at), S[kt][r], acc);
-                    }
-                if constexpr (!STATE) {
-                    acc = pair_sum(acc) * a.scale;
-                    if (on && half == 0) op[(int64_t)(base + j) * a.o_row + c0 + col] = acc;
+            for (int r = 15; r >= 0; --r)
+                if (!(fabsf(v[r]) < INFINITY)) {
+                    bad = acc_row(r, half);
+                    v[r] = 0.0f;
                 }
-            }
-            continue;
+            bad = min(bad, __shfl_xor(bad, 32));
+            if (bad >= n) bad = C;
         }
         if constexpr (!STATE) {
             f32x16 z, o;
@@ -538,7 +510,7 @@ __global__ __launch_bounds__(NW * 64) void linear_chunk32_kernel(LinearArgs a) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     const int j = acc_row(r, half);
-                    if (j < n) op[(int64_t)(base + j) * a.o_row + c0 + col] = o[r];
+                    if (j < n) op[(int64_t)(base + j) * a.o_row + c0 + col] = j >= bad ? NAN : o[r];
                 }
         }
 #pragma unroll
@@ -556,6 +528,11 @@ __global__ __launch_bounds__(NW * 64) void linear_chunk32_kernel(LinearArgs a) {
                 S[kt] = mfma(lds_read<float>(kb + j * DP * 4 + (((kt * 8 + (col >> 2)) ^ swz32<NC>(j)) * 16) + (col & 3) * 4), v[r], S[kt]);
             }
         }
+        if (odd && bad < C)
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) S[kt][r] = NAN;
     }
     float* to = nullptr;
     if (STATE) to = a.states + ((t.u + 1) * a.heads + h) * (int64_t)a.dk * a.dv;
