@@ -124,6 +124,13 @@ __device__ __forceinline__ s16x4 lds_read_tr(uint32_t at) {
     return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at);
 }
 
+// x y, and 0 where one of them is 0, whatever the other holds (v_mul_legacy_f32).
+extern "C" __device__ float drl_mul_legacy(float, float) __asm("llvm.amdgcn.fmul.legacy");
+__device__ __forceinline__ float mul_legacy(float x, float y) { return drl_mul_legacy(x, y); }
+
+// LDS reads stay on their side of this; everything else may be moved across.
+__device__ __forceinline__ void keep_reads() { __builtin_amdgcn_sched_barrier(0x67f); }
+
 // The larger / the sum of a lane's value and that of the lane 32 away.
 __device__ __forceinline__ float pair_max(float x) {
     const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);

@@ -269,7 +269,7 @@ __global__ __launch_bounds__(NW * 64, 2) void linear_chunk_kernel(LinearArgs a) 
             }
 #pragma unroll
             for (int s = 0; s < 2 * KT; ++s) {
-                if (s % 2 == 0) __builtin_amdgcn_sched_barrier(0);     // two steps' reads in flight, no more: registers
+                if (s % 2 == 0) keep_reads();                          // two steps' reads in flight, no more: registers
                 const x8 q = read_row(qb, s), k = read_row(kb, s);
                 z = mfma(k, q, z);
                 x8 b;
@@ -277,12 +277,9 @@ __global__ __launch_bounds__(NW * 64, 2) void linear_chunk_kernel(LinearArgs a) 
                 for (int e = 0; e < 8; ++e) b[e] = (T)(F16 ? S[s >> 1][8 * (s & 1) + e] * s_scale : S[s >> 1][8 * (s & 1) + e]);
                 o = mfma(q, b, o);
             }
-            __builtin_amdgcn_sched_barrier(0);
             float p[16];
-            int apart = col - 4 * half;
-            asm volatile("" : "+v"(apart));                    // compared here: 16 lane masks are more than there are registers for
 #pragma unroll
-            for (int r = 0; r < 16; ++r) p[r] = apart >= acc_row(r, 0) ? z[r] * inner[r] : 0.0f;
+            for (int r = 0; r < 16; ++r) p[r] = mul_legacy(z[r], inner[r]);     // 0 where inner is 0, whatever the score
             float p_scale = 1.0f, p_back = 1.0f;
             f32x16 w = o;
 #pragma unroll
@@ -321,7 +318,6 @@ __global__ __launch_bounds__(NW * 64, 2) void linear_chunk_kernel(LinearArgs a) 
             }
         }
 
-        __builtin_amdgcn_sched_barrier(0);
         float x[16], v_scale = 1.0f, v_back = 1.0f;
 #pragma unroll
         for (int e = 0; e < 16; ++e) x[e] = (float)v[e >> 3][e & 7];
@@ -358,7 +354,7 @@ __global__ __launch_bounds__(NW * 64, 2) void linear_chunk_kernel(LinearArgs a) 
         }
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt) {
-            __builtin_amdgcn_sched_barrier(0);
+            keep_reads();
             f32x16 acc;
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
