@@ -11,6 +11,8 @@
 #pragma once
 #include "seq_common.hip.h"
 
+#include <type_traits>
+
 namespace seq {
 
 struct AttnArgs {
@@ -214,28 +216,15 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
         }
     }
 
-    // staging: thread's slots of a tile, row and chunk; chunks behind the width come from zeros
     const char* kp = (const char*)((const T*)a.k + t.s.k0 * a.k_row + (int64_t)t.kv * a.k_head);
     const char* vp = (const char*)((const T*)a.v + t.s.k0 * a.v_row + (int64_t)t.kv * a.v_head);
     const int64_t kr = a.k_row * 2, vr = a.v_row * 2;
-    int srow[LOADS], schunk[LOADS];
-#pragma unroll
-    for (int n = 0; n < LOADS; ++n) {
-        const int slot = n * 256 + threadIdx.x;
-        srow[n] = slot / NC;
-        schunk[n] = ((slot % NC) ^ swz<NC>(srow[n])) * 16;
-        if (schunk[n] >= a.dim * 2) schunk[n] = -1;
-    }
+    const TileLoad<BK, NC, 256, Swz<NC>> load_k(threadIdx.x, a.dim * 2, kr), load_v(threadIdx.x, a.dim * 2, vr);
+    for (int b = 0; b < 4; ++b) load_k.clear(lds + b * TILE);
     auto stage = [&](int base, int buf) {
         const uint32_t at = lds + buf * 2 * TILE + wave * 1024;
-#pragma unroll
-        for (int n = 0; n < LOADS; ++n) {
-            const int j = min(base + srow[n], t.nk - 1);
-            const void* kg = schunk[n] >= 0 ? (const void*)(kp + j * kr + schunk[n]) : (const void*)&zero16;
-            const void* vg = schunk[n] >= 0 ? (const void*)(vp + j * vr + schunk[n]) : (const void*)&zero16;
-            load_lds16(kg, at + n * 4096);
-            load_lds16(vg, at + TILE + n * 4096);
-        }
+        load_k(kp + base * kr, t.nk - base, at);
+        load_v(vp + base * vr, t.nk - base, at + TILE);
     };
 
     // operand reads: keys as rows, values transposed
@@ -283,7 +272,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
 #pragma unroll
             for (int n = 0; n < LOADS; ++n) {
                 const uint32_t at = vt_ + (n * 256 + threadIdx.x) * 16;
-                if (!((there >> srow[n]) & 1)) lds_write<u32x4>(at, u32x4{0, 0, 0, 0});
+                if (!((there >> load_v.row(n)) & 1)) lds_write<u32x4>(at, u32x4{0, 0, 0, 0});
                 else odd |= not_finite<T>(lds_read<u32x4>(at));
             }
             if (__syncthreads_or(odd)) { strange = true; break; }
@@ -396,22 +385,12 @@ __global__ __launch_bounds__(256, 2) void attn_tile32_kernel(AttnArgs a) {
     const char* kp = (const char*)((const float*)a.k + t.s.k0 * a.k_row + (int64_t)t.kv * a.k_head);
     const char* vp = (const char*)((const float*)a.v + t.s.k0 * a.v_row + (int64_t)t.kv * a.v_head);
     const int64_t kr = a.k_row * 4, vr = a.v_row * 4;
-    int srow[LOADS], schunk[LOADS];
-#pragma unroll
-    for (int n = 0; n < LOADS; ++n) {
-        const int slot = n * 256 + threadIdx.x;
-        srow[n] = slot / NC;
-        schunk[n] = ((slot % NC) ^ swz32<NC>(srow[n])) * 16;
-        if (schunk[n] >= a.dim * 4) schunk[n] = -1;
-    }
+    const TileLoad<BK, NC, 256, Swz32<NC>> load_k(threadIdx.x, a.dim * 4, kr), load_v(threadIdx.x, a.dim * 4, vr);
+    for (int b = 0; b < 4; ++b) load_k.clear(lds + b * TILE);
     auto stage = [&](int base, int buf) {
         const uint32_t at = lds + buf * 2 * TILE + wave * 1024;
-#pragma unroll
-        for (int n = 0; n < LOADS; ++n) {
-            const int j = min(base + srow[n], t.nk - 1);
-            load_lds16(schunk[n] >= 0 ? (const void*)(kp + j * kr + schunk[n]) : (const void*)&zero16, at + n * 4096);
-            load_lds16(schunk[n] >= 0 ? (const void*)(vp + j * vr + schunk[n]) : (const void*)&zero16, at + TILE + n * 4096);
-        }
+        load_k(kp + base * kr, t.nk - base, at);
+        load_v(vp + base * vr, t.nk - base, at + TILE);
     };
     const float c1 = a.scale * LOG2E;
     float ref = -INFINITY, mc = 0.0f, l = 0.0f;
@@ -438,7 +417,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile32_kernel(AttnArgs a) {
 #pragma unroll
             for (int n = 0; n < LOADS; ++n) {
                 const uint32_t at = vt_ + (n * 256 + threadIdx.x) * 16;
-                if (!((there >> srow[n]) & 1)) lds_write<u32x4>(at, u32x4{0, 0, 0, 0});
+                if (!((there >> load_v.row(n)) & 1)) lds_write<u32x4>(at, u32x4{0, 0, 0, 0});
                 else odd |= not_finite<float>(lds_read<u32x4>(at));
             }
             if (__syncthreads_or(odd)) { strange = true; break; }
@@ -538,20 +517,12 @@ __global__ __launch_bounds__(NW * 64) void attn_step_kernel(AttnArgs a) {
     const char* vp = (const char*)((const T*)a.v + t.s.k0 * a.v_row + (int64_t)t.kv * a.v_head);
     const int64_t kr = a.k_row * sizeof(T), vr = a.v_row * sizeof(T);
     const uint32_t mine = lds + wave * 4 * TILE;
+    const TileLoad<BK, NC, 64, std::conditional_t<F32, Swz32<NC>, Swz<NC>>> load_k(lane, a.dim * sizeof(T), kr), load_v(lane, a.dim * sizeof(T), vr);
+    for (int b = 0; b < 4; ++b) load_k.clear(mine + b * TILE);
     auto stage = [&](int base, int buf) {
         const uint32_t at = mine + buf * 2 * TILE;
-#pragma unroll
-        for (int n = 0; n < LOADS; ++n) {
-            const int slot = n * 64 + lane, r = slot / NC, c = ((slot % NC) ^ sw(r)) * 16;
-            const int64_t j = min(base + r, t.nk - 1);
-            load_lds16(c < a.dim * (int)sizeof(T) ? (const void*)(kp + j * kr + c) : (const void*)&zero16, at + n * 1024);
-        }
-#pragma unroll
-        for (int n = 0; n < LOADS; ++n) {
-            const int slot = n * 64 + lane, r = slot / NC, c = ((slot % NC) ^ sw(r)) * 16;
-            const int64_t j = min(base + r, t.nk - 1);
-            load_lds16(c < a.dim * (int)sizeof(T) ? (const void*)(vp + j * vr + c) : (const void*)&zero16, at + TILE + n * 1024);
-        }
+        load_k(kp + base * kr, t.nk - base, at);
+        load_v(vp + base * vr, t.nk - base, at + TILE);
     };
     const float c1 = a.scale * LOG2E;
     float ref = -INFINITY, mc = 0.0f, l = 0.0f;

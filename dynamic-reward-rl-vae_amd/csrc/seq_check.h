@@ -62,6 +62,9 @@ inline bool seq_aligned(int dtype, const void* p, int64_t row, int64_t head) {
     return !((uintptr_t)p & 15) && row >= 0 && head >= 0 && row <= most && head <= most && row % unit == 0 && head % unit == 0;
 }
 
+// The kernels count the rows of a tile in 32 bits.
+constexpr int64_t SEQ_MAX_ROW = (int64_t)1 << 24;
+
 // Rows and heads of an output may lie either way round, but not on each other.
 inline bool seq_apart(int64_t rows, int64_t row, int heads, int64_t head, int width) {
     const bool row_major = head >= width && row >= (heads - 1) * head + width;
@@ -87,6 +90,7 @@ inline int seq_check_attention(SeqError& e, const SeqRows* l, const drl_seq_call
     if (!seq_aligned(c->dtype, a->q, a->q_row, a->q_head) || !seq_aligned(c->dtype, a->k, a->k_row, a->k_head) ||
         !seq_aligned(c->dtype, a->v, a->v_row, a->v_head) || !seq_aligned(c->dtype, a->out, a->o_row, a->o_head))
         return e.set(DRL_ERR_ARG, "%s: a pointer or stride is negative or not a multiple of 16 bytes", who);
+    if (a->k_row > SEQ_MAX_ROW || a->v_row > SEQ_MAX_ROW) return e.set(DRL_ERR_UNSUPPORTED, "%s: a row stride of k or v above 2^24", who);
     if (((uintptr_t)a->lse & 3) || ((uintptr_t)a->k_len & 3)) return e.set(DRL_ERR_ARG, "%s: lse or k_len not 4-byte aligned", who);
     if (!seq_apart(l->q_end, a->o_row, a->n_heads, a->o_head, a->dim)) return e.set(DRL_ERR_ARG, "%s: rows or heads of out overlap", who);
     return DRL_OK;
@@ -108,6 +112,8 @@ inline int seq_check_linear(SeqError& e, const char* who, int64_t rows, const dr
         !seq_aligned(c->dtype, a->v, a->v_row, a->v_head) || !seq_aligned(c->dtype, a->out, a->o_row, a->o_head) ||
         ((uintptr_t)a->state_in & 15) || ((uintptr_t)a->state_out & 15) || ((uintptr_t)a->log_decay & 3))
         return e.set(DRL_ERR_ARG, "%s: a pointer or stride is negative or not a multiple of 16 bytes", who);
+    if (a->q_row > SEQ_MAX_ROW || a->k_row > SEQ_MAX_ROW || a->v_row > SEQ_MAX_ROW)
+        return e.set(DRL_ERR_UNSUPPORTED, "%s: a row stride above 2^24", who);
     if (!seq_apart(rows, a->o_row, a->n_heads, a->o_head, a->dim_v)) return e.set(DRL_ERR_ARG, "%s: rows or heads of out overlap", who);
     return DRL_OK;
 }

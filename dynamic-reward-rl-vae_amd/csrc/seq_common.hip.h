@@ -84,12 +84,53 @@ __device__ __forceinline__ int swz32(int r) {
 typedef __attribute__((address_space(3))) char lds_char;
 __device__ __forceinline__ uint32_t lds_offset(const void* p) { return (uint32_t)(uintptr_t)(lds_char*)p; }
 
-// 16 bytes per lane from global memory into LDS at `lds` + 16 * lane (the same `lds` for the whole wave), without
-// registers between.  Nothing waits for it by itself: wait_loads() does, then a barrier shows it to the other waves.
-// (m0 is written: nothing else in these kernels uses it, and the compiler sets it before uses of its own.)
-__device__ __forceinline__ void load_lds16(const void* g, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(g) : "memory");
+// 16 bytes per lane from global memory, `base` (the same for the whole wave) + `offset` bytes, into LDS at `lds` + 16 * lane
+// (the same `lds` for the whole wave), without registers between.  Nothing waits for it by itself: wait_loads() does,
+// then a barrier shows it to the other waves.  (m0 is written: nothing else in these kernels uses it, and the compiler
+// sets it before uses of its own.)
+__device__ __forceinline__ void load_lds16(const void* base, uint32_t offset, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory");
 }
+
+// A tile of ROWS rows of NC 16-byte chunks on its way into LDS, THREADS threads at it: where each of a thread's loads comes
+// from and goes to.  Chunks behind the rows' width are not loaded: their places are cleared once, with clear().
+// SW::at(row) is where a row's chunks are moved.  Row strides are below 2^26 bytes.
+template <int ROWS, int NC, int THREADS, typename SW>
+struct TileLoad {
+    static constexpr int LOADS = (ROWS * NC + THREADS - 1) / THREADS;
+    uint32_t offset[LOADS];
+    int width, stride;            // bytes
+    int first;                    // this thread's number among those at the tile
+    __device__ __forceinline__ int row(int n) const { return (n * THREADS + first) / NC; }
+    __device__ __forceinline__ int chunk(int n) const { return (((n * THREADS + first) % NC) ^ SW::at(row(n))) * 16; }
+    __device__ __forceinline__ bool has(int n) const { return ROWS * NC % THREADS == 0 || n * THREADS + first < ROWS * NC; }
+    __device__ __forceinline__ TileLoad(int first_, int width_, int64_t stride_) : width(width_), stride((int)stride_), first(first_) {
+#pragma unroll
+        for (int n = 0; n < LOADS; ++n) offset[n] = (uint32_t)row(n) * (uint32_t)stride + chunk(n);
+    }
+    __device__ __forceinline__ void clear(uint32_t tile) const {
+        if (width < NC * 16)
+#pragma unroll
+            for (int n = 0; n < LOADS; ++n)
+                if (has(n) && chunk(n) >= width) *(__attribute__((address_space(3))) u32x4*)(tile + (n * THREADS + first) * 16) = u32x4{0, 0, 0, 0};
+    }
+    // The rows from `base` on, of which there are `rows`: behind them the last one again.  `tile`: where the wave's first
+    // lane writes.
+    __device__ __forceinline__ void operator()(const void* base, int rows, uint32_t tile) const {
+        if (rows >= ROWS && width == NC * 16) {
+#pragma unroll
+            for (int n = 0; n < LOADS; ++n)
+                if (has(n)) load_lds16(base, offset[n], tile + n * THREADS * 16);
+        } else {
+#pragma unroll
+            for (int n = 0; n < LOADS; ++n)
+                if (has(n) && chunk(n) < width) load_lds16(base, (uint32_t)min(row(n), rows - 1) * (uint32_t)stride + chunk(n), tile + n * THREADS * 16);
+        }
+    }
+};
+template <int NC> struct Swz { static __device__ __forceinline__ int at(int r) { return swz<NC>(r); } };
+template <int NC> struct Swz32 { static __device__ __forceinline__ int at(int r) { return swz32<NC>(r); } };
+
 __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 // All but the last N loads.
@@ -148,8 +189,5 @@ __device__ __forceinline__ f32x16 mfma(Vec<f16>::x8 a, Vec<f16>::x8 b, f32x16 c)
 // 32x32x2 product: one element of the inner axis per lane half.
 __device__ __forceinline__ f32x16 mfma(float a, float b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ int acc_row(int r, int half) { return (r & 3) + 8 * (r >> 2) + 4 * half; }
-
-// Sixteen bytes of zeros: where lanes load from whose chunk lies behind a row's end.
-__device__ const u32x4 zero16 = {0, 0, 0, 0};
 
 }  // namespace seq

@@ -132,7 +132,7 @@ __device__ __forceinline__ float into_range(float x, float& back) {
 // float16 in two), and loses nothing from call to call.  float16 has no range to spare: scores, state columns and
 // weighted values are scaled by powers of two before they are rounded.
 template <typename T, int KT, int NW, bool STATE>
-__global__ __launch_bounds__(NW * 64, 2) void linear_chunk_kernel(LinearArgs a) {
+__global__ __launch_bounds__(NW * 64, STATE ? 3 : 2) void linear_chunk_kernel(LinearArgs a) {
     typedef typename Vec<T>::x8 x8;
     typedef typename Vec<T>::x4 x4;
     typedef short s16x8 __attribute__((ext_vector_type(8)));
@@ -141,9 +141,8 @@ __global__ __launch_bounds__(NW * 64, 2) void linear_chunk_kernel(LinearArgs a) 
     constexpr int DP = KT <= 1 ? 32 : KT <= 2 ? 64 : 128, NC = DP / 8;     // key width of an LDS row, in chunks of 8
     constexpr int VP = 32 * NW, VC = VP / 8;
     constexpr int QK = C * DP * 2, VB = C * VP * 2, STAGE = (STATE ? 1 : 2) * QK + VB;
-    constexpr int KL = (C * NC + THREADS - 1) / THREADS, VL = C * VC / THREADS;
-    extern __shared__ char smem[];
-    const uint32_t lds = lds_offset(smem);
+    extern __shared__ __align__(256) char smem[];
+    const uint32_t lds = lds_offset(smem), table = lds + 2 * STAGE;
     const int h = blockIdx.x % a.heads, blk = (blockIdx.x / a.heads) % a.blocks;
     const LinearUnit t = linear_unit(a, blockIdx.x / (a.heads * a.blocks));
     if (!t.any || (STATE && t.last)) return;
@@ -172,55 +171,55 @@ __global__ __launch_bounds__(NW * 64, 2) void linear_chunk_kernel(LinearArgs a) 
     const char* qp = (const char*)((const T*)a.q + row0 * a.q_row + (int64_t)h * a.q_head);
     const char* kp = (const char*)((const T*)a.k + row0 * a.k_row + (int64_t)(h / a.rep) * a.k_head);
     const char* vp = (const char*)((const T*)a.v + row0 * a.v_row + (int64_t)(h / a.rep) * a.v_head + blk * VP);
-    const int vw = (a.dv - blk * VP) * 2;                      // bytes of values from here on
+    const TileLoad<C, NC, THREADS, Swz<NC>> load_q(threadIdx.x, a.dk * 2, a.q_row * 2), load_k(threadIdx.x, a.dk * 2, a.k_row * 2);
+    const TileLoad<C, VC, THREADS, Swz<VC>> load_v(threadIdx.x, min(a.dv - blk * VP, VP) * 2, a.v_row * 2);
+    for (int b = 0; b < 2; ++b) {
+        load_k.clear(lds + b * STAGE);
+        load_v.clear(lds + b * STAGE + QK);
+        if (!STATE) load_q.clear(lds + b * STAGE + QK + VB);
+    }
     auto stage = [&](int base, int buf) {
         const uint32_t at = lds + buf * STAGE + wave * 1024;
-#pragma unroll
-        for (int n = 0; n < KL; ++n) {
-            if (C * NC < THREADS && wave * 64 >= C * NC) break;        // a narrow key tile: the first waves load it
-            const int slot = n * THREADS + threadIdx.x, r = slot / NC, c = ((slot % NC) ^ swz<NC>(r)) * 16;
-            const int64_t j = min(base + r, t.rows - 1);
-            const bool in = c < a.dk * 2;
-            load_lds16(in ? (const void*)(kp + j * a.k_row * 2 + c) : (const void*)&zero16, at + n * THREADS * 16);
-            if (!STATE) load_lds16(in ? (const void*)(qp + j * a.q_row * 2 + c) : (const void*)&zero16, at + QK + VB + n * THREADS * 16);
-        }
-#pragma unroll
-        for (int n = 0; n < VL; ++n) {
-            const int slot = n * THREADS + threadIdx.x, r = slot / VC, c = ((slot % VC) ^ swz<VC>(r)) * 16;
-            const int64_t j = min(base + r, t.rows - 1);
-            load_lds16(c < vw ? (const void*)(vp + j * a.v_row * 2 + c) : (const void*)&zero16, at + QK + n * THREADS * 16);
-        }
+        load_k(kp + base * a.k_row * 2, t.rows - base, at);
+        load_v(vp + base * a.v_row * 2, t.rows - base, at + QK);
+        if (!STATE) load_q(qp + base * a.q_row * 2, t.rows - base, at + QK + VB);
     };
 
-    // LDS places: rows in the order of the accumulator's registers (two reads of 4), and transposed
-    const int g = (lane >> 4) & 1, i4 = lane & 15;
-    auto row_at = [&](int s, int j) { return (uint32_t)(col * (DP * 2) + (((2 * s + j) ^ swz<NC>(col)) * 16) + half * 8); };
-    auto tr_at = [&](int width, int sw_c, int r) { return (uint32_t)(r * width * 2 + sw_c * 16 + (i4 & 1) * 8); };
-    uint32_t ktr[KT][2], vtr[2];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const int r = 8 * j + 4 * half + (i4 >> 2), cc = g * 2 + ((i4 & 3) >> 1);
-#pragma unroll
-        for (int kt = 0; kt < KT; ++kt) ktr[kt][j] = tr_at(DP, (kt * 4 + cc) ^ swz<NC>(r), r);
-        vtr[j] = QK + tr_at(VP, (wave * 4 + cc) ^ swz<VC>(r), r);
-    }
+    // LDS places: rows in the order of the accumulators' registers (two reads of 4), and transposed.  Chunk c lies at place
+    // c ^ swz of its row, so that one place gives the others by an exclusive or (tiles begin at whole rows).
+    const int g = (lane >> 4) & 1, i4 = lane & 15, tr = 4 * half + (i4 >> 2), tc = g * 2 + ((i4 & 3) >> 1);
+    const uint32_t row4 = col * (DP * 2) + swz<NC>(col) * 16 + half * 8;
+    const uint32_t ktr = tr * (DP * 2) + ((tc ^ swz<NC>(tr)) * 16) + (i4 & 1) * 8;
+    const uint32_t ktr8 = (tr + 8) * (DP * 2) + ((tc ^ swz<NC>(tr + 8)) * 16) + (i4 & 1) * 8;
+    const uint32_t vtr = QK + tr * (VP * 2) + (((wave * 4 + tc) ^ swz<VC>(tr)) * 16) + (i4 & 1) * 8;
+    const uint32_t vtr8 = QK + (tr + 8) * (VP * 2) + (((wave * 4 + tc) ^ swz<VC>(tr + 8)) * 16) + (i4 & 1) * 8;
     auto read_tr = [&](uint32_t a0, uint32_t a1) {
         return __builtin_bit_cast(x8, (s16x8)__builtin_shufflevector(lds_read_tr(a0), lds_read_tr(a1), 0, 1, 2, 3, 4, 5, 6, 7));
     };
     auto read_row = [&](uint32_t base, int s) {
-        const x4 x = lds_read<x4>(base + row_at(s, 0)), y = lds_read<x4>(base + row_at(s, 1));
+        const x4 x = lds_read<x4>((base + row4) ^ (s * 32)), y = lds_read<x4>((base + row4) ^ (s * 32 + 16));
         return (x8)__builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
     };
 
-    // powers of lam: between a row (lane) and a key (register), of a value's row to the chunk's end, of a row from its start
-    // (the last two are a lane's part times a register's, which is the same for all lanes)
-    float inner[STATE ? 1 : 16], up[16];
+    // Powers of lam, the same for all waves and chunks, in LDS, four registers' worth side by side per lane: of a value's row
+    // to the chunk's end; of a row from its start, times the scale; between a row (lane) and a key (register), times the
+    // scale, 0 for the keys behind it.
+    const uint32_t mine = table + lane * 16;
+    if (wave == 0)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) up[r] = uniform(power(ld2, acc_row(r, 0)));        // lam^0 .. lam^27, and back from 27
-    if constexpr (!STATE)
+        for (int r = 0; r < 16; r += 4) {
+            f32x4 left, grown, inner;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) inner[r] = col >= acc_row(r, half) ? a.scale * power(ld2, col - acc_row(r, half)) : 0.0f;
-    const float lane_up = a.scale * power(ld2, 4 * half + 1), lane_left = power(ld2, 4 - 4 * half);
+            for (int e = 0; e < 4; ++e) {
+                const int row = acc_row(r + e, half);
+                left[e] = power(ld2, C - 1 - row);
+                grown[e] = a.scale * power(ld2, row + 1);
+                inner[e] = col >= row ? a.scale * power(ld2, col - row) : 0.0f;
+            }
+            lds_write<f32x4>(mine + r * 256, left);
+            if (!STATE) lds_write<f32x4>(mine + 4096 + r * 256, grown);
+            if (!STATE) lds_write<f32x4>(mine + 8192 + r * 256, inner);
+        }
     float fall = expm1f(decay_log(a, h) * (float)C);           // lam^n - 1: lam^n itself, rounded, would drift over many chunks
 
     T* op = (T*)a.out + row0 * a.o_row + (int64_t)h * a.o_head + c0;
@@ -228,7 +227,9 @@ __global__ __launch_bounds__(NW * 64, 2) void linear_chunk_kernel(LinearArgs a) 
     int buf = 0;
     for (int base = 0; base < t.rows; base += C, buf ^= 1) {
         const int n = min(C, t.rows - base);
-        wait_loads();
+        // The chunk has to be here; the two stores of the chunk before, younger than its loads, need not be done.
+        if (STATE || base == 0 || c0 >= a.dv) wait_loads();
+        else wait_loads_but<2>();
         __syncthreads();
         if (base + C < t.rows) stage(base + C, buf ^ 1);
         if (c0 >= a.dv) continue;                              // a wave behind the values' width only loads
@@ -237,7 +238,7 @@ __global__ __launch_bounds__(NW * 64, 2) void linear_chunk_kernel(LinearArgs a) 
 
         x8 v[2];
 #pragma unroll
-        for (int s = 0; s < 2; ++s) v[s] = read_tr(kb + vtr[0] + s * 16 * VP * 2, kb + vtr[1] + s * 16 * VP * 2);
+        for (int s = 0; s < 2; ++s) v[s] = read_tr(kb + vtr + s * 16 * VP * 2, kb + vtr8 + s * 16 * VP * 2);
         // A value that is not finite must not meet the rows before its own, not even with weight 0: it is taken out, and its
         // column is set to NaN from its row on.
         int bad;
@@ -279,11 +280,19 @@ __global__ __launch_bounds__(NW * 64, 2) void linear_chunk_kernel(LinearArgs a) 
             }
             float p[16];
 #pragma unroll
-            for (int r = 0; r < 16; ++r) p[r] = mul_legacy(z[r], inner[r]);     // 0 where inner is 0, whatever the score
+            for (int r = 0; r < 16; r += 4) {
+                const f32x4 inner = lds_read<f32x4>(mine + 8192 + r * 256);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) p[r + e] = mul_legacy(z[r + e], inner[e]);     // 0 where inner is 0, whatever the score
+            }
             float p_scale = 1.0f, p_back = 1.0f;
             f32x16 w = o;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) o[r] *= F16 ? lane_up * up[r] * s_back : lane_up * up[r];
+            for (int r = 0; r < 16; r += 4) {
+                const f32x4 grown = lds_read<f32x4>(mine + 4096 + r * 256);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[r + e] *= F16 ? grown[e] * s_back : grown[e];
+            }
             if constexpr (F16) {
                 float m = 0.0f;
 #pragma unroll
@@ -306,14 +315,17 @@ __global__ __launch_bounds__(NW * 64, 2) void linear_chunk_kernel(LinearArgs a) 
             if (odd)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) w[r] = acc_row(r, half) >= bad ? NAN : w[r];
-            // rows of 64 bytes through this wave's corner of LDS, then 16 bytes per lane
-            const uint32_t ob = lds + 2 * STAGE + wave * (C * 64);
+            // through the values' own place in LDS, which no other wave reads, and out 16 bytes per lane
+            const uint32_t vb = kb + QK;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) lds_write<T>(ob + acc_row(r, half) * 64 + col * 2, (T)w[r]);
+            for (int r = 0; r < 16; ++r) {
+                const int row = acc_row(r, half);
+                lds_write<T>(vb + row * (VP * 2) + (((wave * 4 + (col >> 3)) ^ swz<VC>(row)) * 16) + (col & 7) * 2, (T)w[r]);
+            }
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
                 const int j = m * 16 + (lane >> 2);
-                const u32x4 y = lds_read<u32x4>(ob + m * 1024 + lane * 16);
+                const u32x4 y = lds_read<u32x4>(vb + j * (VP * 2) + (((wave * 4 + (lane & 3)) ^ swz<VC>(j)) * 16));
                 if (j < n && c0 + (lane & 3) * 8 < a.dv) *(u32x4*)(op + (int64_t)(base + j) * a.o_row + (lane & 3) * 8) = y;
             }
         }
@@ -323,7 +335,11 @@ __global__ __launch_bounds__(NW * 64, 2) void linear_chunk_kernel(LinearArgs a) 
         for (int e = 0; e < 16; ++e) x[e] = (float)v[e >> 3][e & 7];
         if (n == C) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) x[e] *= lane_left * up[15 - e];             // 31 - row = (4 - 4 half) + (27 - the register's part)
+            for (int r = 0; r < 16; r += 4) {
+                const f32x4 left = lds_read<f32x4>(mine + r * 256);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[r + e] *= left[e];
+            }
         } else {
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
@@ -363,7 +379,7 @@ __global__ __launch_bounds__(NW * 64, 2) void linear_chunk_kernel(LinearArgs a) 
             }
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
-                const x8 k = read_tr(kb + ktr[kt][0] + s * 16 * DP * 2, kb + ktr[kt][1] + s * 16 * DP * 2);
+                const x8 k = read_tr(((kb + ktr) ^ (kt * 64)) + s * 16 * DP * 2, ((kb + ktr8) ^ (kt * 64)) + s * 16 * DP * 2);
 #pragma unroll
                 for (int m = 0; m < N; ++m) acc = mfma(k, y[s][m], acc);
             }
@@ -398,8 +414,6 @@ __global__ __launch_bounds__(NW * 64) void linear_chunk32_kernel(LinearArgs a) {
     constexpr int DP = KT <= 1 ? 32 : KT <= 2 ? 64 : 128, NC = DP / 4;
     constexpr int VP = 32 * NW, VC = VP / 4;
     constexpr int QK = C * DP * 4, VB = C * VP * 4, STAGE = (STATE ? 1 : 2) * QK + VB;
-    constexpr int KL = C * NC / THREADS, VL = C * VC / THREADS;
-    static_assert(KL >= 1 && VL >= 1, "a load per thread at least");
     extern __shared__ char smem[];
     const uint32_t lds = lds_offset(smem);
     const int h = blockIdx.x % a.heads, blk = (blockIdx.x / a.heads) % a.blocks;
@@ -425,23 +439,18 @@ __global__ __launch_bounds__(NW * 64) void linear_chunk32_kernel(LinearArgs a) {
     const char* qp = (const char*)((const float*)a.q + row0 * a.q_row + (int64_t)h * a.q_head);
     const char* kp = (const char*)((const float*)a.k + row0 * a.k_row + (int64_t)(h / a.rep) * a.k_head);
     const char* vp = (const char*)((const float*)a.v + row0 * a.v_row + (int64_t)(h / a.rep) * a.v_head + blk * VP);
-    const int vw = (a.dv - blk * VP) * 4;
+    const TileLoad<C, NC, THREADS, Swz32<NC>> load_q(threadIdx.x, a.dk * 4, a.q_row * 4), load_k(threadIdx.x, a.dk * 4, a.k_row * 4);
+    const TileLoad<C, VC, THREADS, Swz32<VC>> load_v(threadIdx.x, min(a.dv - blk * VP, VP) * 4, a.v_row * 4);
+    for (int b = 0; b < 2; ++b) {
+        load_k.clear(lds + b * STAGE);
+        load_v.clear(lds + b * STAGE + QK);
+        if (!STATE) load_q.clear(lds + b * STAGE + QK + VB);
+    }
     auto stage = [&](int base, int buf) {
         const uint32_t at = lds + buf * STAGE + wave * 1024;
-#pragma unroll
-        for (int n = 0; n < KL; ++n) {
-            const int slot = n * THREADS + threadIdx.x, r = slot / NC, c = ((slot % NC) ^ swz32<NC>(r)) * 16;
-            const int64_t j = min(base + r, t.rows - 1);
-            const bool in = c < a.dk * 4;
-            load_lds16(in ? (const void*)(kp + j * a.k_row * 4 + c) : (const void*)&zero16, at + n * THREADS * 16);
-            if (!STATE) load_lds16(in ? (const void*)(qp + j * a.q_row * 4 + c) : (const void*)&zero16, at + QK + VB + n * THREADS * 16);
-        }
-#pragma unroll
-        for (int n = 0; n < VL; ++n) {
-            const int slot = n * THREADS + threadIdx.x, r = slot / VC, c = ((slot % VC) ^ swz32<VC>(r)) * 16;
-            const int64_t j = min(base + r, t.rows - 1);
-            load_lds16(c < vw ? (const void*)(vp + j * a.v_row * 4 + c) : (const void*)&zero16, at + QK + n * THREADS * 16);
-        }
+        load_k(kp + base * a.k_row * 4, t.rows - base, at);
+        load_v(vp + base * a.v_row * 4, t.rows - base, at + QK);
+        if (!STATE) load_q(qp + base * a.q_row * 4, t.rows - base, at + QK + VB);
     };
     float up[16];
 #pragma unroll
