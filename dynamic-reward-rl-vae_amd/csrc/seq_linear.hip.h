@@ -142,7 +142,7 @@ __global__ __launch_bounds__(NW * 64, STATE ? 3 : 2) void linear_chunk_kernel(Li
     constexpr int VP = 32 * NW, VC = VP / 8;
     constexpr int QK = C * DP * 2, VB = C * VP * 2, STAGE = (STATE ? 1 : 2) * QK + VB;
     extern __shared__ __align__(256) char smem[];
-    const uint32_t lds = lds_offset(smem), table = lds + 2 * STAGE;
+    const uint32_t lds = lds_offset(smem), table = lds + 3 * STAGE;
     const int h = blockIdx.x % a.heads, blk = (blockIdx.x / a.heads) % a.blocks;
     const LinearUnit t = linear_unit(a, blockIdx.x / (a.heads * a.blocks));
     if (!t.any || (STATE && t.last)) return;
@@ -173,7 +173,7 @@ __global__ __launch_bounds__(NW * 64, STATE ? 3 : 2) void linear_chunk_kernel(Li
     const char* vp = (const char*)((const T*)a.v + row0 * a.v_row + (int64_t)(h / a.rep) * a.v_head + blk * VP);
     const TileLoad<C, NC, THREADS, Swz<NC>> load_q(threadIdx.x, a.dk * 2, a.q_row * 2), load_k(threadIdx.x, a.dk * 2, a.k_row * 2);
     const TileLoad<C, VC, THREADS, Swz<VC>> load_v(threadIdx.x, min(a.dv - blk * VP, VP) * 2, a.v_row * 2);
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < 3; ++b) {
         load_k.clear(lds + b * STAGE);
         load_v.clear(lds + b * STAGE + QK);
         if (!STATE) load_q.clear(lds + b * STAGE + QK + VB);
@@ -201,10 +201,10 @@ __global__ __launch_bounds__(NW * 64, STATE ? 3 : 2) void linear_chunk_kernel(Li
         return (x8)__builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
     };
 
-    // Powers of lam, the same for all waves and chunks, in LDS, four registers' worth side by side per lane: of a value's row
-    // to the chunk's end; of a row from its start, times the scale; between a row (lane) and a key (register), times the
-    // scale, 0 for the keys behind it.
-    const uint32_t mine = table + lane * 16;
+    // Powers of lam, the same for all waves and chunks, in LDS, four registers' worth side by side: between a row (lane) and a
+    // key (register), times the scale, 0 for the keys behind it; of a value's row to the chunk's end; of a row from its
+    // start, times the scale.
+    const uint32_t inner_at = table + 256 + lane * 16, left_at = table + half * 64, grown_at = table + 128 + half * 64;
     if (wave == 0)
 #pragma unroll
         for (int r = 0; r < 16; r += 4) {
@@ -216,22 +216,28 @@ __global__ __launch_bounds__(NW * 64, STATE ? 3 : 2) void linear_chunk_kernel(Li
                 grown[e] = a.scale * power(ld2, row + 1);
                 inner[e] = col >= row ? a.scale * power(ld2, col - row) : 0.0f;
             }
-            lds_write<f32x4>(mine + r * 256, left);
-            if (!STATE) lds_write<f32x4>(mine + 4096 + r * 256, grown);
-            if (!STATE) lds_write<f32x4>(mine + 8192 + r * 256, inner);
+            lds_write<f32x4>(left_at + r * 4, left);
+            if (!STATE) lds_write<f32x4>(grown_at + r * 4, grown);
+            if (!STATE) lds_write<f32x4>(inner_at + r * 256, inner);
         }
     float fall = expm1f(decay_log(a, h) * (float)C);           // lam^n - 1: lam^n itself, rounded, would drift over many chunks
 
     T* op = (T*)a.out + row0 * a.o_row + (int64_t)h * a.o_head + c0;
+    // Loads run two chunks ahead.  AHEAD: how many a wave issues for a chunk, at least; STORES: what it stores of one.
+    constexpr int AHEAD = (STATE ? 1 : 2) * (C * NC / THREADS) + C * VC / THREADS, STORES = STATE ? 0 : 2;
+    const bool stores = c0 < a.dv;
     if (t.rows > 0) stage(0, 0);
-    int buf = 0;
-    for (int base = 0; base < t.rows; base += C, buf ^= 1) {
+    if (t.rows > C) stage(C, 1);
+    int buf = 0, far = 2;
+    for (int base = 0; base < t.rows; base += C, far = buf, buf = buf == 2 ? 0 : buf + 1) {
         const int n = min(C, t.rows - base);
-        // The chunk has to be here; the two stores of the chunk before, younger than its loads, need not be done.
-        if (STATE || base == 0 || c0 >= a.dv) wait_loads();
-        else wait_loads_but<2>();
+        // The chunk has to be here; what was issued after its loads need not be done: the stores of the two chunks before, the
+        // next one's loads.
+        if (base + C >= t.rows) wait_loads();
+        else if (base < 2 * C || !stores) wait_loads_but<AHEAD>();
+        else wait_loads_but<AHEAD + 2 * STORES>();
         __syncthreads();
-        if (base + C < t.rows) stage(base + C, buf ^ 1);
+        if (base + 2 * C < t.rows) stage(base + 2 * C, far);
         if (c0 >= a.dv) continue;                              // a wave behind the values' width only loads
         if (n < C) fall = expm1f(decay_log(a, h) * (float)n);
         const uint32_t kb = lds + buf * STAGE, qb = kb + QK + VB;
@@ -281,7 +287,7 @@ __global__ __launch_bounds__(NW * 64, STATE ? 3 : 2) void linear_chunk_kernel(Li
             float p[16];
 #pragma unroll
             for (int r = 0; r < 16; r += 4) {
-                const f32x4 inner = lds_read<f32x4>(mine + 8192 + r * 256);
+                const f32x4 inner = lds_read<f32x4>(inner_at + r * 256);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) p[r + e] = mul_legacy(z[r + e], inner[e]);     // 0 where inner is 0, whatever the score
             }
@@ -289,7 +295,7 @@ __global__ __launch_bounds__(NW * 64, STATE ? 3 : 2) void linear_chunk_kernel(Li
             f32x16 w = o;
 #pragma unroll
             for (int r = 0; r < 16; r += 4) {
-                const f32x4 grown = lds_read<f32x4>(mine + 4096 + r * 256);
+                const f32x4 grown = lds_read<f32x4>(grown_at + r * 4);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[r + e] *= F16 ? grown[e] * s_back : grown[e];
             }
@@ -336,7 +342,7 @@ __global__ __launch_bounds__(NW * 64, STATE ? 3 : 2) void linear_chunk_kernel(Li
         if (n == C) {
 #pragma unroll
             for (int r = 0; r < 16; r += 4) {
-                const f32x4 left = lds_read<f32x4>(mine + r * 256);
+                const f32x4 left = lds_read<f32x4>(left_at + r * 4);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) x[r + e] *= left[e];
             }
@@ -565,14 +571,19 @@ static __global__ __launch_bounds__(256) void linear_scan_kernel(LinearArgs a) {
     float* at = a.states + ((s.cum / a.piece + slot) * a.heads + h) * size + e;
     const int64_t next = a.heads * size;
     *(f32x4*)at = S;
-    f32x4 add = n > 1 ? *(const f32x4*)(at + next) : S;
-    for (int k = 1; k < n; ++k) {
-        at += next;
-        const f32x4 mine = add;
-        if (k + 1 < n) add = *(const f32x4*)(at + next);
+    constexpr int U = 8;                                       // pieces in flight
+    for (int k = 1; k < n; k += U) {
+        f32x4 add[U];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) S[c] = fmaf(S[c], fall, S[c]) + mine[c];
-        *(f32x4*)at = S;
+        for (int u = 0; u < U; ++u) add[u] = *(const f32x4*)(at + next * (min(k + u, n - 1) - k + 1));
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (k + u >= n) break;
+            at += next;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) S[c] = fmaf(S[c], fall, S[c]) + add[u][c];
+            *(f32x4*)at = S;
+        }
     }
 }
 

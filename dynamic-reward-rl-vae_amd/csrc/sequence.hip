@@ -254,14 +254,19 @@ static LinearPlan linear_plan(const DrlCtxView& v, const drl_seq_layout* l, cons
     p.blocks = (tiles + p.waves - 1) / p.waves;
     p.piece = 0x7fffffff;
     p.units = l->rows.n_seg;
-    // Pieces cost a second reading of k and v and the states between them: only where workgroups are fewer than two per
-    // CU, and then as many as make that, of 256 rows at least.
-    const int64_t groups = (int64_t)a->n_heads * p.blocks, want = 2 * v.n_cu;
-    if (groups * l->rows.n_seg < want && l->max_q > 512) {
-        const int64_t rows = l->n_q * groups / want;
-        p.piece = (int)std::max<int64_t>(256, (rows + 31) / 32 * 32);
-        if (p.piece >= l->max_q) p.piece = 0x7fffffff;
-        else {
+    // Pieces cost a second reading of k and v and the states between them: only where the workgroups are fewer than the CUs
+    // (384 of 2,048 rows: 222 us whole, 226 in pieces of 512; 64 of 32,768: 2.9 ms whole, 0.76 in pieces of 4,096).
+    // A piece is long enough that two workgroups per CU do it all at once, and that going through its chunks twice takes
+    // about as long as going through the pieces' states (1.6 us a chunk, 0.3 a state: pieces of sqrt(3 rows), 8,192 rows
+    // of 16 heads in 81 us at 256).
+    const int64_t groups = (int64_t)a->n_heads * p.blocks;
+    if (groups * l->rows.n_seg < v.n_cu) {
+        const int64_t rows = std::max<int64_t>(l->n_q * groups / (2 * v.n_cu), (int64_t)std::sqrt(3.0 * l->max_q));
+        const int64_t piece = std::max<int64_t>(64, (rows + 31) / 32 * 32);
+        if (piece < l->max_q) {
+            // pieces of one length
+            const int64_t n = (l->max_q + piece - 1) / piece;
+            p.piece = (int)(((l->max_q + n - 1) / n + 31) / 32 * 32);
             p.units = l->n_q / p.piece + l->rows.n_seg;
             p.workspace = p.units * a->n_heads * a->dim_k * a->dim_v * 4;
         }
@@ -293,12 +298,12 @@ static seq::LinearArgs linear_args(const drl_linear_args* a, const seq::SegInfo*
 template <typename T, int KT, int NW, bool STATE>
 static void linear_chunks(const LinearPlan& p, const seq::LinearArgs& k, hipStream_t st) {
     constexpr int DP = KT <= 1 ? 32 : KT <= 2 ? 64 : 128;
-    constexpr int stage = 32 * sizeof(T) * ((STATE ? 1 : 2) * DP + 32 * NW), out = sizeof(T) == 4 ? 0 : STATE ? 4096 : 3 * 4096;       // and tables
+    constexpr int stage = 32 * sizeof(T) * ((STATE ? 1 : 2) * DP + 32 * NW), stages = sizeof(T) == 2 ? 3 : 2, table = sizeof(T) == 4 ? 0 : STATE ? 256 : 256 + 4096;
     const dim3 grid((unsigned)(p.units * k.heads * p.blocks));
     auto go = [&](auto kernel) {
         // more LDS than a kernel gets unasked
-        if (2 * stage + out > 64 * 1024) (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 2 * stage + out);
-        hipLaunchKernelGGL(kernel, grid, dim3(NW * 64), 2 * stage + out, st, k);
+        if (stages * stage + table > 64 * 1024) (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, stages * stage + table);
+        hipLaunchKernelGGL(kernel, grid, dim3(NW * 64), stages * stage + table, st, k);
     };
     if constexpr (sizeof(T) == 2) go(seq::linear_chunk_kernel<T, KT, NW, STATE>);
     else go(seq::linear_chunk32_kernel<KT, NW, STATE>);
