@@ -46,6 +46,18 @@ __device__ __forceinline__ int keys_of(const AttnArgs& a, const SegInfo& s) {
     return a.k_len ? max(0, min(a.k_len[s.seg], s.nk)) : s.nk;
 }
 
+// Which of a tile's BK keys from `base` on are there at all: in front of `end`, and not masked.  The mask's bytes are asked
+// for a tile ahead.
+template <int BK>
+__device__ __forceinline__ int ask_keys(const AttnArgs& a, const SegInfo& s, int base, int end) {
+    const int j = base + (threadIdx.x & (BK - 1));
+    return a.key_mask && j < end ? a.key_mask[s.k0 + j] : 1;
+}
+template <int BK>
+__device__ __forceinline__ uint64_t have_keys(int asked, int base, int end) {
+    return __ballot(asked && base + (int)(threadIdx.x & (BK - 1)) < end) & (~0ull >> (64 - BK));
+}
+
 // m and l of a row to its log-sum; l = 0 where nothing was seen.
 __device__ __forceinline__ float log_sum(float m, float l) { return l == 0.0f ? -INFINITY : m + LN2 * __builtin_amdgcn_logf(l); }
 
@@ -197,12 +209,13 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
     int LO, HI, x0, x1;      // what any row of the workgroup sees
     visible(a, t.i0, t.s.nq, t.nk, LO, x0);
     visible(a, t.i0 + (t.rows - 1) / t.n_heads, t.s.nq, t.nk, x1, HI);
-    const int all_lo = x1, all_hi = x0;                        // what all of them see
     if (a.splits > 1) {
         LO += (int)min((int64_t)blockIdx.y * a.chunk, (int64_t)0x3fffffff);
         HI = min(HI, LO + a.chunk);
     }
-    const int wl = __builtin_amdgcn_readfirstlane(__shfl(lo, 0)), wh = __builtin_amdgcn_readfirstlane(__shfl(hi, 31));  // this wave's rows: they rise with the lane
+    // what any row of the wave sees, and what all of them see: they rise with the lane
+    const int wl = __builtin_amdgcn_readfirstlane(__shfl(lo, 0)), wh = __builtin_amdgcn_readfirstlane(__shfl(hi, 31));
+    const int all_lo = __builtin_amdgcn_readfirstlane(__shfl(lo, 31)), all_hi = __builtin_amdgcn_readfirstlane(__shfl(hi, 0));
 
     x8 qf[KS];
     {
@@ -221,10 +234,11 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
     const int64_t kr = a.k_row * 2, vr = a.v_row * 2;
     const TileLoad<BK, NC, 256, Swz<NC>> load_k(threadIdx.x, a.dim * 2, kr), load_v(threadIdx.x, a.dim * 2, vr);
     for (int b = 0; b < 4; ++b) load_k.clear(lds + b * TILE);
-    auto stage = [&](int base, int buf) {
+    auto stage = [&](int base, int buf, uint64_t there) {
+        if (!there) return;
         const uint32_t at = lds + buf * 2 * TILE + wave * 1024;
-        load_k(kp + base * kr, t.nk - base, at);
-        load_v(vp + base * vr, t.nk - base, at + TILE);
+        load_k.pick(kp + base * kr, there, at);
+        load_v.pick(vp + base * vr, there, at + TILE);
     };
 
     // operand reads: keys as rows, values transposed
@@ -252,32 +266,36 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[dt][r] = 0.0f;
 
+    // Keys that are not there are not loaded; a key that is stands in their places, and only what a row does not see has to
+    // be kept from it.  A tile that some of a wave's rows see only in part: values that are not finite must not meet the
+    // weight 0 of the others; if it holds any, the wave's rows are done one by one.
     bool strange = false;
-    if (LO < HI) stage(LO, 0);
+    uint64_t coming = 0;
+    int asked = 1;
+    if (LO < HI) {
+        coming = have_keys<BK>(ask_keys<BK>(a, t.s, LO, HI), LO, HI);
+        stage(LO, 0, coming);
+        asked = ask_keys<BK>(a, t.s, LO + BK, HI);
+    }
     int buf = 0;
     for (int base = LO; base < HI; base += BK, buf ^= 1) {
         wait_loads();
         __syncthreads();
-        if (base + BK < HI) stage(base + BK, buf ^ 1);
-        const uint32_t kt_ = lds + buf * 2 * TILE, vt_ = kt_ + TILE;
-
-        // A tile that some rows see only in part: values that are not finite must not meet the weight 0 of the rows that
-        // do not see them.  Rows that nobody sees are cleared; if others hold such values, the rows are done one by one.
-        uint64_t there = ~0ull;
-        const bool edge = a.key_mask || base < all_lo || base + BK > all_hi;
-        if (edge) {
-            const int j = base + lane;
-            there = __ballot(j < HI && (!a.key_mask || a.key_mask[t.s.k0 + j]));
-            int odd = 0;
-#pragma unroll
-            for (int n = 0; n < LOADS; ++n) {
-                const uint32_t at = vt_ + (n * 256 + threadIdx.x) * 16;
-                if (!((there >> load_v.row(n)) & 1)) lds_write<u32x4>(at, u32x4{0, 0, 0, 0});
-                else odd |= not_finite<T>(lds_read<u32x4>(at));
-            }
-            if (__syncthreads_or(odd)) { strange = true; break; }
+        const uint64_t there = coming;
+        if (base + BK < HI) {
+            coming = have_keys<BK>(asked, base + BK, HI);
+            stage(base + BK, buf ^ 1, coming);
+            asked = ask_keys<BK>(a, t.s, base + 2 * BK, HI);
         }
-        if (base >= wh || base + BK <= wl || wave * 32 >= t.rows) continue;         // nothing of it for this wave
+        if (!there || strange || base >= wh || base + BK <= wl || wave * 32 >= t.rows) continue;      // nothing of it for this wave
+        const uint32_t kt_ = lds + buf * 2 * TILE, vt_ = kt_ + TILE;
+        const bool edge = base < all_lo || base + BK > all_hi;
+        if (edge) {
+            bool odd = false;
+#pragma unroll
+            for (int n = 0; n < TILE / 1024; ++n) odd |= not_finite<T>(lds_read<u32x4>(vt_ + (n * 64 + lane) * 16));
+            if (__any(odd)) { strange = true; continue; }
+        }
 
         f32x16 z[2];
 #pragma unroll
@@ -287,7 +305,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
 #pragma unroll
             for (int s = 0; s < KS; ++s) z[kt] = mfma(lds_read<x8>(kt_ + koff[s] + kt * 32 * DP * 2), qf[s], z[kt]);
         }
-        if (edge) {
+        if (edge || there != ~0ull >> (64 - BK)) {
             const int from = max(lo - base, 0), to = min(hi - base, 64);
             uint64_t see = to <= from ? 0 : there & (~0ull << from) & (~0ull >> (64 - to));
             see >>= 4 * half;
@@ -340,7 +358,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
     }
     if (strange) {
         wait_loads();
-        for (int r = wave; r < t.rows; r += 4)
+        for (int r = wave * 32; r < min(t.rows, wave * 32 + 32); ++r)
             attn_row<T>(a, t.s, t.nk, t.i0 + r / t.n_heads, t.head0 + r % t.n_heads, LO, HI, blockIdx.y);
         return;
     }
@@ -363,15 +381,17 @@ __global__ __launch_bounds__(256, 2) void attn_tile32_kernel(AttnArgs a) {
     const bool row_ok = pr < t.rows;
     const int prc = row_ok ? pr : t.rows - 1;
     const int i = t.i0 + prc / t.n_heads, h = t.head0 + prc % t.n_heads;
-    int lo, hi, LO, HI, all_lo, all_hi;
+    int lo, hi, LO, HI, x0, x1;
     visible(a, i, t.s.nq, t.nk, lo, hi);
-    visible(a, t.i0, t.s.nq, t.nk, LO, all_hi);
-    visible(a, t.i0 + (t.rows - 1) / t.n_heads, t.s.nq, t.nk, all_lo, HI);
+    visible(a, t.i0, t.s.nq, t.nk, LO, x0);
+    visible(a, t.i0 + (t.rows - 1) / t.n_heads, t.s.nq, t.nk, x1, HI);
     if (a.splits > 1) {
         LO += (int)min((int64_t)blockIdx.y * a.chunk, (int64_t)0x3fffffff);
         HI = min(HI, LO + a.chunk);
     }
+    // what any row of the wave sees, and what all of them see: they rise with the lane
     const int wl = __builtin_amdgcn_readfirstlane(__shfl(lo, 0)), wh = __builtin_amdgcn_readfirstlane(__shfl(hi, 31));
+    const int all_lo = __builtin_amdgcn_readfirstlane(__shfl(lo, 31)), all_hi = __builtin_amdgcn_readfirstlane(__shfl(hi, 0));
 
     f32x4 qf[KS];                            // elements 8 s + 4 half .. of this lane's row
     {
@@ -387,10 +407,11 @@ __global__ __launch_bounds__(256, 2) void attn_tile32_kernel(AttnArgs a) {
     const int64_t kr = a.k_row * 4, vr = a.v_row * 4;
     const TileLoad<BK, NC, 256, Swz32<NC>> load_k(threadIdx.x, a.dim * 4, kr), load_v(threadIdx.x, a.dim * 4, vr);
     for (int b = 0; b < 4; ++b) load_k.clear(lds + b * TILE);
-    auto stage = [&](int base, int buf) {
+    auto stage = [&](int base, int buf, uint64_t there) {
+        if (!there) return;
         const uint32_t at = lds + buf * 2 * TILE + wave * 1024;
-        load_k(kp + base * kr, t.nk - base, at);
-        load_v(vp + base * vr, t.nk - base, at + TILE);
+        load_k.pick(kp + base * kr, there, at);
+        load_v.pick(vp + base * vr, there, at + TILE);
     };
     const float c1 = a.scale * LOG2E;
     float ref = -INFINITY, mc = 0.0f, l = 0.0f;
@@ -400,29 +421,36 @@ __global__ __launch_bounds__(256, 2) void attn_tile32_kernel(AttnArgs a) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[dt][r] = 0.0f;
 
+    // Keys that are not there are not loaded; a key that is stands in their places, and only what a row does not see has to
+    // be kept from it.  A tile that some of a wave's rows see only in part: values that are not finite must not meet the
+    // weight 0 of the others; if it holds any, the wave's rows are done one by one.
     bool strange = false;
-    if (LO < HI) stage(LO, 0);
+    uint64_t coming = 0;
+    int asked = 1;
+    if (LO < HI) {
+        coming = have_keys<BK>(ask_keys<BK>(a, t.s, LO, HI), LO, HI);
+        stage(LO, 0, coming);
+        asked = ask_keys<BK>(a, t.s, LO + BK, HI);
+    }
     int buf = 0;
     for (int base = LO; base < HI; base += BK, buf ^= 1) {
         wait_loads();
         __syncthreads();
-        if (base + BK < HI) stage(base + BK, buf ^ 1);
-        const uint32_t kt_ = lds + buf * 2 * TILE, vt_ = kt_ + TILE;
-        uint32_t there = ~0u;
-        const bool edge = a.key_mask || base < all_lo || base + BK > all_hi;
-        if (edge) {
-            const int j = base + col;
-            there = (uint32_t)__ballot(j < HI && (!a.key_mask || a.key_mask[t.s.k0 + j]));
-            int odd = 0;
-#pragma unroll
-            for (int n = 0; n < LOADS; ++n) {
-                const uint32_t at = vt_ + (n * 256 + threadIdx.x) * 16;
-                if (!((there >> load_v.row(n)) & 1)) lds_write<u32x4>(at, u32x4{0, 0, 0, 0});
-                else odd |= not_finite<float>(lds_read<u32x4>(at));
-            }
-            if (__syncthreads_or(odd)) { strange = true; break; }
+        const uint64_t there = coming;
+        if (base + BK < HI) {
+            coming = have_keys<BK>(asked, base + BK, HI);
+            stage(base + BK, buf ^ 1, coming);
+            asked = ask_keys<BK>(a, t.s, base + 2 * BK, HI);
         }
-        if (base >= wh || base + BK <= wl || wave * 32 >= t.rows) continue;
+        if (!there || strange || base >= wh || base + BK <= wl || wave * 32 >= t.rows) continue;      // nothing of it for this wave
+        const uint32_t kt_ = lds + buf * 2 * TILE, vt_ = kt_ + TILE;
+        const bool edge = base < all_lo || base + BK > all_hi;
+        if (edge) {
+            bool odd = false;
+#pragma unroll
+            for (int n = 0; n < TILE / 1024; ++n) odd |= not_finite<float>(lds_read<u32x4>(vt_ + (n * 64 + lane) * 16));
+            if (__any(odd)) { strange = true; continue; }
+        }
 
         f32x16 z;
 #pragma unroll
@@ -433,9 +461,9 @@ __global__ __launch_bounds__(256, 2) void attn_tile32_kernel(AttnArgs a) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) z = mfma(k[e], qf[s][e], z);
         }
-        if (edge) {
+        if (edge || there != ~0ull >> (64 - BK)) {
             const int from = max(lo - base, 0), to = min(hi - base, 32);
-            const uint32_t see = (to <= from ? 0 : there & (~0u << from) & (~0u >> (32 - to))) >> (4 * half);
+            const uint32_t see = (to <= from ? 0 : (uint32_t)there & (~0u << from) & (~0u >> (32 - to))) >> (4 * half);
 #pragma unroll
             for (int r = 0; r < 16; ++r) z[r] = (see >> acc_row(r, 0)) & 1 ? z[r] : -INFINITY;
         }
@@ -470,7 +498,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile32_kernel(AttnArgs a) {
     }
     if (strange) {
         wait_loads();
-        for (int r = wave; r < t.rows; r += 4)
+        for (int r = wave * 32; r < min(t.rows, wave * 32 + 32); ++r)
             attn_row<float>(a, t.s, t.nk, t.i0 + r / t.n_heads, t.head0 + r % t.n_heads, LO, HI, blockIdx.y);
         return;
     }
@@ -519,10 +547,11 @@ __global__ __launch_bounds__(NW * 64) void attn_step_kernel(AttnArgs a) {
     const uint32_t mine = lds + wave * 4 * TILE;
     const TileLoad<BK, NC, 64, std::conditional_t<F32, Swz32<NC>, Swz<NC>>> load_k(lane, a.dim * sizeof(T), kr), load_v(lane, a.dim * sizeof(T), vr);
     for (int b = 0; b < 4; ++b) load_k.clear(mine + b * TILE);
-    auto stage = [&](int base, int buf) {
+    auto stage = [&](int base, int buf, uint64_t there) {
+        if (!there) return;
         const uint32_t at = mine + buf * 2 * TILE;
-        load_k(kp + base * kr, t.nk - base, at);
-        load_v(vp + base * vr, t.nk - base, at + TILE);
+        load_k.pick(kp + base * kr, there, at);
+        load_v.pick(vp + base * vr, there, at + TILE);
     };
     const float c1 = a.scale * LOG2E;
     float ref = -INFINITY, mc = 0.0f, l = 0.0f;
@@ -533,26 +562,21 @@ __global__ __launch_bounds__(NW * 64) void attn_step_kernel(AttnArgs a) {
         for (int r = 0; r < 16; ++r) o[dt][r] = 0.0f;
     int odd = 0;
     const int first = LO + wave * BK, stride = NW * BK;
-    if (first < HI) stage(first, 0);
-    if (first + stride < HI) stage(first + stride, 1);
+    auto keys = [&](int base) { return base < HI ? have_keys<BK>(ask_keys<BK>(a, t.s, base, HI), base, HI) : 0; };
+    uint64_t there = keys(first), coming = keys(first + stride);
+    stage(first, 0, there);
+    stage(first + stride, 1, coming);
     int buf = 0;
     for (int base = first; base < HI; base += stride, buf ^= 1) {
         // this tile's loads, not the next one's
-        if (base + stride < HI) wait_loads_but<2 * LOADS>();
+        if (coming) wait_loads_but<2 * LOADS>();
         else wait_loads();
         const uint32_t kt_ = mine + buf * 2 * TILE, vt_ = kt_ + TILE;
-        uint32_t there = ~0u;
-        const bool edge = a.key_mask || base < all_lo || base + BK > all_hi || base + BK > HI;
-        if (edge) {
-            const int j = base + col;
-            there = (uint32_t)__ballot(j < HI && (!a.key_mask || a.key_mask[t.s.k0 + j]));
+        const bool edge = base < all_lo || base + BK > all_hi;
+        if (edge && there)
 #pragma unroll
-            for (int n = 0; n < LOADS; ++n) {
-                const uint32_t at = vt_ + (n * 64 + lane) * 16;
-                if (!((there >> ((n * 64 + lane) / NC)) & 1)) lds_write<u32x4>(at, u32x4{0, 0, 0, 0});
-                else odd |= not_finite<T>(lds_read<u32x4>(at));
-            }
-        }
+            for (int n = 0; n < LOADS; ++n) odd |= not_finite<T>(lds_read<u32x4>(vt_ + (n * 64 + lane) * 16));
+        if (there) {
         f32x16 z;
 #pragma unroll
         for (int r = 0; r < 16; ++r) z[r] = 0.0f;
@@ -565,9 +589,9 @@ __global__ __launch_bounds__(NW * 64) void attn_step_kernel(AttnArgs a) {
                 for (int e = 0; e < 4; ++e) z = mfma(kf[e], q[e], z);
             } else z = mfma(__builtin_bit_cast(typename Vec<T>::x8, k), __builtin_bit_cast(typename Vec<T>::x8, qf[s]), z);
         }
-        if (edge) {
+        if (edge || there != 0xffffffffu) {
             const int from = max(lo - base, 0), to = min(hi - base, 32);
-            const uint32_t see = (to <= from ? 0 : there & (~0u << from) & (~0u >> (32 - to))) >> (4 * half);
+            const uint32_t see = (to <= from ? 0 : (uint32_t)there & (~0u << from) & (~0u >> (32 - to))) >> (4 * half);
 #pragma unroll
             for (int r = 0; r < 16; ++r) z[r] = (see >> acc_row(r, 0)) & 1 ? z[r] : -INFINITY;
         }
@@ -626,9 +650,12 @@ __global__ __launch_bounds__(NW * 64) void attn_step_kernel(AttnArgs a) {
                 }
             }
         }
+        }
         // the tile is read: its place may be loaded again
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        if (base + 2 * stride < HI) stage(base + 2 * stride, buf);
+        there = coming;
+        coming = keys(base + 2 * stride);
+        stage(base + 2 * stride, buf, coming);
     }
     l = pair_sum(l);
     if (__syncthreads_or(odd)) {

@@ -127,6 +127,22 @@ struct TileLoad {
                 if (has(n) && chunk(n) < width) load_lds16(base, (uint32_t)min(row(n), rows - 1) * (uint32_t)stride + chunk(n), tile + n * THREADS * 16);
         }
     }
+    // The rows whose bit is set in `there` (one at least); in the others' places the first of these.
+    __device__ __forceinline__ void pick(const void* base, uint64_t there, uint32_t tile) const {
+        constexpr uint64_t ALL = ~0ull >> (64 - ROWS);
+        if (there == ALL && width == NC * 16) {
+#pragma unroll
+            for (int n = 0; n < LOADS; ++n)
+                if (has(n)) load_lds16(base, offset[n], tile + n * THREADS * 16);
+        } else {
+            const int first_row = __builtin_ctzll(there);
+#pragma unroll
+            for (int n = 0; n < LOADS; ++n) {
+                const int r = (there >> row(n)) & 1 ? row(n) : first_row;
+                if (has(n) && chunk(n) < width) load_lds16(base, (uint32_t)r * (uint32_t)stride + chunk(n), tile + n * THREADS * 16);
+            }
+        }
+    }
 };
 template <int NC> struct Swz { static __device__ __forceinline__ int at(int r) { return swz<NC>(r); } };
 template <int NC> struct Swz32 { static __device__ __forceinline__ int at(int r) { return swz32<NC>(r); } };
