@@ -227,6 +227,8 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
             if (d < a.dim) x = *(const u32x4*)(q + d);
             qf[s] = __builtin_bit_cast(x8, x);
         }
+#pragma unroll
+        for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(qf[s]));       // arrived: no wait for them inside the loop
     }
 
     const char* kp = (const char*)((const T*)a.k + t.s.k0 * a.k_row + (int64_t)t.kv * a.k_head);
@@ -297,13 +299,28 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
             if (__any(odd)) { strange = true; continue; }
         }
 
+        // all reads of the first 32 keys, then a read of the others behind each product
         f32x16 z[2];
+        {
+            x8 kf[2][KS];
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt) {
+            for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) z[kt][r] = 0.0f;
+                for (int s = 0; s < KS; ++s) kf[kt][s] = lds_read<x8>(kt_ + koff[s] + kt * 32 * DP * 2);
 #pragma unroll
-            for (int s = 0; s < KS; ++s) z[kt] = mfma(lds_read<x8>(kt_ + koff[s] + kt * 32 * DP * 2), qf[s], z[kt]);
+            for (int kt = 0; kt < 2; ++kt) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) z[kt][r] = 0.0f;
+#pragma unroll
+                for (int s = 0; s < KS; ++s) z[kt] = mfma(kf[kt][s], qf[s], z[kt]);
+            }
+            sched_reads(KS);
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                sched_products(1);
+                sched_reads(1);
+            }
+            sched_products(KS);
         }
         if (edge || there != ~0ull >> (64 - BK)) {
             const int from = max(lo - base, 0), to = min(hi - base, 64);

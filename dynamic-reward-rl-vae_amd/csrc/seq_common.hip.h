@@ -185,6 +185,10 @@ __device__ __forceinline__ s16x4 lds_read_tr(uint32_t at) {
 extern "C" __device__ float drl_mul_legacy(float, float) __asm("llvm.amdgcn.fmul.legacy");
 __device__ __forceinline__ float mul_legacy(float x, float y) { return drl_mul_legacy(x, y); }
 
+// The next so many LDS reads (matrix products) in this order.
+#define sched_reads(n) __builtin_amdgcn_sched_group_barrier(0x100, n, 0)
+#define sched_products(n) __builtin_amdgcn_sched_group_barrier(0x008, n, 0)
+
 // LDS reads stay on their side of this; everything else may be moved across.
 __device__ __forceinline__ void keep_reads() { __builtin_amdgcn_sched_barrier(0x67f); }
 
