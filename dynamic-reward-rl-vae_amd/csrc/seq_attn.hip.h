@@ -246,7 +246,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
     // operand reads: keys as rows, values transposed
     uint32_t koff[KS], voff[DT][2];
 #pragma unroll
-    for (int s = 0; s < KS; ++s) koff[s] = col * (DP * 2) + (((2 * s + half) ^ swz<NC>(col)) * 16);
+    for (int s = 0; s < KS; ++s) koff[s] = lds + col * (DP * 2) + (((2 * s + half) ^ swz<NC>(col)) * 16);
     {
         const int g = (lane >> 4) & 1, i4 = lane & 15;
 #pragma unroll
@@ -255,7 +255,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
             for (int j = 0; j < 2; ++j) {
                 const int r = 8 * j + 4 * half + (i4 >> 2);
                 const int c = dt * 4 + g * 2 + ((i4 & 3) >> 1);
-                voff[dt][j] = r * (DP * 2) + ((c ^ swz<NC>(r)) * 16) + (i4 & 1) * 8;
+                voff[dt][j] = lds + r * (DP * 2) + ((c ^ swz<NC>(r)) * 16) + (i4 & 1) * 8;
             }
     }
 
@@ -279,8 +279,8 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
         stage(LO, 0, coming);
         asked = ask_keys<BK>(a, t.s, LO + BK, HI);
     }
-    int buf = 0;
-    for (int base = LO; base < HI; base += BK, buf ^= 1) {
+    auto tile = [&](auto which, int base) {                    // one tile, in buffer `which`: its places are constants
+        constexpr int buf = decltype(which)::value;
         wait_loads();
         __syncthreads();
         const uint64_t there = coming;
@@ -289,14 +289,14 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
             stage(base + BK, buf ^ 1, coming);
             asked = ask_keys<BK>(a, t.s, base + 2 * BK, HI);
         }
-        if (!there || strange || base >= wh || base + BK <= wl || wave * 32 >= t.rows) continue;      // nothing of it for this wave
-        const uint32_t kt_ = lds + buf * 2 * TILE, vt_ = kt_ + TILE;
+        if (!there || strange || base >= wh || base + BK <= wl || wave * 32 >= t.rows) return;      // nothing of it for this wave
+        constexpr uint32_t kt_ = buf * 2 * TILE, vt_ = kt_ + TILE;
         const bool edge = base < all_lo || base + BK > all_hi;
         if (edge) {
             bool odd = false;
 #pragma unroll
-            for (int n = 0; n < TILE / 1024; ++n) odd |= not_finite<T>(lds_read<u32x4>(vt_ + (n * 64 + lane) * 16));
-            if (__any(odd)) { strange = true; continue; }
+            for (int n = 0; n < TILE / 1024; ++n) odd |= not_finite<T>(lds_read<u32x4>(lds + vt_ + (n * 64 + lane) * 16));
+            if (__any(odd)) { strange = true; return; }
         }
 
         // all reads of the first 32 keys, then a read of the others behind each product
@@ -306,7 +306,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-                for (int s = 0; s < KS; ++s) kf[kt][s] = lds_read<x8>(kt_ + koff[s] + kt * 32 * DP * 2);
+                for (int s = 0; s < KS; ++s) kf[kt][s] = lds_read<x8>(koff[s] + (kt_ + kt * 32 * DP * 2));
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt) {
 #pragma unroll
@@ -333,10 +333,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
                 z[1][r] = (s1 >> acc_row(r, 0)) & 1 ? z[1][r] : -INFINITY;
             }
         }
-        float m = fmaxf(z[0][0], z[1][0]);
-#pragma unroll
-        for (int r = 1; r < 16; ++r) m = fmaxf(m, fmaxf(z[0][r], z[1][r]));
-        m = pair_max(m);
+        const float m = pair_max(fmaxf(max16(z[0]), max16(z[1])));
         if (__any((m - ref) * c1 > 8.0f)) {
             const float now = fmaxf(m, ref);
             const float mcn = now == -INFINITY ? 0.0f : now * c1;
@@ -366,12 +363,16 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
         for (int s = 0; s < 4; ++s)
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) {
-                const s16x4 v0 = lds_read_tr(vt_ + voff[dt][0] + s * 16 * DP * 2);
-                const s16x4 v1 = lds_read_tr(vt_ + voff[dt][1] + s * 16 * DP * 2);
+                const s16x4 v0 = lds_read_tr(voff[dt][0] + (vt_ + s * 16 * DP * 2));
+                const s16x4 v1 = lds_read_tr(voff[dt][1] + (vt_ + s * 16 * DP * 2));
                 typedef short s16x8 __attribute__((ext_vector_type(8)));
                 const s16x8 v = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
                 o[dt] = mfma(__builtin_bit_cast(x8, v), p[s], o[dt]);
             }
+    };
+    for (int base = LO; base < HI; base += 2 * BK) {
+        tile(std::integral_constant<int, 0>(), base);
+        if (base + BK < HI) tile(std::integral_constant<int, 1>(), base + BK);
     }
     if (strange) {
         wait_loads();
@@ -484,10 +485,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile32_kernel(AttnArgs a) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) z[r] = (see >> acc_row(r, 0)) & 1 ? z[r] : -INFINITY;
         }
-        float m = z[0];
-#pragma unroll
-        for (int r = 1; r < 16; ++r) m = fmaxf(m, z[r]);
-        m = pair_max(m);
+        const float m = pair_max(max16(z));
         if (__any((m - ref) * c1 > 8.0f)) {
             const float now = fmaxf(m, ref);
             const float mcn = now == -INFINITY ? 0.0f : now * c1;
@@ -612,10 +610,7 @@ __global__ __launch_bounds__(NW * 64) void attn_step_kernel(AttnArgs a) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) z[r] = (see >> acc_row(r, 0)) & 1 ? z[r] : -INFINITY;
         }
-        float m = z[0];
-#pragma unroll
-        for (int r = 1; r < 16; ++r) m = fmaxf(m, z[r]);
-        m = pair_max(m);
+        const float m = pair_max(max16(z));
         if (__any((m - ref) * c1 > 8.0f)) {
             const float now = fmaxf(m, ref);
             const float mcn = now == -INFINITY ? 0.0f : now * c1;

@@ -185,6 +185,21 @@ __device__ __forceinline__ s16x4 lds_read_tr(uint32_t at) {
 extern "C" __device__ float drl_mul_legacy(float, float) __asm("llvm.amdgcn.fmul.legacy");
 __device__ __forceinline__ float mul_legacy(float x, float y) { return drl_mul_legacy(x, y); }
 
+// The largest of a product's 16 results.  Assembly, because the compiler quietens each NaN first and
+// takes three times the instructions; it waits for the products itself (19 states are the most that any needs).
+__device__ __forceinline__ float max16(const f32x16& x) {
+    float m, n;
+    asm("s_nop 15\n\ts_nop 3\n\t"
+        "v_max3_f32 %0, %2, %3, %4\n\tv_max3_f32 %1, %5, %6, %7\n\t"
+        "v_max3_f32 %0, %0, %8, %9\n\tv_max3_f32 %1, %1, %10, %11\n\t"
+        "v_max3_f32 %0, %0, %12, %13\n\tv_max3_f32 %1, %1, %14, %15\n\t"
+        "v_max3_f32 %0, %0, %16, %17\n\tv_max_f32 %0, %0, %1"
+        : "=&v"(m), "=&v"(n)
+        : "v"(x[0]), "v"(x[1]), "v"(x[2]), "v"(x[3]), "v"(x[4]), "v"(x[5]), "v"(x[6]), "v"(x[7]), "v"(x[8]), "v"(x[9]), "v"(x[10]),
+          "v"(x[11]), "v"(x[12]), "v"(x[13]), "v"(x[14]), "v"(x[15]));
+    return m;
+}
+
 // The next so many LDS reads (matrix products) in this order.
 #define sched_reads(n) __builtin_amdgcn_sched_group_barrier(0x100, n, 0)
 #define sched_products(n) __builtin_amdgcn_sched_group_barrier(0x008, n, 0)
