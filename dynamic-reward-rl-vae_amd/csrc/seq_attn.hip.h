@@ -302,6 +302,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
         // all reads of the first 32 keys, then a read of the others behind each product
         f32x16 z[2];
         {
+            __builtin_amdgcn_s_setprio(1);
             x8 kf[2][KS];
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt)
@@ -321,6 +322,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
                 sched_reads(1);
             }
             sched_products(KS);
+            __builtin_amdgcn_s_setprio(0);
         }
         if (edge || there != ~0ull >> (64 - BK)) {
             const int from = max(lo - base, 0), to = min(hi - base, 64);
@@ -329,10 +331,16 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
             const uint32_t s0 = (uint32_t)see, s1 = (uint32_t)(see >> 32);
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                z[0][r] = (s0 >> acc_row(r, 0)) & 1 ? z[0][r] : -INFINITY;
-                z[1][r] = (s1 >> acc_row(r, 0)) & 1 ? z[1][r] : -INFINITY;
+                z[0][r] = if_bit(s0, acc_row(r, 0), z[0][r], -INFINITY);
+                z[1][r] = if_bit(s1, acc_row(r, 0), z[1][r], -INFINITY);
             }
         }
+        s16x4 va[DT][2];                                       // the first values' reads, before the softmax
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) va[dt][j] = lds_read_tr(voff[dt][j] + vt_);
+        __builtin_amdgcn_sched_barrier(0);
         const float m = pair_max(fmaxf(max16(z[0]), max16(z[1])));
         if (__any((m - ref) * c1 > 8.0f)) {
             const float now = fmaxf(m, ref);
@@ -363,12 +371,18 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
         for (int s = 0; s < 4; ++s)
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) {
-                const s16x4 v0 = lds_read_tr(voff[dt][0] + (vt_ + s * 16 * DP * 2));
-                const s16x4 v1 = lds_read_tr(voff[dt][1] + (vt_ + s * 16 * DP * 2));
+                const s16x4 v0 = s == 0 ? va[dt][0] : lds_read_tr(voff[dt][0] + (vt_ + s * 16 * DP * 2));
+                const s16x4 v1 = s == 0 ? va[dt][1] : lds_read_tr(voff[dt][1] + (vt_ + s * 16 * DP * 2));
                 typedef short s16x8 __attribute__((ext_vector_type(8)));
                 const s16x8 v = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
                 o[dt] = mfma(__builtin_bit_cast(x8, v), p[s], o[dt]);
             }
+#pragma unroll
+        for (int n = 0; n < 3 * DT; ++n) {                     // a read ahead of each product
+            sched_reads(2);
+            sched_products(1);
+        }
+        sched_products(DT);
     };
     for (int base = LO; base < HI; base += 2 * BK) {
         tile(std::integral_constant<int, 0>(), base);
@@ -483,7 +497,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile32_kernel(AttnArgs a) {
             const int from = max(lo - base, 0), to = min(hi - base, 32);
             const uint32_t see = (to <= from ? 0 : (uint32_t)there & (~0u << from) & (~0u >> (32 - to))) >> (4 * half);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) z[r] = (see >> acc_row(r, 0)) & 1 ? z[r] : -INFINITY;
+            for (int r = 0; r < 16; ++r) z[r] = if_bit(see, acc_row(r, 0), z[r], -INFINITY);
         }
         const float m = pair_max(max16(z));
         if (__any((m - ref) * c1 > 8.0f)) {
@@ -608,7 +622,7 @@ __global__ __launch_bounds__(NW * 64) void attn_step_kernel(AttnArgs a) {
             const int from = max(lo - base, 0), to = min(hi - base, 32);
             const uint32_t see = (to <= from ? 0 : (uint32_t)there & (~0u << from) & (~0u >> (32 - to))) >> (4 * half);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) z[r] = (see >> acc_row(r, 0)) & 1 ? z[r] : -INFINITY;
+            for (int r = 0; r < 16; ++r) z[r] = if_bit(see, acc_row(r, 0), z[r], -INFINITY);
         }
         const float m = pair_max(max16(z));
         if (__any((m - ref) * c1 > 8.0f)) {

@@ -200,6 +200,12 @@ __device__ __forceinline__ float max16(const f32x16& x) {
     return m;
 }
 
+// x where bit n of `bits` is set, else y: two instructions, and no lane mask between.
+__device__ __forceinline__ float if_bit(uint32_t bits, int n, float x, float y) {
+    const uint32_t m = (uint32_t)__builtin_amdgcn_sbfe((int)bits, n, 1);
+    return __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, x) & m) | (__builtin_bit_cast(uint32_t, y) & ~m));
+}
+
 // The next so many LDS reads (matrix products) in this order.
 #define sched_reads(n) __builtin_amdgcn_sched_group_barrier(0x100, n, 0)
 #define sched_products(n) __builtin_amdgcn_sched_group_barrier(0x008, n, 0)
