@@ -135,11 +135,13 @@ struct TileLoad {
             for (int n = 0; n < LOADS; ++n)
                 if (has(n)) load_lds16(base, offset[n], tile + n * THREADS * 16);
         } else {
-            const int first_row = __builtin_ctzll(there);
+            const uint32_t lo = (uint32_t)there, hi = (uint32_t)(there >> 32), instead = __builtin_ctzll(there) * (uint32_t)stride;
 #pragma unroll
             for (int n = 0; n < LOADS; ++n) {
-                const int r = (there >> row(n)) & 1 ? row(n) : first_row;
-                if (has(n) && chunk(n) < width) load_lds16(base, (uint32_t)r * (uint32_t)stride + chunk(n), tile + n * THREADS * 16);
+                constexpr int STEP = THREADS / NC;             // rows that go at once
+                const uint32_t word = ROWS <= 32 ? lo : STEP <= 32 ? (n * STEP < 32 ? lo : hi) : row(n) < 32 ? lo : hi;
+                const uint32_t off = (word >> (row(n) & 31)) & 1 ? offset[n] : instead + chunk(n);
+                if (has(n) && chunk(n) < width) load_lds16(base, off, tile + n * THREADS * 16);
             }
         }
     }
