@@ -227,8 +227,6 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
             if (d < a.dim) x = *(const u32x4*)(q + d);
             qf[s] = __builtin_bit_cast(x8, x);
         }
-#pragma unroll
-        for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(qf[s]));       // arrived: no wait for them inside the loop
     }
 
     const char* kp = (const char*)((const T*)a.k + t.s.k0 * a.k_row + (int64_t)t.kv * a.k_head);
@@ -279,6 +277,9 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
         stage(LO, 0, coming);
         asked = ask_keys<BK>(a, t.s, LO + BK, HI);
     }
+    // q has arrived: no wait for it inside the loop, where it would be one for the keys to come
+#pragma unroll
+    for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(qf[s]));
     auto tile = [&](auto which, int base) {                    // one tile, in buffer `which`: its places are constants
         constexpr int buf = decltype(which)::value;
         wait_loads();
@@ -464,6 +465,9 @@ __global__ __launch_bounds__(256, 2) void attn_tile32_kernel(AttnArgs a) {
         stage(LO, 0, coming);
         asked = ask_keys<BK>(a, t.s, LO + BK, HI);
     }
+    // q has arrived: no wait for it inside the loop, where it would be one for the keys to come
+#pragma unroll
+    for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(qf[s]));
     int buf = 0;
     for (int base = LO; base < HI; base += BK, buf ^= 1) {
         wait_loads();
@@ -493,6 +497,13 @@ __global__ __launch_bounds__(256, 2) void attn_tile32_kernel(AttnArgs a) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) z = mfma(k[e], qf[s][e], z);
         }
+        sched_reads(2);
+#pragma unroll
+        for (int s = 0; s < KS - 2; ++s) {
+            sched_products(4);
+            sched_reads(1);
+        }
+        sched_products(8);
         if (edge || there != ~0ull >> (64 - BK)) {
             const int from = max(lo - base, 0), to = min(hi - base, 32);
             const uint32_t see = (to <= from ? 0 : (uint32_t)there & (~0u << from) & (~0u >> (32 - to))) >> (4 * half);
@@ -524,6 +535,13 @@ __global__ __launch_bounds__(256, 2) void attn_tile32_kernel(AttnArgs a) {
             for (int dt = 0; dt < DT; ++dt)
                 o[dt] = mfma(lds_read<float>(vt_ + row * (DP * 4) + (((dt * 8 + (col >> 2)) ^ swz32<NC>(row)) * 16) + (col & 3) * 4), z[r], o[dt]);
         }
+        sched_reads(4);                                        // reads four products ahead
+#pragma unroll
+        for (int n = 0; n < 16 * DT - 4; ++n) {
+            sched_products(1);
+            sched_reads(1);
+        }
+        sched_products(4);
     }
     if (strange) {
         wait_loads();
@@ -595,6 +613,9 @@ __global__ __launch_bounds__(NW * 64) void attn_step_kernel(AttnArgs a) {
     uint64_t there = keys(first), coming = keys(first + stride);
     stage(first, 0, there);
     stage(first + stride, 1, coming);
+    // q has arrived: no wait for it inside the loop, where it would be one for the keys to come
+#pragma unroll
+    for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(qf[s]));
     int buf = 0;
     for (int base = first; base < HI; base += stride, buf ^= 1) {
         // this tile's loads, not the next one's

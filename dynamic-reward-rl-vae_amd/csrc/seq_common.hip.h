@@ -47,17 +47,23 @@ __device__ __forceinline__ float wave_sum(float x) {
 }
 
 // The entry that holds unit `t` when the entries own floor(cum / per) + index .. units (a tiling of each series in
-// blocks of `per` rows, at most one empty unit per series): the last s with floor(cum_s / per) + s <= t.  64-ary search,
-// one load per lane and round.
+// blocks of `per` rows, at most one empty unit per series): the last s with floor(cum_s / per) + s <= t.  Four entries per
+// lane and round: one round of loads up to 256 series.
 __device__ __forceinline__ int find_seg(const SegInfo* segs, int n_seg, int64_t t, int per) {
     const int lane = threadIdx.x & 63;
     int lo = 0, hi = n_seg;                   // answer in [lo, hi)
     while (hi - lo > 1) {
-        const int step = (hi - lo + 63) / 64;
-        const int at = lo + lane * step;
-        const bool below = at < hi && segs[at].cum / per + at <= t;
-        const int n = __popcll(__ballot(below));      // lane 0 is always below
-        lo = lo + (n - 1) * step;
+        const int step = (hi - lo + 255) / 256;
+        int below = 0;
+        int64_t cum[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) cum[k] = segs[min(lo + (lane + 64 * k) * step, hi - 1)].cum;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int at = lo + (lane + 64 * k) * step;
+            below += __popcll(__ballot(at < hi && cum[k] / per + at <= t));
+        }
+        lo = lo + (below - 1) * step;         // the first of them is always below
         hi = min(hi, lo + step);
     }
     return __builtin_amdgcn_readfirstlane(lo);

@@ -151,22 +151,6 @@ __global__ __launch_bounds__(NW * 64, STATE ? 3 : 2) void linear_chunk_kernel(Li
     const bool on = c0 + col < a.dv;
     const float ld2 = decay_log(a, h) * LOG2E;
 
-    // the state
-    f32x16 S[KT];
-    const float* from = nullptr;
-    if (!STATE) from = a.states ? a.states + (t.u * a.heads + h) * (int64_t)a.dk * a.dv
-                                : a.state_in ? a.state_in + ((int64_t)t.s.seg * a.heads + h) * (int64_t)a.dk * a.dv : nullptr;
-    const uint32_t lane_s = 4 * half * a.dv + c0 + col;         // state element of a register: a row of the wave's plus the lane's
-#pragma unroll
-    for (int kt = 0; kt < KT; ++kt) {
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const int d = kt * 32 + acc_row(r, 0);
-            S[kt][r] = from && on && d < a.dk ? (from + d * a.dv)[lane_s] : 0.0f;    // dk is a multiple of 8: d + 4 is inside too
-        }
-    }
-
     const int64_t row0 = t.s.q0 + t.first;
     const char* qp = (const char*)((const T*)a.q + row0 * a.q_row + (int64_t)h * a.q_head);
     const char* kp = (const char*)((const T*)a.k + row0 * a.k_row + (int64_t)(h / a.rep) * a.k_head);
@@ -184,6 +168,25 @@ __global__ __launch_bounds__(NW * 64, STATE ? 3 : 2) void linear_chunk_kernel(Li
         load_v(vp + base * a.v_row * 2, t.rows - base, at + QK);
         if (!STATE) load_q(qp + base * a.q_row * 2, t.rows - base, at + QK + VB);
     };
+    if (t.rows > 0) stage(0, 0);
+    if (t.rows > C) stage(C, 1);
+
+    // the state
+    f32x16 S[KT];
+    const float* from = nullptr;
+    if (!STATE) from = a.states ? a.states + (t.u * a.heads + h) * (int64_t)a.dk * a.dv
+                                : a.state_in ? a.state_in + ((int64_t)t.s.seg * a.heads + h) * (int64_t)a.dk * a.dv : nullptr;
+    const uint32_t lane_s = 4 * half * a.dv + c0 + col;         // state element of a register: a row of the wave's plus the lane's
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) {
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int d = kt * 32 + acc_row(r, 0);
+            S[kt][r] = from && on && d < a.dk ? (from + d * a.dv)[lane_s] : 0.0f;    // dk is a multiple of 8: d + 4 is inside too
+        }
+    }
+
 
     // LDS places: rows in the order of the accumulators' registers (two reads of 4), and transposed.  Chunk c lies at place
     // c ^ swz of its row, so that one place gives the others by an exclusive or (tiles begin at whole rows).
@@ -223,11 +226,12 @@ __global__ __launch_bounds__(NW * 64, STATE ? 3 : 2) void linear_chunk_kernel(Li
     float fall = expm1f(decay_log(a, h) * (float)C);           // lam^n - 1: lam^n itself, rounded, would drift over many chunks
 
     T* op = (T*)a.out + row0 * a.o_row + (int64_t)h * a.o_head + c0;
+    // the state has arrived: no wait for it inside the loop, where it would be one for the chunks to come
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) asm volatile("" : "+v"(S[kt]));
     // Loads run two chunks ahead.  AHEAD: how many a wave issues for a chunk, at least; STORES: what it stores of one.
     constexpr int AHEAD = (STATE ? 1 : 2) * (C * NC / THREADS) + C * VC / THREADS, STORES = STATE ? 0 : 2;
     const bool stores = c0 < a.dv;
-    if (t.rows > 0) stage(0, 0);
-    if (t.rows > C) stage(C, 1);
     int buf = 0, far = 2;
     for (int base = 0; base < t.rows; base += C, far = buf, buf = buf == 2 ? 0 : buf + 1) {
         const int n = min(C, t.rows - base);
@@ -429,18 +433,6 @@ __global__ __launch_bounds__(NW * 64) void linear_chunk32_kernel(LinearArgs a) {
     const int c0 = blk * VP + wave * 32;
     const bool on = c0 + col < a.dv;
     const float ld2 = decay_log(a, h) * LOG2E;
-    f32x16 S[KT];
-    const float* from = nullptr;
-    if (!STATE) from = a.states ? a.states + (t.u * a.heads + h) * (int64_t)a.dk * a.dv
-                                : a.state_in ? a.state_in + ((int64_t)t.s.seg * a.heads + h) * (int64_t)a.dk * a.dv : nullptr;
-    const uint32_t lane_s = 4 * half * a.dv + c0 + col;
-#pragma unroll
-    for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const int d = kt * 32 + acc_row(r, 0);
-            S[kt][r] = from && on && d < a.dk ? (from + d * a.dv)[lane_s] : 0.0f;
-        }
     const int64_t row0 = t.s.q0 + t.first;
     const char* qp = (const char*)((const float*)a.q + row0 * a.q_row + (int64_t)h * a.q_head);
     const char* kp = (const char*)((const float*)a.k + row0 * a.k_row + (int64_t)(h / a.rep) * a.k_head);
@@ -458,13 +450,29 @@ __global__ __launch_bounds__(NW * 64) void linear_chunk32_kernel(LinearArgs a) {
         load_v(vp + base * a.v_row * 4, t.rows - base, at + QK);
         if (!STATE) load_q(qp + base * a.q_row * 4, t.rows - base, at + QK + VB);
     };
+    if (t.rows > 0) stage(0, 0);
+
+    f32x16 S[KT];
+    const float* from = nullptr;
+    if (!STATE) from = a.states ? a.states + (t.u * a.heads + h) * (int64_t)a.dk * a.dv
+                                : a.state_in ? a.state_in + ((int64_t)t.s.seg * a.heads + h) * (int64_t)a.dk * a.dv : nullptr;
+    const uint32_t lane_s = 4 * half * a.dv + c0 + col;
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int d = kt * 32 + acc_row(r, 0);
+            S[kt][r] = from && on && d < a.dk ? (from + d * a.dv)[lane_s] : 0.0f;
+        }
+
     float up[16];
 #pragma unroll
     for (int r = 0; r < 16; ++r) up[r] = uniform(power(ld2, acc_row(r, 0)));
     const float lane_up = a.scale * power(ld2, 4 * half + 1), lane_left = power(ld2, 4 - 4 * half);
     float fall = expm1f(decay_log(a, h) * (float)C);
     float* op = (float*)a.out + row0 * a.o_row + (int64_t)h * a.o_head;
-    if (t.rows > 0) stage(0, 0);
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) asm volatile("" : "+v"(S[kt]));        // arrived
     int buf = 0;
     for (int base = 0; base < t.rows; base += C, buf ^= 1) {
         const int n = min(C, t.rows - base);
