@@ -127,18 +127,17 @@ struct AttnTile {
     int nk, kv, head0, n_heads, i0, rows;     // rows: (row, head) pairs
     bool any;
 };
-__device__ __forceinline__ AttnTile attn_tile(const AttnArgs& a, int64_t id) {
+__device__ __forceinline__ AttnTile attn_tile(const AttnArgs& a, uint32_t id) {
     AttnTile t;
-    const int b = (int)(id % a.kv_blocks);
-    const int64_t u = id / a.kv_blocks;
+    const uint32_t b = id % (uint32_t)a.kv_blocks, u = id / (uint32_t)a.kv_blocks;
     const int slot = find_seg(a.segs, a.n_seg, u, a.per);
     t.s = a.segs[slot];
-    t.kv = b / a.blocks;
-    const int first = (b % a.blocks) * a.rep_b;
+    t.kv = b / (uint32_t)a.blocks;
+    const int first = (int)(b % (uint32_t)a.blocks) * a.rep_b;
     t.head0 = t.kv * a.rep + first;
     t.n_heads = min(a.rep_b, a.rep - first);
-    const int n = (t.s.nq + a.per - 1) / a.per;
-    const int k = (int)(u - (t.s.cum / a.per + slot));
+    const int n = (int)(((uint32_t)t.s.nq + a.per - 1) / (uint32_t)a.per);
+    const int k = (int)(u - (t.s.cum / (uint32_t)a.per + slot));
     t.any = k < n && t.n_heads > 0;
     t.i0 = (n - 1 - k) * a.per;
     t.rows = t.any ? min(a.per, t.s.nq - t.i0) * t.n_heads : 0;

@@ -26,10 +26,9 @@ __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_ex
 // the total.
 struct SegInfo {
     int64_t q0, k0;       // first row in q / k
-    int64_t cum;
+    uint32_t cum;
     int32_t nq, nk;
     int32_t seg;          // its number in the caller's order
-    int32_t pad;
 };
 
 // A value that is the same in all lanes, into a scalar register.
@@ -49,13 +48,13 @@ __device__ __forceinline__ float wave_sum(float x) {
 // The entry that holds unit `t` when the entries own floor(cum / per) + index .. units (a tiling of each series in
 // blocks of `per` rows, at most one empty unit per series): the last s with floor(cum_s / per) + s <= t.  Four entries per
 // lane and round: one round of loads up to 256 series.
-__device__ __forceinline__ int find_seg(const SegInfo* segs, int n_seg, int64_t t, int per) {
+__device__ __forceinline__ int find_seg(const SegInfo* segs, int n_seg, uint32_t t, uint32_t per) {
     const int lane = threadIdx.x & 63;
     int lo = 0, hi = n_seg;                   // answer in [lo, hi)
     while (hi - lo > 1) {
         const int step = (hi - lo + 255) / 256;
         int below = 0;
-        int64_t cum[4];
+        uint32_t cum[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) cum[k] = segs[min(lo + (lane + 64 * k) * step, hi - 1)].cum;
 #pragma unroll

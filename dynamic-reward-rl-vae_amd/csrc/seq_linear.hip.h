@@ -39,13 +39,13 @@ struct LinearUnit {
     int first, rows;              // rows of the series in this piece
     bool any, last;
 };
-__device__ __forceinline__ LinearUnit linear_unit(const LinearArgs& a, int64_t u) {
+__device__ __forceinline__ LinearUnit linear_unit(const LinearArgs& a, uint32_t u) {
     LinearUnit t;
     t.u = u;
     const int slot = find_seg(a.segs, a.n_seg, u, a.piece);
     t.s = a.segs[slot];
-    const int k = (int)(u - (t.s.cum / a.piece + slot));
-    const int n = max(1, (int)(((int64_t)t.s.nq + a.piece - 1) / a.piece));
+    const int k = (int)(u - (t.s.cum / (uint32_t)a.piece + slot));
+    const int n = max(1, (int)(((uint32_t)t.s.nq + a.piece - 1) / (uint32_t)a.piece));
     t.any = k < n;
     t.last = k == n - 1;
     t.first = k * a.piece;
@@ -572,11 +572,11 @@ static __global__ __launch_bounds__(256) void linear_scan_kernel(LinearArgs a) {
     const int64_t size = (int64_t)a.dk * a.dv, e = ((int64_t)blockIdx.z * 256 + threadIdx.x) * 4;
     if (e >= size) return;
     const SegInfo s = a.segs[slot];
-    const int n = max(1, (int)(((int64_t)s.nq + a.piece - 1) / a.piece));
+    const int n = max(1, (int)(((uint32_t)s.nq + a.piece - 1) / (uint32_t)a.piece));
     const float fall = expm1f(decay_log(a, h) * (float)a.piece);
     f32x4 S = {0.0f, 0.0f, 0.0f, 0.0f};
     if (a.state_in) S = *(const f32x4*)(a.state_in + ((int64_t)s.seg * a.heads + h) * size + e);
-    float* at = a.states + ((s.cum / a.piece + slot) * a.heads + h) * size + e;
+    float* at = a.states + ((int64_t)(s.cum / (uint32_t)a.piece + slot) * a.heads + h) * size + e;
     const int64_t next = a.heads * size;
     *(f32x4*)at = S;
     constexpr int U = 8;                                       // pieces in flight

@@ -152,8 +152,8 @@ __global__ __launch_bounds__(256) void norm_series_kernel(NormArgs a) {
     __shared__ float stat[256][2];
     const int slot = find_seg(a.segs, a.n_seg, blockIdx.x, a.piece);
     const SegInfo s = a.segs[slot];
-    const int64_t unit0 = s.cum / a.piece + slot;
-    const int k = (int)(blockIdx.x - unit0), units = (int)(((int64_t)s.nq + a.piece - 1) / a.piece);
+    const uint32_t unit0 = s.cum / (uint32_t)a.piece + slot;
+    const int k = (int)(blockIdx.x - unit0), units = (int)(((uint32_t)s.nq + a.piece - 1) / (uint32_t)a.piece);
     if (k >= units) return;
     const int first = k * a.piece, rows = min(a.piece, s.nq - first);
     const int cg = a.channels / a.groups, g0 = blockIdx.y * a.slice, ng = min(a.slice, a.groups - g0);
@@ -227,7 +227,7 @@ __global__ __launch_bounds__(256) void norm_series_kernel(NormArgs a) {
         for (int g = threadIdx.x >> 6; g < ng; g += 4) {
             Moments t = {0.0f, 0.0f, 0.0f};
             for (int u = threadIdx.x & 63; u < units; u += 64) {
-                const float* o = a.part + ((unit0 + u) * a.groups + g0 + g) * 2;
+                const float* o = a.part + ((int64_t)(unit0 + u) * a.groups + g0 + g) * 2;
                 t = join(t, {(float)min(a.piece, s.nq - u * a.piece) * (float)cg, o[0], o[1]});
             }
             t = join_lanes(t, 64);

@@ -98,15 +98,15 @@ int drl_seq_layout_create(drl_ctx* c, const int64_t* qo, const int64_t* ko, int 
             return qa != qb ? qa > qb : ko[a + 1] - ko[a] > ko[b + 1] - ko[b];
         });
         std::vector<seq::SegInfo> segs((size_t)n_seg + 1);
-        int64_t cum = 0;
+        uint32_t cum = 0;
         for (int i = 0; i < n_seg; ++i) {
             const int s = order[i];
-            segs[i] = {qo[s], ko[s], cum, (int32_t)(qo[s + 1] - qo[s]), (int32_t)(ko[s + 1] - ko[s]), s, 0};
+            segs[i] = {qo[s], ko[s], cum, (int32_t)(qo[s + 1] - qo[s]), (int32_t)(ko[s + 1] - ko[s]), s};
             cum += segs[i].nq;
             l->max_q = std::max(l->max_q, segs[i].nq);
             l->max_k = std::max(l->max_k, segs[i].nk);
         }
-        segs[n_seg] = {qo[n_seg], ko[n_seg], cum, 0, 0, n_seg, 0};
+        segs[n_seg] = {qo[n_seg], ko[n_seg], cum, 0, 0, n_seg};
         const size_t bytes = segs.size() * sizeof(segs[0]);
         drl_count_alloc();
         hipError_t err = hipMalloc((void**)&l->segs, bytes);
