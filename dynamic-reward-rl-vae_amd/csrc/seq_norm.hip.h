@@ -79,17 +79,23 @@ __global__ __launch_bounds__(256) void norm_rows_kernel(NormArgs a) {
                 ga[n][e] = a.gamma && in ? a.gamma[c] : 1.0f;
                 be[n][e] = a.beta && in ? a.beta[c] : 0.0f;
             }
+        auto load = [&](int64_t row, P (&p)[NV]) {
+#pragma unroll
+            for (int n = 0; n < NV; ++n) {
+                p[n] = P{};
+                if (on && sub + n * a.lanes < nv) p[n] = *(const P*)((const T*)a.x + row * a.x_row + c0 + (sub + n * a.lanes) * V);
+            }
+        };
+        P next[NV];
+        if (id / sets < a.rows) load(id / sets, next);
         for (int64_t row = id / sets; row < a.rows; row += step) {
-            const T* x = (const T*)a.x + row * a.x_row + c0;
             T* y = (T*)a.y + row * a.y_row + c0;
             float f[NV][V], s = 0.0f;
 #pragma unroll
-            for (int n = 0; n < NV; ++n) {
-                P p = {};
-                if (on && sub + n * a.lanes < nv) p = *(const P*)(x + (sub + n * a.lanes) * V);
+            for (int n = 0; n < NV; ++n)
 #pragma unroll
-                for (int e = 0; e < V; ++e) s += f[n][e] = (float)p.e[e];
-            }
+                for (int e = 0; e < V; ++e) s += f[n][e] = (float)next[n].e[e];
+            if (row + step < a.rows) load(row + step, next);          // on its way while this row is done
             const float mean = sum(s) * inv;
             float d2 = 0.0f;
 #pragma unroll
@@ -139,6 +145,65 @@ __global__ __launch_bounds__(256) void norm_rows_kernel(NormArgs a) {
                 }
         }
     }
+}
+
+// Short series: a workgroup has one group of one series in registers, R packs of V channels per thread, and sums it in two
+// passes over them: x is read once, in one launch.
+template <typename T, int V, int R, int THREADS>
+__global__ __launch_bounds__(THREADS) void norm_short_kernel(NormArgs a) {
+    typedef Pack<T, V> P;
+    __shared__ float red[2][THREADS / 64];
+    // a series' groups share lines of memory: one XCD (the workgroup's number modulo 8) does all of them, one after the other
+    const uint32_t eight = blockIdx.x / 8, slot = eight / a.groups * 8 + blockIdx.x % 8;
+    if (slot >= (uint32_t)a.n_seg) return;
+    const SegInfo s = a.segs[slot];
+    if (s.nq == 0) return;
+    const int cg = a.channels / a.groups, per = cg / V, packs = s.nq * per, c0 = (int)(eight % a.groups) * cg;
+    const T* x = (const T*)a.x + s.q0 * a.x_row + c0;
+    T* y = (T*)a.y + s.q0 * a.y_row + c0;
+    auto sum = [&](float v, int k) {
+        v = wave_sum(v);
+        if ((threadIdx.x & 63) == 0) red[k][threadIdx.x >> 6] = v;
+        __syncthreads();
+        float all = 0.0f;
+#pragma unroll
+        for (int w = 0; w < THREADS / 64; ++w) all += red[k][w];
+        return all;
+    };
+    P p[R];
+    float f = 0.0f;
+    int row[R], pos[R];
+#pragma unroll
+    for (int n = 0; n < R; ++n) {
+        const uint32_t i = n * THREADS + threadIdx.x;
+        row[n] = i / (uint32_t)per;
+        pos[n] = (i - row[n] * per) * V;
+        if (i < (uint32_t)packs) p[n] = *(const P*)(x + (int64_t)row[n] * a.x_row + pos[n]);
+    }
+#pragma unroll
+    for (int n = 0; n < R; ++n)
+        if (n * THREADS + (int)threadIdx.x < packs)
+#pragma unroll
+            for (int e = 0; e < V; ++e) f += (float)p[n].e[e];
+    const float inv = 1.0f / (float)(s.nq * cg), mean = sum(f, 0) * inv;
+    f = 0.0f;
+#pragma unroll
+    for (int n = 0; n < R; ++n)
+        if (n * THREADS + (int)threadIdx.x < packs)
+#pragma unroll
+            for (int e = 0; e < V; ++e) { const float d = (float)p[n].e[e] - mean; f = fmaf(d, d, f); }
+    const float rstd = 1.0f / sqrtf(fmaf(sum(f, 1), inv, a.eps));
+#pragma unroll
+    for (int n = 0; n < R; ++n)
+        if (n * THREADS + (int)threadIdx.x < packs) {
+            P q;
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const int c = c0 + pos[n] + e;
+                q.e[e] = (T)activate(fmaf(((float)p[n].e[e] - mean) * rstd, a.gamma ? a.gamma[c] : 1.0f, a.beta ? a.beta[c] : 0.0f), a.act);
+            }
+            *(P*)(y + (int64_t)row[n] * a.y_row + pos[n]) = q;
+        }
 }
 
 // Series.  A workgroup has `piece` rows of one series and `slice` groups of channels; a thread has a pack of V channels
