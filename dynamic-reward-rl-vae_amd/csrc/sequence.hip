@@ -154,12 +154,15 @@ static AttnPlan attn_plan(const DrlCtxView& v, const drl_seq_layout* l, const dr
     p.few = (int64_t)std::min(l->max_q, p.per) * p.rep_b <= 32;
     p.tiles = (l->n_q / p.per + l->rows.n_seg) * (int64_t)(a->n_kv_heads * p.blocks);
     p.splits = 1;
-    // keys one tile can see; runs of at least 256 of them, for 8 workgroups per CU (two are resident at a time: series
-    // of different lengths then still end together)
+    // Keys one tile can see, cut into runs where the tiles are fewer than what is resident at once: steps one workgroup per
+    // CU (two where their LDS lets them), others two.  More and shorter runs only add the reading of q and the joining (16
+    // caches of up to 32,768 rows: 256 us at one run per CU, 275 at two, 265 at eight; one of 30,000: 33, 41, 62; 8,192
+    // rows of two heads: 71 us at two, 85 at eight, 169 whole).
     const int64_t most = a->window > 0 && a->causal ? std::min<int64_t>(l->max_k, (int64_t)a->window + p.per) : l->max_k;
-    if (most > 512 && p.tiles < 2 * v.n_cu) {
-        const int64_t want = (8 * v.n_cu + p.tiles - 1) / p.tiles;
-        const int64_t chunk = std::max<int64_t>(256, ((most + want - 1) / want + 63) / 64 * 64);
+    const int64_t room = p.few && (call->dtype == DRL_F32 ? a->dim > 32 : a->dim > 64) ? v.n_cu : 2 * v.n_cu, least = p.few && call->dtype == DRL_F32 ? 128 : 256;
+    const int64_t want = p.tiles > 0 ? (room + p.tiles / 2) / p.tiles : 1;
+    if (most > 2 * least && want > 1) {
+        const int64_t chunk = std::max<int64_t>(least, ((most + want - 1) / want + 63) / 64 * 64);
         p.splits = (int)((most + chunk - 1) / chunk);
         p.chunk = (int)chunk;
     }
