@@ -401,7 +401,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
 // float32.  The same on 32x32x2 products, with tiles of 32 keys: the matrix pipe is 16 times slower, and what it does takes
 // most of the time.  Here a score register is at once an operand of values^T x weights, and nothing is rounded.
 template <int DT>
-__global__ __launch_bounds__(256, 2) void attn_tile32_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, DT > 2 ? 1 : 2) void attn_tile32_kernel(AttnArgs a) {
     constexpr int DP = DT <= 1 ? 32 : DT <= 2 ? 64 : 128, NC = DP / 4, KS = 4 * DT, BK = 32;
     constexpr int TILE = BK * DP * 4, LOADS = BK * NC / 256;
     extern __shared__ char smem[];

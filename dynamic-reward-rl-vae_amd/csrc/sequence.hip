@@ -6,6 +6,9 @@
 #include "seq_norm.hip.h"
 
 #include <algorithm>
+#include <cmath>
+#include <map>
+#include <mutex>
 #include <new>
 #include <numeric>
 #include <vector>
@@ -17,12 +20,79 @@ struct drl_seq_layout {
     int64_t q_first = 0;
     int max_q = 0, max_k = 0;
     seq::SegInfo* segs = nullptr;     // device, n_seg + 1 entries
+    size_t bytes = 0;
 };
 
 namespace {
 
 using seq::bf16;
 using seq::f16;
+
+// Device memory of the layouts' tables.  Small ones come out of slabs: a layout is made for every new batch, and asking the
+// runtime for memory takes longer than the rest of it.  A table given back may still be read by work under way, on any
+// stream: it waits among the retired until the device has been waited for once, which happens when many have gathered.
+class TablePool {
+    static constexpr size_t SLAB = 256 << 10, LARGEST = 32 << 10, MOST_RETIRED = 64;
+    std::mutex mu;
+    std::vector<void*> free_[16], retired[16];       // by size: 256 bytes << k
+    char* slab = nullptr;
+    size_t left = 0, n_retired = 0;
+    static int size_class(size_t bytes) {
+        int k = 0;
+        while (((size_t)256 << k) < bytes) ++k;
+        return k;
+    }
+
+public:
+    hipError_t get(size_t bytes, void** p) {
+        if (bytes > LARGEST) {
+            drl_count_alloc();
+            return hipMalloc(p, bytes);
+        }
+        std::lock_guard<std::mutex> lk(mu);
+        const int k = size_class(bytes);
+        if (free_[k].empty() && n_retired >= MOST_RETIRED && hipDeviceSynchronize() == hipSuccess) {
+            for (int i = 0; i < 16; ++i) {
+                free_[i].insert(free_[i].end(), retired[i].begin(), retired[i].end());
+                retired[i].clear();
+            }
+            n_retired = 0;
+        }
+        if (!free_[k].empty()) {
+            *p = free_[k].back();
+            free_[k].pop_back();
+            return hipSuccess;
+        }
+        const size_t size = (size_t)256 << k;
+        if (left < size) {
+            void* fresh = nullptr;
+            drl_count_alloc();
+            const hipError_t err = hipMalloc(&fresh, SLAB);
+            if (err != hipSuccess) return err;
+            slab = (char*)fresh;
+            left = SLAB;
+        }
+        *p = slab;
+        slab += size;
+        left -= size;
+        return hipSuccess;
+    }
+    void put(void* p, size_t bytes) {
+        if (bytes > LARGEST) {
+            (void)hipFree(p);
+            return;
+        }
+        std::lock_guard<std::mutex> lk(mu);
+        retired[size_class(bytes)].push_back(p);
+        ++n_retired;
+    }
+};
+TablePool& table_pool(int device) {
+    static std::mutex mu;
+    static auto* pools = new std::map<int, TablePool>();       // never destroyed: layouts may be, after everything else
+    std::lock_guard<std::mutex> lk(mu);
+    return (*pools)[device];
+}
 
 // The context's GPU is current inside a call; the caller's is again behind it.
 struct DeviceGuard {
@@ -108,15 +178,16 @@ int drl_seq_layout_create(drl_ctx* c, const int64_t* qo, const int64_t* ko, int 
         }
         segs[n_seg] = {qo[n_seg], ko[n_seg], cum, 0, 0, n_seg};
         const size_t bytes = segs.size() * sizeof(segs[0]);
-        drl_count_alloc();
-        hipError_t err = hipMalloc((void**)&l->segs, bytes);
+        l->bytes = bytes;
+        hipError_t err = table_pool(l->device).get(bytes, (void**)&l->segs);
         if (err == hipSuccess) err = hipMemcpy(l->segs, segs.data(), bytes, hipMemcpyHostToDevice);
         if (err != hipSuccess) {
-            if (l->segs) (void)hipFree(l->segs);
+            if (l->segs) table_pool(l->device).put(l->segs, bytes);
             delete l;
             return hip_fail(c, "drl_seq_layout_create", err);
         }
     } catch (const std::bad_alloc&) {
+        if (l->segs) table_pool(l->device).put(l->segs, l->bytes);
         delete l;
         return drl_ctx_fail(c, DRL_ERR_STATE, "drl_seq_layout_create: out of host memory");
     }
@@ -127,7 +198,9 @@ int drl_seq_layout_create(drl_ctx* c, const int64_t* qo, const int64_t* ko, int 
 void drl_seq_layout_destroy(drl_seq_layout* l) {
     if (!l) return;
     DeviceGuard guard(l->device);
-    if (l->segs) (void)hipFree(l->segs);
+    try {
+        if (l->segs) table_pool(l->device).put(l->segs, l->bytes);
+    } catch (const std::bad_alloc&) {}               // the table is lost, not more
     delete l;
 }
 
