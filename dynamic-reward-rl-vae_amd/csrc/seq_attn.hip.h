@@ -42,6 +42,13 @@ __device__ __forceinline__ void visible(const AttnArgs& a, int i, int nq, int nk
     lo = a.window > 0 ? (int)max((int64_t)0, min((int64_t)nk, end + 1 - a.window)) : 0;
 }
 
+// Run blockIdx.y of these keys.
+__device__ __forceinline__ void run_of(const AttnArgs& a, int& lo, int& hi) {
+    const int64_t from = lo + (int64_t)blockIdx.y * a.chunk;
+    lo = (int)min(from, (int64_t)hi);
+    hi = (int)min(from + a.chunk, (int64_t)hi);
+}
+
 __device__ __forceinline__ int keys_of(const AttnArgs& a, const SegInfo& s) {
     return a.k_len ? max(0, min(a.k_len[s.seg], s.nk)) : s.nk;
 }
@@ -57,6 +64,11 @@ template <int BK>
 __device__ __forceinline__ uint64_t have_keys(int asked, int base, int end) {
     return __ballot(asked && base + (int)(threadIdx.x & (BK - 1)) < end) & (~0ull >> (64 - BK));
 }
+
+// float16 weights are multiplied by 2^7: the largest is 2^15 then (an exponent of 8 above the reference at most), and what
+// is lost below float16's smallest, 2^-25 a key, is 2^-32 of the sum; a long flat tail behind one large score counts in full.
+template <typename T>
+__device__ constexpr float lift() { return __is_same(T, f16) ? 7.0f : 0.0f; }
 
 // m and l of a row to its log-sum; l = 0 where nothing was seen.
 __device__ __forceinline__ float log_sum(float m, float l) { return l == 0.0f ? -INFINITY : m + LN2 * __builtin_amdgcn_logf(l); }
@@ -209,8 +221,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
     visible(a, t.i0, t.s.nq, t.nk, LO, x0);
     visible(a, t.i0 + (t.rows - 1) / t.n_heads, t.s.nq, t.nk, x1, HI);
     if (a.splits > 1) {
-        LO += (int)min((int64_t)blockIdx.y * a.chunk, (int64_t)0x3fffffff);
-        HI = min(HI, LO + a.chunk);
+        run_of(a, LO, HI);
     }
     // what any row of the wave sees, and what all of them see: they rise with the lane
     const int wl = __builtin_amdgcn_readfirstlane(__shfl(lo, 0)), wh = __builtin_amdgcn_readfirstlane(__shfl(hi, 31));
@@ -257,7 +268,8 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
     }
 
     const float c1 = a.scale * LOG2E;
-    float ref = -INFINITY, mc = 0.0f;        // the reference, in units of the raw score; mc = ref * c1, 0 while there is none
+    constexpr float LIFT = lift<T>();
+    float ref = -INFINITY, mc = 0.0f;        // the reference, in units of the raw score; mc = ref * c1 - LIFT, 0 while there is none
     float l0 = 0.0f, l1 = 0.0f;
     f32x16 o[DT];
 #pragma unroll
@@ -344,7 +356,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
         const float m = pair_max(fmaxf(max16(z[0]), max16(z[1])));
         if (__any((m - ref) * c1 > 8.0f)) {
             const float now = fmaxf(m, ref);
-            const float mcn = now == -INFINITY ? 0.0f : now * c1;
+            const float mcn = now == -INFINITY ? 0.0f : now * c1 - LIFT;
             const float f = ref == -INFINITY ? 0.0f : exp2_fast(mc - mcn);
             ref = now;
             mc = mcn;
@@ -418,8 +430,7 @@ __global__ __launch_bounds__(256, DT > 2 ? 1 : 2) void attn_tile32_kernel(AttnAr
     visible(a, t.i0, t.s.nq, t.nk, LO, x0);
     visible(a, t.i0 + (t.rows - 1) / t.n_heads, t.s.nq, t.nk, x1, HI);
     if (a.splits > 1) {
-        LO += (int)min((int64_t)blockIdx.y * a.chunk, (int64_t)0x3fffffff);
-        HI = min(HI, LO + a.chunk);
+        run_of(a, LO, HI);
     }
     // what any row of the wave sees, and what all of them see: they rise with the lane
     const int wl = __builtin_amdgcn_readfirstlane(__shfl(lo, 0)), wh = __builtin_amdgcn_readfirstlane(__shfl(hi, 31));
@@ -573,8 +584,7 @@ __global__ __launch_bounds__(NW * 64) void attn_step_kernel(AttnArgs a) {
     visible(a, t.i0, t.s.nq, t.nk, LO, all_hi);
     visible(a, t.i0 + (t.rows - 1) / t.n_heads, t.s.nq, t.nk, all_lo, HI);
     if (a.splits > 1) {
-        LO += (int)min((int64_t)blockIdx.y * a.chunk, (int64_t)0x3fffffff);
-        HI = min(HI, LO + a.chunk);
+        run_of(a, LO, HI);
     }
     auto sw = [](int r) { return F32 ? swz32<NC>(r) : swz<NC>(r); };
 
@@ -600,6 +610,7 @@ __global__ __launch_bounds__(NW * 64) void attn_step_kernel(AttnArgs a) {
         load_v.pick(vp + base * vr, there, at + TILE);
     };
     const float c1 = a.scale * LOG2E;
+    constexpr float LIFT = lift<T>();
     float ref = -INFINITY, mc = 0.0f, l = 0.0f;
     f32x16 o[DT];
 #pragma unroll
@@ -647,7 +658,7 @@ __global__ __launch_bounds__(NW * 64) void attn_step_kernel(AttnArgs a) {
         const float m = pair_max(max16(z));
         if (__any((m - ref) * c1 > 8.0f)) {
             const float now = fmaxf(m, ref);
-            const float mcn = now == -INFINITY ? 0.0f : now * c1;
+            const float mcn = now == -INFINITY ? 0.0f : now * c1 - LIFT;
             const float f = ref == -INFINITY ? 0.0f : exp2_fast(mc - mcn);
             ref = now;
             mc = mcn;

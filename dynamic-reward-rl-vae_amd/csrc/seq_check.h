@@ -24,7 +24,8 @@ struct SeqRows {
     int n_seg = 0;
 };
 
-constexpr int64_t SEQ_MAX_ROWS = 0x7fffffffLL;
+// Rows are counted in 32 bits, and a tile or two past the last one.
+constexpr int64_t SEQ_MAX_ROWS = 0x7fff0000LL;
 
 inline int seq_check_layout(SeqError& e, const int64_t* qo, const int64_t* ko, int n_seg) {
     if (n_seg < 0 || n_seg > (1 << 24)) return e.set(DRL_ERR_ARG, "drl_seq_layout_create: n_seg %d (0 .. 2^24)", n_seg);
@@ -34,7 +35,7 @@ inline int seq_check_layout(SeqError& e, const int64_t* qo, const int64_t* ko, i
         if (o[0] < 0) return e.set(DRL_ERR_ARG, "drl_seq_layout_create: negative offset");
         for (int i = 0; i < n_seg; ++i)
             if (o[i + 1] < o[i]) return e.set(DRL_ERR_ARG, "drl_seq_layout_create: %s_offsets decrease at series %d", side ? "k" : "q", i);
-        if (o[n_seg] > SEQ_MAX_ROWS) return e.set(DRL_ERR_UNSUPPORTED, "drl_seq_layout_create: 2^31 rows or more");
+        if (o[n_seg] > SEQ_MAX_ROWS) return e.set(DRL_ERR_UNSUPPORTED, "drl_seq_layout_create: more than 2^31 - 2^16 rows");
     }
     return DRL_OK;
 }
@@ -53,6 +54,14 @@ inline int seq_check_workspace(SeqError& e, const char* who, const drl_seq_call*
     if (need > 0 && (!c->workspace || c->workspace_bytes < need))
         return e.set(DRL_ERR_ARG, "%s: workspace of %lld bytes needed, %lld given", who, (long long)need,
                      c->workspace ? (long long)c->workspace_bytes : 0LL);
+    return DRL_OK;
+}
+
+// A launch counts its threads along x in 32 bits.
+inline bool seq_grid_fits(int64_t workgroups, int threads) { return workgroups <= (((int64_t)1 << 32) - 1) / threads; }
+inline int seq_check_grid(SeqError& e, const char* who, int64_t workgroups, int threads) {
+    if (!seq_grid_fits(workgroups, threads))
+        return e.set(DRL_ERR_UNSUPPORTED, "%s: %lld workgroups of %d threads: too many series, rows or heads for one call", who, (long long)workgroups, threads);
     return DRL_OK;
 }
 

@@ -77,14 +77,16 @@ public:
         left -= size;
         return hipSuccess;
     }
-    void put(void* p, size_t bytes) {
+    void put(void* p, size_t bytes) noexcept {
         if (bytes > LARGEST) {
             (void)hipFree(p);
             return;
         }
         std::lock_guard<std::mutex> lk(mu);
-        retired[size_class(bytes)].push_back(p);
-        ++n_retired;
+        try {
+            retired[size_class(bytes)].push_back(p);
+            ++n_retired;
+        } catch (const std::bad_alloc&) {}               // the table is lost, not more
     }
 };
 TablePool& table_pool(int device) {
@@ -198,9 +200,7 @@ int drl_seq_layout_create(drl_ctx* c, const int64_t* qo, const int64_t* ko, int 
 void drl_seq_layout_destroy(drl_seq_layout* l) {
     if (!l) return;
     DeviceGuard guard(l->device);
-    try {
-        if (l->segs) table_pool(l->device).put(l->segs, l->bytes);
-    } catch (const std::bad_alloc&) {}               // the table is lost, not more
+    if (l->segs) table_pool(l->device).put(l->segs, l->bytes);      // the pool was made when the table came out of it
     delete l;
 }
 
@@ -294,7 +294,7 @@ int drl_attention_dev(drl_ctx* c, const drl_seq_layout* l, const drl_seq_call* c
     if (l->n_q == 0) return DRL_OK;
     const DrlCtxView v = drl_ctx_view(c);
     const AttnPlan p = attn_plan(v, l, call, a);
-    if (p.tiles > 0x7fffffff || l->n_q * a->n_heads > ((int64_t)1 << 32)) { e.set(DRL_ERR_UNSUPPORTED, "%s: too many rows and heads", who); return fail(c, e); }
+    if (seq_check_grid(e, who, p.tiles, 256) || (p.splits > 1 && seq_check_grid(e, who, (l->n_q * a->n_heads + 3) / 4, 256))) return fail(c, e);
     if (seq_check_workspace(e, who, call, p.workspace)) return fail(c, e);
     DeviceGuard guard(v.device);
     if (!guard.ok) return hip_fail(c, who, hipErrorInvalidDevice);
@@ -416,7 +416,7 @@ int drl_linear_attention_dev(drl_ctx* c, const drl_seq_layout* l, const drl_seq_
     if (check_layout(e, who, v, l) || seq_check_linear(e, who, l->rows.q_end, call, a, false)) return fail(c, e);
     if (l->rows.n_seg == 0) return DRL_OK;
     const LinearPlan p = linear_plan(v, l, call, a);
-    if (p.units * a->n_heads * p.blocks > 0x7fffffff) { e.set(DRL_ERR_UNSUPPORTED, "%s: too many series and heads", who); return fail(c, e); }
+    if (seq_check_grid(e, who, p.units * a->n_heads * p.blocks, p.waves * 64)) return fail(c, e);
     if (seq_check_workspace(e, who, call, p.workspace)) return fail(c, e);
     DeviceGuard guard(v.device);
     if (!guard.ok) return hip_fail(c, who, hipErrorInvalidDevice);
@@ -435,7 +435,7 @@ int drl_linear_attention_step_dev(drl_ctx* c, int64_t n, const drl_seq_call* cal
     SeqError e;
     if (seq_check_linear(e, who, n, call, a, true)) return fail(c, e);
     if (n == 0) return DRL_OK;
-    if (n * a->n_heads > 0x7fffffff) { e.set(DRL_ERR_UNSUPPORTED, "%s: too many series and heads", who); return fail(c, e); }
+    if (seq_check_grid(e, who, n * a->n_heads, 256)) return fail(c, e);
     const DrlCtxView v = drl_ctx_view(c);
     DeviceGuard guard(v.device);
     if (!guard.ok) return hip_fail(c, who, hipErrorInvalidDevice);
@@ -485,7 +485,7 @@ static NormPlan norm_plan(const DrlCtxView& v, const drl_seq_layout* l, int64_t 
     // series of 700 rows of 128 channels, float32, 17 us (two launches 23), 128 of 300 rows 9 (16), but 67 of 1,461 rows of
     // 512 channels, bf16, 100 MB, 94 us (78).
     const int64_t most = (int64_t)l->max_q * packs;
-    if (most <= 8 * 1024 && l->n_q * a->channels * size <= (int64_t)64 << 20 && (int64_t)(l->rows.n_seg + 7) * a->groups < 0x7fffffff) {
+    if (most <= 8 * 1024 && l->n_q * a->channels * size <= (int64_t)64 << 20 && seq_grid_fits((int64_t)(l->rows.n_seg + 7) * a->groups, 1024)) {
         p.threads = most <= 512 ? 256 : 1024;
         p.share = std::max<int>(1, (int)((most + p.threads - 1) / p.threads));
         return p;
@@ -563,6 +563,7 @@ int drl_group_norm_dev(drl_ctx* c, const drl_seq_layout* l, int64_t rows, const 
     if ((l ? l->n_q : rows) == 0) return DRL_OK;
     const DrlCtxView v = drl_ctx_view(c);
     const NormPlan p = norm_plan(v, l, rows, call, a);
+    if (seq_check_grid(e, who, p.units, 256)) return fail(c, e);
     if (seq_check_workspace(e, who, call, p.workspace)) return fail(c, e);
     DeviceGuard guard(v.device);
     if (!guard.ok) return hip_fail(c, who, hipErrorInvalidDevice);

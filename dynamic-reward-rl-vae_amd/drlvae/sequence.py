@@ -171,7 +171,7 @@ class SequenceOps:
             mask = self._flat("key_mask", key_mask, None, k_rows)
         if k_len is not None:
             klen = self._flat("k_len", k_len, _torch.int32, layout.n_seg)
-        window = int(window)
+        window = max(-1, min(int(window), 0x7fffffff))             # more than any series has rows
         args = _abi.pack_attn(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(), mask, klen,
                               qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os_[0], os_[1], heads, kv, dim, 1 if causal else 0, window,
                               dim ** -0.5 if scale is None else scale)

@@ -246,7 +246,7 @@ enum { DRL_ACT_SILU = 3 };      /* drl_group_norm_dev only: x * sigmoid(x); drl_
 /* Which rows belong to which series: the plan of the calls below, made once per batch layout.  Series i owns rows
  * q_offsets[i] .. q_offsets[i+1]-1 of q (x, out) and rows k_offsets[i] .. k_offsets[i+1]-1 of k and v; offsets are host
  * memory, n_seg+1 entries, non-decreasing and not negative; rows outside q_offsets[0] .. q_offsets[n_seg] are neither
- * read nor written.  k_offsets NULL: the same as q_offsets.  Fewer than 2^31 rows on each side.  Creation and
+ * read nor written.  k_offsets NULL: the same as q_offsets.  At most 2^31 - 2^16 rows on each side.  Creation and
  * destruction allocate and free device memory and may synchronise: not during a capture.  A layout is immutable, may
  * be used from any context on the same GPU, and has to outlive the calls, and the captured graphs, that use it. */
 typedef struct drl_seq_layout drl_seq_layout;

@@ -205,6 +205,18 @@ def test_attention_large_scores(sc, dt):
 
 
 @pytest.mark.parametrize("dt", ALL)
+@pytest.mark.parametrize("nq,nk", [(1, 30000), (150, 12000), (3, 700)])
+def test_attention_one_large_score_and_a_long_flat_tail(sc, dt, nq, nk):
+    """The tail's weights, exp(-17.625) = 2^-25.4 each, are below float16's smallest, but all of the result."""
+    q, k = torch.zeros(nq, 2, 32), torch.zeros(nk, 1, 32)
+    q[:, :, 0], k[0, 0, 0] = 17.625, 1
+    v = torch.ones(nk, 1, 32)
+    v[0] = 0
+    q, k, v = (x.to(DT[dt]).cuda() for x in (q, k, v))
+    check_attention(sc, dt, q, k, v, [0, nq], [0, nk], scale=1.0, causal=False)
+
+
+@pytest.mark.parametrize("dt", ALL)
 def test_attention_strides_and_layout_gaps(sc, dt):
     """Fused projections, heads before rows, rows of no series: left as they were."""
     g = torch.Generator().manual_seed(2)
@@ -572,3 +584,71 @@ def test_empty_calls(sc):
     q = torch.ones(3, 2, 32, device="cuda")
     out, lse = sc.attention(q, z, z, sc.seq_layout([0, 3], [0, 0]), return_lse=True)
     assert torch.all(out == 0) and torch.all(lse == -math.inf)
+
+
+def test_layouts_come_and_go_under_work(sc):
+    """Tables that are given back are not written over while work may read them."""
+    g = torch.Generator().manual_seed(5)
+    q, k, v = (normal(g, (3000, h, 64), "bf16") for h in (4, 2, 2))
+    r = torch.Generator().manual_seed(6)
+    kept, offsets = [], []
+    for i in range(300):
+        cuts = sorted(int(x) for x in torch.randint(0, 3001, (int(torch.randint(1, 90, (1,), generator=r)),), generator=r))
+        offsets.append([0] + cuts + [3000])
+        kept.append(sc.attention(q, k, v, sc.seq_layout(offsets[-1]), window=40))       # the layout dies with the call
+    for i in range(0, 300, 7):
+        layout = sc.seq_layout(offsets[i])
+        assert torch.equal(sc.attention(q, k, v, layout, window=40), kept[i]), i
+
+
+def test_linear_steps_of_many_series(sc):
+    n, H, D = (1 << 20) - 1, 16, 8                             # 16 workgroups short of the most that one call takes
+    g = torch.Generator(device="cuda").manual_seed(2)
+    q, k, v = (torch.randn(n, H, D, device="cuda", dtype=torch.bfloat16, generator=g) for _ in range(3))
+    ld = -torch.rand(H, device="cuda", generator=g)
+    state = torch.randn(n, H, D, D, device="cuda", generator=g)
+    some = torch.tensor([0, 1, 77777, 524288, n - 2, n - 1], device="cuda")
+    before = state[some].cpu()
+    out = sc.linear_attention_step(q, k, v, ld, state, scale=0.5)
+    want, final, oa, sa = orc.linear_attention(q[some], k[some], v[some], ld, list(range(len(some) + 1)), scale=0.5, state=before)
+    E = (D + 512) * U
+    within(out[some], want, (3 * half("bf16") + E) * oa + half("bf16") * want.abs())
+    within(state[some], final, E * sa)
+    with pytest.raises(Exception, match="too many"):
+        sc.linear_attention_step(*(x[:1].expand(1 << 20, H, D) for x in (q, k, v)), ld, torch.empty(1 << 20, H, D, D, device="cuda"),
+                                 out=torch.empty(1 << 20, H, D, device="cuda", dtype=torch.bfloat16))
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+def test_linear_offsets_past_32_bits(sc, dt):
+    n, stride = 300, 1 << 23
+    big = torch.empty(n * stride, device="cuda", dtype=DT[dt])
+    g = torch.Generator().manual_seed(3)
+    q, k, v = (big.as_strided((n, 1, 32), (stride, 32, 1), at) for at in (0, 64, 128))
+    for x in (q, k, v):
+        x.copy_(normal(g, (n, 1, 32), dt))
+    ld = torch.tensor([-0.1], device="cuda")
+    layout = sc.seq_layout([0, n])
+    out, final = sc.linear_attention(q, k, v, ld, layout)
+    want, last, oa, sa = orc.linear_attention(q, k, v, ld, [0, n], scale=32 ** -0.5)
+    E = (32 + 512 + n / 64) * U
+    within(out, want, (3 * half(dt) + E) * oa + half(dt) * want.abs())
+    within(final, last, E * sa)
+
+
+@pytest.mark.parametrize("series", [False, True])
+def test_norm_offsets_past_32_bits(sc, series):
+    rows, C, G = 4_300_000, 512, 8                             # 2.2e9 values
+    x = torch.empty(rows, C, device="cuda", dtype=torch.bfloat16).normal_()
+    tail = 1000
+    x[:tail] = x[-tail:]
+    if series:
+        y = sc.group_norm(x, G, layout=sc.seq_layout([0, tail, rows - tail, rows]), activation="silu")
+    else:
+        y = sc.group_norm(x, G, activation="silu")
+    off = [0, tail] if series else list(range(tail + 1))
+    want, size = orc.group_norm(x[-tail:], G, None, None, off, eps=1e-5, activation="silu")
+    n = C // G * (tail if series else 1)
+    tol = 1.1 * (64 + n / 256) * U * size + half("bf16") * want.abs()
+    within(y[-tail:], want, tol)
+    within(y[:tail], want, tol)

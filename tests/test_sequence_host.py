@@ -23,6 +23,7 @@ int t_attn(int64_t qe, int64_t ke, const drl_seq_call* c, const drl_attn_args* a
 int t_linear(int64_t rows, const drl_seq_call* c, const drl_linear_args* a, int step, char* m) {
     SeqError e; seq_check_linear(e, "t", rows, c, a, step); return done(e, m); }
 int t_norm(int64_t rows, const drl_seq_call* c, const drl_norm_args* a, char* m) { SeqError e; seq_check_norm(e, rows, c, a); return done(e, m); }
+int t_grid(int64_t workgroups, int threads, char* m) { SeqError e; seq_check_grid(e, "t", workgroups, threads); return done(e, m); }
 int t_ws(const drl_seq_call* c, int64_t need, char* m) { SeqError e; seq_check_workspace(e, "t", c, need); return done(e, m); }
 int t_sizes(int64_t* o) {
     o[0] = sizeof(drl_seq_call); o[1] = sizeof(drl_attn_args); o[2] = sizeof(drl_linear_args); o[3] = sizeof(drl_norm_args);
@@ -150,6 +151,19 @@ def test_workspace_refusals(chk):
     assert chk.t_ws(C.byref(_call(workspace=4096, workspace_bytes=15)), C.c_int64(16), m) == ARG
     assert chk.t_ws(C.byref(_call(workspace=4096, workspace_bytes=16)), C.c_int64(16), m) == OK
     assert chk.t_ws(C.byref(_call(workspace_bytes=16)), C.c_int64(16), m) == ARG
+
+
+@pytest.mark.parametrize("workgroups,threads,code", [(0, 256, OK), ((1 << 24) - 1, 256, OK), (1 << 24, 256, UNSUPPORTED), ((1 << 22) - 1, 1024, OK),
+                                                    (1 << 22, 1024, UNSUPPORTED), (1 << 40, 64, UNSUPPORTED)])
+def test_launches_that_do_not_fit_are_refused(chk, workgroups, threads, code):
+    m = C.create_string_buffer(256)
+    assert chk.t_grid(C.c_int64(workgroups), threads, m) == code
+
+
+def test_rows_leave_room_to_count_past_the_last(chk):
+    m = C.create_string_buffer(256)
+    for n, code in ((0x7fff0000, OK), (0x7fff0001, UNSUPPORTED)):
+        assert chk.t_layout((C.c_int64 * 2)(0, n), None, 1, m) == code
 
 
 def test_entry_points_without_a_context_return_an_error():
