@@ -413,7 +413,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
 // float32.  The same on 32x32x2 products, with tiles of 32 keys: the matrix pipe is 16 times slower, and what it does takes
 // most of the time.  Here a score register is at once an operand of values^T x weights, and nothing is rounded.
 template <int DT>
-__global__ __launch_bounds__(256, DT > 2 ? 1 : 2) void attn_tile32_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, 2) void attn_tile32_kernel(AttnArgs a) {
     constexpr int DP = DT <= 1 ? 32 : DT <= 2 ? 64 : 128, NC = DP / 4, KS = 4 * DT, BK = 32;
     constexpr int TILE = BK * DP * 4, LOADS = BK * NC / 256;
     extern __shared__ char smem[];
@@ -456,6 +456,15 @@ __global__ __launch_bounds__(256, DT > 2 ? 1 : 2) void attn_tile32_kernel(AttnAr
         load_k.pick(kp + base * kr, there, at);
         load_v.pick(vp + base * vr, there, at + TILE);
     };
+    // Operand reads: 32 s bytes on in a row of keys is an exclusive or, since tiles begin at whole rows; in a column of values
+    // the lane's part of the place takes four forms, and the rest is constant.
+    const uint32_t koff = lds + col * (DP * 4) + ((half ^ swz32<NC>(col)) * 16);
+    uint32_t voff[4];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+        const int j = NC == 8 ? (n >> 1) * 2 + (n & 1) * 8 : n;
+        voff[n] = lds + TILE + 4 * half * (DP * 4) + (((col >> 2) ^ swz32<NC>(j + 4 * half)) * 16) + (col & 3) * 4;
+    }
     const float c1 = a.scale * LOG2E;
     float ref = -INFINITY, mc = 0.0f, l = 0.0f;
     f32x16 o[DT];
@@ -489,12 +498,12 @@ __global__ __launch_bounds__(256, DT > 2 ? 1 : 2) void attn_tile32_kernel(AttnAr
             asked = ask_keys<BK>(a, t.s, base + 2 * BK, HI);
         }
         if (!there || strange || base >= wh || base + BK <= wl || wave * 32 >= t.rows) continue;      // nothing of it for this wave
-        const uint32_t kt_ = lds + buf * 2 * TILE, vt_ = kt_ + TILE;
+        const uint32_t at = buf * 2 * TILE;
         const bool edge = base < all_lo || base + BK > all_hi;
         if (edge) {
             bool odd = false;
 #pragma unroll
-            for (int n = 0; n < TILE / 1024; ++n) odd |= not_finite<float>(lds_read<u32x4>(vt_ + (n * 64 + lane) * 16));
+            for (int n = 0; n < TILE / 1024; ++n) odd |= not_finite<float>(lds_read<u32x4>(lds + at + TILE + (n * 64 + lane) * 16));
             if (__any(odd)) { strange = true; continue; }
         }
 
@@ -503,7 +512,7 @@ __global__ __launch_bounds__(256, DT > 2 ? 1 : 2) void attn_tile32_kernel(AttnAr
         for (int r = 0; r < 16; ++r) z[r] = 0.0f;
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
-            const f32x4 k = lds_read<f32x4>(kt_ + col * (DP * 4) + (((2 * s + half) ^ swz32<NC>(col)) * 16));
+            const f32x4 k = lds_read<f32x4>((koff + at) ^ (s * 32));
 #pragma unroll
             for (int e = 0; e < 4; ++e) z = mfma(k[e], qf[s][e], z);
         }
@@ -540,10 +549,10 @@ __global__ __launch_bounds__(256, DT > 2 ? 1 : 2) void attn_tile32_kernel(AttnAr
         }
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            const int row = acc_row(r, half);
+            const int row = acc_row(r, 0), eight = (r >> 2) & 1;
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt)
-                o[dt] = mfma(lds_read<float>(vt_ + row * (DP * 4) + (((dt * 8 + (col >> 2)) ^ swz32<NC>(row)) * 16) + (col & 3) * 4), z[r], o[dt]);
+                o[dt] = mfma(lds_read<float>(voff[NC == 8 ? (r & 2) + eight : r & 3] + at + (row * (DP * 4) + (NC == 8 ? 0 : (dt ^ eight) * 128))), z[r], o[dt]);
         }
         sched_reads(4);                                        // reads four products ahead
 #pragma unroll
