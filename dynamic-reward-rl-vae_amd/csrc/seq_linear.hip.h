@@ -465,6 +465,16 @@ __global__ __launch_bounds__(NW * 64) void linear_chunk32_kernel(LinearArgs a) {
             S[kt][r] = from && on && d < a.dk ? (from + d * a.dv)[lane_s] : 0.0f;
         }
 
+    // LDS places as in the attention kernel for float32: rows by exclusive or, columns in four forms (NC = 8: two, at rows
+    // 0 and 8), the rest constant; a wave's values lie at chunk 8 wave, which rows 8 .. 15 exchange with its neighbour.
+    const uint32_t row4 = lds + col * (DP * 4) + ((half ^ swz32<NC>(col)) * 16);
+    uint32_t kcol[4], vcol[4];
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {
+        const int j = NC == 8 ? (m >> 1) * 2 + (m & 1) * 8 : m;
+        kcol[m] = lds + 4 * half * (DP * 4) + (((col >> 2) ^ swz32<NC>(j + 4 * half)) * 16) + (col & 3) * 4;
+        vcol[m] = lds + QK + 4 * half * (VP * 4) + (((wave * 8 + (col >> 2)) ^ (m + 4 * half)) * 16) + (col & 3) * 4;
+    }
     float up[16];
 #pragma unroll
     for (int r = 0; r < 16; ++r) up[r] = uniform(power(ld2, acc_row(r, 0)));
@@ -481,13 +491,12 @@ __global__ __launch_bounds__(NW * 64) void linear_chunk32_kernel(LinearArgs a) {
         if (base + C < t.rows) stage(base + C, buf ^ 1);
         if (c0 >= a.dv) continue;
         if (n < C) fall = expm1f(decay_log(a, h) * (float)n);
-        const uint32_t kb = lds + buf * STAGE, vb = kb + QK, qb = vb + VB;
+        const uint32_t at = buf * STAGE;
         float v[16];
         bool odd = false;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            const int j = acc_row(r, half);
-            v[r] = lds_read<float>(vb + j * VP * 4 + (((wave * 8 + (col >> 2)) ^ swz32<VC>(j)) * 16) + (col & 3) * 4);
+            v[r] = lds_read<float>(((vcol[r & 3] + at) ^ ((r >> 2) & 1) * 128) + acc_row(r, 0) * (VP * 4));
             odd |= !(fabsf(v[r]) < INFINITY);
         }
         int bad = C;                                           // as for the 16-bit types
@@ -508,8 +517,7 @@ __global__ __launch_bounds__(NW * 64) void linear_chunk32_kernel(LinearArgs a) {
             for (int r = 0; r < 16; ++r) z[r] = o[r] = 0.0f;
 #pragma unroll
             for (int s = 0; s < 4 * KT; ++s) {
-                const uint32_t at = col * (DP * 4) + (((2 * s + half) ^ swz32<NC>(col)) * 16);
-                const f32x4 q = lds_read<f32x4>(qb + at), k = lds_read<f32x4>(kb + at);
+                const f32x4 q = lds_read<f32x4>((row4 + at + QK + VB) ^ (s * 32)), k = lds_read<f32x4>((row4 + at) ^ (s * 32));
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     z = mfma(k[e], q[e], z);
@@ -543,8 +551,9 @@ __global__ __launch_bounds__(NW * 64) void linear_chunk32_kernel(LinearArgs a) {
             for (int r = 0; r < 16; ++r) S[kt][r] = fmaf(S[kt][r], fall, S[kt][r]);
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                const int j = acc_row(r, half);
-                S[kt] = mfma(lds_read<float>(kb + j * DP * 4 + (((kt * 8 + (col >> 2)) ^ swz32<NC>(j)) * 16) + (col & 3) * 4), v[r], S[kt]);
+                const int eight = (r >> 2) & 1;
+                const uint32_t k = kcol[NC == 8 ? (r & 2) + eight : r & 3] + at + (acc_row(r, 0) * (DP * 4) + (NC == 8 ? 0 : (kt ^ eight) * 128));
+                S[kt] = mfma(lds_read<float>(k), v[r], S[kt]);
             }
         }
         if (odd && bad < C)
