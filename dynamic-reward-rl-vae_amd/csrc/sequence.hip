@@ -334,11 +334,12 @@ static LinearPlan linear_plan(const DrlCtxView& v, const drl_seq_layout* l, cons
     // (384 of 2,048 rows: 222 us whole, 226 in pieces of 512; 64 of 32,768: 2.9 ms whole, 0.76 in pieces of 4,096).
     // A piece is long enough that two workgroups per CU do it all at once, and that going through its chunks twice takes
     // about as long as going through the pieces' states (1.6 us a chunk, 0.3 a state: pieces of sqrt(3 rows), 8,192 rows
-    // of 16 heads in 81 us at 256).
+    // of 16 heads in 81 us at 256), in whole chunks, rounded down by up to a quarter of one (375 rows of 4 heads,
+    // float32: 18.9 us in pieces of 32, 25.1 of 64; 1,000 rows: 26.4 and 26.3; 4,000 rows of 8 heads: 51 at 96, 43 at 128).
     const int64_t groups = (int64_t)a->n_heads * p.blocks;
     if (groups * l->rows.n_seg < v.n_cu) {
         const int64_t rows = std::max<int64_t>(l->n_q * groups / (2 * v.n_cu), (int64_t)std::sqrt(3.0 * l->max_q));
-        const int64_t piece = std::max<int64_t>(64, (rows + 31) / 32 * 32);
+        const int64_t piece = std::max<int64_t>(32, (rows + 23) / 32 * 32);
         if (piece < l->max_q) {
             // pieces of one length
             const int64_t n = (l->max_q + piece - 1) / piece;
