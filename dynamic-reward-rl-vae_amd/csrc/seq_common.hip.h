@@ -34,16 +34,47 @@ struct SegInfo {
 // A value that is the same in all lanes, into a scalar register.
 __device__ __forceinline__ float uniform(float x) { return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x))); }
 
+// Lanes are joined without LDS: what lane l ^ M holds, where the lanes of each M hold the same (so that for 4 and 8 the
+// mirrored half row and row will do); 4 to 8 cycles each, where a shuffle through LDS takes a hundred.
+template <int M>
+__device__ __forceinline__ float other(float x) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, x);
+    if constexpr (M < 16) {
+        constexpr int CTRL = M == 1 ? 0xb1 : M == 2 ? 0x4e : M == 4 ? 0x141 : 0x140;      // quad_perm 1,0,3,2 and 2,3,0,1; mirrors
+        return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, (int)u, CTRL, 0xf, 0xf, true));
+    } else {
+        const auto r = M == 16 ? __builtin_amdgcn_permlane16_swap(u, u, false, false) : __builtin_amdgcn_permlane32_swap(u, u, false, false);
+        return __builtin_bit_cast(float, (uint32_t)((threadIdx.x & M) ? r[0] : r[1]));
+    }
+}
+// The larger / the sum of a lane's value and that of the lane 32 away.
+__device__ __forceinline__ float pair_max(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
+    return fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
+}
+__device__ __forceinline__ float pair_sum(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
+    return __builtin_bit_cast(float, (uint32_t)r[0]) + __builtin_bit_cast(float, (uint32_t)r[1]);
+}
 __device__ __forceinline__ float wave_max(float x) {
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) x = fmaxf(x, __shfl_xor(x, m));
+    x = fmaxf(x, other<1>(x));
+    x = fmaxf(x, other<2>(x));
+    x = fmaxf(x, other<4>(x));
+    x = fmaxf(x, other<8>(x));
+    x = fmaxf(x, other<16>(x));
+    return pair_max(x);
+}
+// Over groups of `lanes` lanes, a power of two and the same in the whole wave.
+__device__ __forceinline__ float lanes_sum(float x, int lanes) {
+    if (lanes > 1) x += other<1>(x);
+    if (lanes > 2) x += other<2>(x);
+    if (lanes > 4) x += other<4>(x);
+    if (lanes > 8) x += other<8>(x);
+    if (lanes > 16) x += other<16>(x);
+    if (lanes > 32) x = pair_sum(x);
     return x;
 }
-__device__ __forceinline__ float wave_sum(float x) {
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) x += __shfl_xor(x, m);
-    return x;
-}
+__device__ __forceinline__ float wave_sum(float x) { return lanes_sum(x, 64); }
 
 // The entry that holds unit `t` when the entries own floor(cum / per) + index .. units (a tiling of each series in
 // blocks of `per` rows, at most one empty unit per series): the last s with floor(cum_s / per) + s <= t.  Four entries per
@@ -219,16 +250,6 @@ __device__ __forceinline__ float if_bit(uint32_t bits, int n, float x, float y) 
 
 // LDS reads stay on their side of this; everything else may be moved across.
 __device__ __forceinline__ void keep_reads() { __builtin_amdgcn_sched_barrier(0x67f); }
-
-// The larger / the sum of a lane's value and that of the lane 32 away.
-__device__ __forceinline__ float pair_max(float x) {
-    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
-    return fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
-}
-__device__ __forceinline__ float pair_sum(float x) {
-    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
-    return __builtin_bit_cast(float, (uint32_t)r[0]) + __builtin_bit_cast(float, (uint32_t)r[1]);
-}
 
 // 32x32x16 product: lane l holds row (column) l & 31 of A (B), elements 8 (l >> 5) .. + 7 of the inner axis; of the result
 // column l & 31, rows (r & 3) + 8 (r >> 2) + 4 (l >> 5) in registers r = 0 .. 15.

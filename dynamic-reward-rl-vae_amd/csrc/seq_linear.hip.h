@@ -207,22 +207,21 @@ __global__ __launch_bounds__(NW * 64, STATE ? 3 : 2) void linear_chunk_kernel(Li
     // Powers of lam, the same for all waves and chunks, in LDS, four registers' worth side by side: between a row (lane) and a
     // key (register), times the scale, 0 for the keys behind it; of a value's row to the chunk's end; of a row from its
     // start, times the scale.
-    const uint32_t inner_at = table + 256 + lane * 16, left_at = table + half * 64, grown_at = table + 128 + half * 64;
+    const uint32_t inner_at = table + 640 + lane * 16, left_at = table + half * 64, back_at = table + 128 + wave * 128;
     if (wave == 0)
 #pragma unroll
         for (int r = 0; r < 16; r += 4) {
-            f32x4 left, grown, inner;
+            f32x4 left, inner;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int row = acc_row(r + e, half);
                 left[e] = power(ld2, C - 1 - row);
-                grown[e] = a.scale * power(ld2, row + 1);
                 inner[e] = col >= row ? a.scale * power(ld2, col - row) : 0.0f;
             }
             lds_write<f32x4>(left_at + r * 4, left);
-            if (!STATE) lds_write<f32x4>(grown_at + r * 4, grown);
             if (!STATE) lds_write<f32x4>(inner_at + r * 256, inner);
         }
+    const float grown = a.scale * power(ld2, col + 1);         // of this lane's row from the chunk's start
     float fall = expm1f(decay_log(a, h) * (float)C);           // lam^n - 1: lam^n itself, rounded, would drift over many chunks
 
     T* op = (T*)a.out + row0 * a.o_row + (int64_t)h * a.o_head + c0;
@@ -277,6 +276,7 @@ __global__ __launch_bounds__(NW * 64, STATE ? 3 : 2) void linear_chunk_kernel(Li
 #pragma unroll
                     for (int r = 0; r < 16; ++r) m = fmaxf(m, fabsf(S[kt][r]));
                 s_scale = into_range(pair_max(m), s_back);
+                if (half == 0) lds_write<float>(back_at + col * 4, s_back);    // the product has the state's columns along its registers
             }
 #pragma unroll
             for (int s = 0; s < 2 * KT; ++s) {
@@ -286,7 +286,7 @@ __global__ __launch_bounds__(NW * 64, STATE ? 3 : 2) void linear_chunk_kernel(Li
                 x8 b;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) b[e] = (T)(F16 ? S[s >> 1][8 * (s & 1) + e] * s_scale : S[s >> 1][8 * (s & 1) + e]);
-                o = mfma(q, b, o);
+                o = mfma(b, q, o);
             }
             float p[16];
 #pragma unroll
@@ -297,11 +297,11 @@ __global__ __launch_bounds__(NW * 64, STATE ? 3 : 2) void linear_chunk_kernel(Li
             }
             float p_scale = 1.0f, p_back = 1.0f;
             f32x16 w = o;
-#pragma unroll
             for (int r = 0; r < 16; r += 4) {
-                const f32x4 grown = lds_read<f32x4>(grown_at + r * 4);
+                f32x4 back;
+                if (F16) back = lds_read<f32x4>(back_at + r * 8 + half * 16);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[r + e] *= F16 ? grown[e] * s_back : grown[e];
+                for (int e = 0; e < 4; ++e) o[r + e] *= F16 ? grown * back[e] : grown;
             }
             if constexpr (F16) {
                 float m = 0.0f;
@@ -310,33 +310,41 @@ __global__ __launch_bounds__(NW * 64, STATE ? 3 : 2) void linear_chunk_kernel(Li
                     m = fmaxf(m, fabsf(p[r]));
                     w[r] = 0.0f;
                 }
-                p_scale = into_range(wave_max(m), p_back);
+                p_scale = into_range(pair_max(m), p_back);
             } else w = o;
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
                 x8 b;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) b[e] = (T)(F16 ? p[8 * s + e] * p_scale : p[8 * s + e]);
-                w = mfma(b, v[s], w);
+                w = mfma(v[s], b, w);
             }
             if constexpr (F16)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) w[r] = fmaf(w[r], p_back, o[r]);
             if (odd)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) w[r] = acc_row(r, half) >= bad ? NAN : w[r];
-            // through the values' own place in LDS, which no other wave reads, and out 16 bytes per lane
-            const uint32_t vb = kb + QK;
+                for (int r = 0; r < 16; ++r) w[r] = col >= __shfl(bad, acc_row(r, half)) ? NAN : w[r];
+            // Four columns of the lane's row are in four registers, the next four those of the lane 32 away: halves are
+            // exchanged, and each lane writes eight.
+            u32x4 out[2];
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int row = acc_row(r, half);
-                lds_write<T>(vb + row * (VP * 2) + (((wave * 4 + (col >> 3)) ^ swz<VC>(row)) * 16) + (col & 7) * 2, (T)w[r]);
+            for (int g = 0; g < 2; ++g) {
+                u32x2 x = __builtin_bit_cast(u32x2, x4{(T)w[8 * g], (T)w[8 * g + 1], (T)w[8 * g + 2], (T)w[8 * g + 3]});
+                u32x2 y = __builtin_bit_cast(u32x2, x4{(T)w[8 * g + 4], (T)w[8 * g + 5], (T)w[8 * g + 6], (T)w[8 * g + 7]});
+                const auto e0 = __builtin_amdgcn_permlane32_swap(x[0], y[0], false, false), e1 = __builtin_amdgcn_permlane32_swap(x[1], y[1], false, false);
+                out[g] = u32x4{(uint32_t)e0[0], (uint32_t)e1[0], (uint32_t)e0[1], (uint32_t)e1[1]};
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const auto r = __builtin_amdgcn_permlane16_swap(out[0][e], out[1][e], false, false);
+                out[0][e] = r[0];
+                out[1][e] = r[1];
             }
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
-                const int j = m * 16 + (lane >> 2);
-                const u32x4 y = lds_read<u32x4>(vb + j * (VP * 2) + (((wave * 4 + (lane & 3)) ^ swz<VC>(j)) * 16));
-                if (j < n && c0 + (lane & 3) * 8 < a.dv) *(u32x4*)(op + (int64_t)(base + j) * a.o_row + (lane & 3) * 8) = y;
+                const int j = m * 16 + (lane & 15), c = (lane & 16) + 8 * half;
+                if (j < n && c0 + c < a.dv) *(u32x4*)(op + (int64_t)(base + j) * a.o_row + c) = out[m];
             }
         }
 

@@ -41,12 +41,19 @@ __device__ __forceinline__ Moments join(const Moments& a, const Moments& b) {
     const float d = b.mean - a.mean, w = b.n / n;
     return {n, fmaf(d, w, a.mean), a.dev + b.dev + d * d * a.n * w};
 }
-__device__ __forceinline__ Moments join_lanes(Moments m, int width) {
-    for (int k = 1; k < width; k <<= 1) {
-        const Moments o = {__shfl_xor(m.n, k), __shfl_xor(m.mean, k), __shfl_xor(m.dev, k)};
-        // the lower lane first on both sides: the same result in both
-        m = (threadIdx.x & k) ? join(o, m) : join(m, o);
-    }
+template <int K>
+__device__ __forceinline__ Moments join_other(const Moments& m) {
+    const Moments o = {other<K>(m.n), other<K>(m.mean), other<K>(m.dev)};
+    // the lower lane first on both sides: the same result in both
+    return (threadIdx.x & K) ? join(o, m) : join(m, o);
+}
+__device__ __forceinline__ Moments join_lanes(Moments m, int lanes) {
+    if (lanes > 1) m = join_other<1>(m);
+    if (lanes > 2) m = join_other<2>(m);
+    if (lanes > 4) m = join_other<4>(m);
+    if (lanes > 8) m = join_other<8>(m);
+    if (lanes > 16) m = join_other<16>(m);
+    if (lanes > 32) m = join_other<32>(m);
     return m;
 }
 
@@ -64,10 +71,7 @@ __global__ __launch_bounds__(256) void norm_rows_kernel(NormArgs a) {
     const bool on = g < a.groups;
     const int c0 = (on ? g : 0) * cg;
     const float inv = 1.0f / (float)cg;
-    auto sum = [&](float v) {
-        for (int k = 1; k < a.lanes; k <<= 1) v += __shfl_xor(v, k);
-        return v;
-    };
+    auto sum = [&](float v) { return lanes_sum(v, a.lanes); };
     if constexpr (NV > 0) {
         float ga[NV][V], be[NV][V];
 #pragma unroll

@@ -375,7 +375,7 @@ static seq::LinearArgs linear_args(const drl_linear_args* a, const seq::SegInfo*
 template <typename T, int KT, int NW, bool STATE>
 static void linear_chunks(const LinearPlan& p, const seq::LinearArgs& k, hipStream_t st) {
     constexpr int DP = KT <= 1 ? 32 : KT <= 2 ? 64 : 128;
-    constexpr int stage = 32 * sizeof(T) * ((STATE ? 1 : 2) * DP + 32 * NW), stages = sizeof(T) == 2 ? 3 : 2, table = sizeof(T) == 4 ? 0 : STATE ? 256 : 256 + 4096;
+    constexpr int stage = 32 * sizeof(T) * ((STATE ? 1 : 2) * DP + 32 * NW), stages = sizeof(T) == 2 ? 3 : 2, table = sizeof(T) == 4 ? 0 : STATE ? 256 : 640 + 4096;
     const dim3 grid((unsigned)(p.units * k.heads * p.blocks));
     auto go = [&](auto kernel) {
         // more LDS than a kernel gets unasked
