@@ -55,13 +55,15 @@ __device__ __forceinline__ int keys_of(const AttnArgs& a, const SegInfo& s) {
 
 // Which of a tile's BK keys from `base` on are there at all: in front of `end`, and not masked.  The mask's bytes are asked
 // for a tile ahead.
-template <int BK>
+template <int BK, bool MASK = true>
 __device__ __forceinline__ int ask_keys(const AttnArgs& a, const SegInfo& s, int base, int end) {
+    if (!MASK) return 1;
     const int j = base + (threadIdx.x & (BK - 1));
     return a.key_mask && j < end ? a.key_mask[s.k0 + j] : 1;
 }
-template <int BK>
+template <int BK, bool MASK = true>
 __device__ __forceinline__ uint64_t have_keys(int asked, int base, int end) {
+    if (!MASK) return ~0ull >> (64 - min(BK, end - base));
     return __ballot(asked && base + (int)(threadIdx.x & (BK - 1)) < end) & (~0ull >> (64 - BK));
 }
 
@@ -196,7 +198,7 @@ __device__ __forceinline__ void attn_store(const AttnArgs& a, const AttnTile& t,
 // away has the others), the maximum is one exchange away, and the weights, rounded to the inputs' type (relative error
 // u = eps/2 each, as the result's own rounding), are as they lie in registers the second operand of values^T x weights: the
 // order of the keys inside the product is free, and the values are read with ds_read_b64_tr_b16 in the weights' order.
-template <typename T, int DT>
+template <typename T, int DT, bool MASK>
 __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
     typedef typename Vec<T>::x8 x8;
     typedef typename Vec<T>::x4 x4;
@@ -269,6 +271,11 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
 
     const float c1 = a.scale * LOG2E;
     constexpr float LIFT = lift<T>();
+    // Where all rows see all keys but the masked ones, whose scores are copies of a visible one's, a product with a column
+    // that holds the type's lowest value for them takes them away: 16 x -65504 x 65504 for float16, -inf for bfloat16 (which
+    // has the range).  A quarter of the time that choosing score by score takes (ragged batch: 140 -> 135 us, with the choice made where there is a mask at all).
+    constexpr bool F16 = __is_same(T, f16);
+    const bool by_product = !F16 || c1 * 6.8e10f > 1000.0f;
     float ref = -INFINITY, mc = 0.0f;        // the reference, in units of the raw score; mc = ref * c1 - LIFT, 0 while there is none
     float l0 = 0.0f, l1 = 0.0f;
     f32x16 o[DT];
@@ -284,9 +291,9 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
     uint64_t coming = 0;
     int asked = 1;
     if (LO < HI) {
-        coming = have_keys<BK>(ask_keys<BK>(a, t.s, LO, HI), LO, HI);
+        coming = have_keys<BK, MASK>(ask_keys<BK, MASK>(a, t.s, LO, HI), LO, HI);
         stage(LO, 0, coming);
-        asked = ask_keys<BK>(a, t.s, LO + BK, HI);
+        asked = ask_keys<BK, MASK>(a, t.s, LO + BK, HI);
     }
     // q has arrived: no wait for it inside the loop, where it would be one for the keys to come
 #pragma unroll
@@ -297,9 +304,9 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
         __syncthreads();
         const uint64_t there = coming;
         if (base + BK < HI) {
-            coming = have_keys<BK>(asked, base + BK, HI);
+            coming = have_keys<BK, MASK>(asked, base + BK, HI);
             stage(base + BK, buf ^ 1, coming);
-            asked = ask_keys<BK>(a, t.s, base + 2 * BK, HI);
+            asked = ask_keys<BK, MASK>(a, t.s, base + 2 * BK, HI);
         }
         if (!there || strange || base >= wh || base + BK <= wl || wave * 32 >= t.rows) return;      // nothing of it for this wave
         constexpr uint32_t kt_ = buf * 2 * TILE, vt_ = kt_ + TILE;
@@ -336,7 +343,20 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
             sched_products(KS);
             __builtin_amdgcn_s_setprio(0);
         }
-        if (edge || there != ~0ull >> (64 - BK)) {
+        if (MASK && !edge && there != ~0ull >> (64 - BK) && by_product) {
+            const T off = (T)(F16 ? -65504.0f : -3.3895314e38f);
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt) {
+                x8 drop, one;
+                const T d = ((uint32_t)(there >> (32 * kt)) >> col) & 1 ? (T)0.0f : off;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    drop[e] = d;
+                    one[e] = (T)(F16 ? 65504.0f : 1.0f);
+                }
+                z[kt] = mfma(drop, one, z[kt]);
+            }
+        } else if (edge || (MASK && there != ~0ull >> (64 - BK))) {
             const int from = max(lo - base, 0), to = min(hi - base, 64);
             uint64_t see = to <= from ? 0 : there & (~0ull << from) & (~0ull >> (64 - to));
             see >>= 4 * half;

@@ -276,7 +276,8 @@ static void attn_tiles(const AttnPlan& p, const seq::AttnArgs& k, hipStream_t st
         constexpr int NW = sizeof(T) == 4 && DT > 2 ? 2 : 4;
         if (p.few) go(seq::attn_step_kernel<T, DT, NW>, NW, std::max(NW * 4 * tile, (size_t)NW * (DT * 4096 + 256)));
         else if constexpr (sizeof(T) == 4) go(seq::attn_tile32_kernel<DT>, 4, 4 * tile);
-        else go(seq::attn_tile_kernel<T, DT>, 4, 8 * tile);
+        else if (k.key_mask) go(seq::attn_tile_kernel<T, DT, true>, 4, 8 * tile);
+        else go(seq::attn_tile_kernel<T, DT, false>, 4, 8 * tile);
     });
     if (p.splits > 1) {
         const dim3 jg((unsigned)((k.part_rows * k.heads + 3) / 4));
