@@ -27,8 +27,9 @@ struct AttnArgs {
     int heads, rep, dim;
     int causal, window;
     float scale;
-    // heads of one kv head are cut into `blocks` runs of `rep_b`; a tile holds `per` rows of q of one run
-    int kv_blocks, blocks, rep_b, per;
+    // heads of one kv head are cut into `blocks` runs of `rep_b`; a tile holds `per` rows of q of one run; every other
+    // `turn` units go backwards
+    int kv_blocks, blocks, rep_b, per, turn;
     // the keys are cut into runs of `chunk` (splits > 1): partial results of run y, normalised, and their log-sums
     int splits, chunk;
     float *part_o, *part_lse;      // [splits][rows][heads][dim], [splits][rows][heads], rows from the first series' first
@@ -143,7 +144,12 @@ struct AttnTile {
 };
 __device__ __forceinline__ AttnTile attn_tile(const AttnArgs& a, uint32_t id) {
     AttnTile t;
-    const uint32_t b = id % (uint32_t)a.kv_blocks, u = id / (uint32_t)a.kv_blocks;
+    const uint32_t b = id % (uint32_t)a.kv_blocks;
+    uint32_t u = id / (uint32_t)a.kv_blocks;
+    if (const uint32_t turn = u / (uint32_t)a.turn; turn & 1) {
+        const uint32_t first = turn * a.turn, n = min((uint32_t)a.turn, gridDim.x / (uint32_t)a.kv_blocks - first);
+        u = first + n - 1 - (u - first);
+    }
     const int slot = find_seg(a.segs, a.n_seg, u, a.per);
     t.s = a.segs[slot];
     t.kv = b / (uint32_t)a.blocks;
