@@ -555,14 +555,17 @@ __global__ __launch_bounds__(NW * 64) void linear_chunk32_kernel(LinearArgs a) {
         }
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt) {
+            f32x16 sum;                                        // the chunk's own: the state is rounded once per chunk
 #pragma unroll
-            for (int r = 0; r < 16; ++r) S[kt][r] = fmaf(S[kt][r], fall, S[kt][r]);
+            for (int r = 0; r < 16; ++r) sum[r] = 0.0f;
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 const int eight = (r >> 2) & 1;
                 const uint32_t k = kcol[NC == 8 ? (r & 2) + eight : r & 3] + at + (acc_row(r, 0) * (DP * 4) + (NC == 8 ? 0 : (kt ^ eight) * 128));
-                S[kt] = mfma(lds_read<float>(k), v[r], S[kt]);
+                sum = mfma(lds_read<float>(k), v[r], sum);
             }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) S[kt][r] = fmaf(S[kt][r], fall, S[kt][r]) + sum[r];
         }
         if (odd && bad < C)
 #pragma unroll

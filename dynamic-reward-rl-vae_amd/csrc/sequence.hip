@@ -216,7 +216,7 @@ static int attn_prepare(drl_ctx* c, const drl_seq_layout* l, const drl_seq_call*
 struct AttnPlan {
     bool few;
     int blocks, rep_b, per, splits, chunk, turn;
-    int64_t tiles, workspace;
+    int64_t tiles, workspace, longest;        // longest: the most keys that one workgroup goes over
 };
 static AttnPlan attn_plan(const DrlCtxView& v, const drl_seq_layout* l, const drl_seq_call* call, const drl_attn_args* a) {
     AttnPlan p = {};
@@ -239,6 +239,7 @@ static AttnPlan attn_plan(const DrlCtxView& v, const drl_seq_layout* l, const dr
         p.splits = (int)((most + chunk - 1) / chunk);
         p.chunk = (int)chunk;
     }
+    p.longest = p.splits > 1 ? p.chunk : most;
     if (p.splits > 1) p.workspace = (int64_t)p.splits * l->n_q * a->n_heads * (a->dim + 1) * 4;
     // Where all workgroups are resident at once, two per CU, each CU's second is taken from the other end of the order, so
     // that a long tile has a short one beside it (8,192 rows of 8 heads, dim 64: 124 -> 120 us, float32 834 -> 667; two
@@ -281,7 +282,10 @@ static void attn_tiles(const AttnPlan& p, const seq::AttnArgs& k, hipStream_t st
         constexpr int DT = decltype(d)::value;
         constexpr int NW = sizeof(T) == 4 && DT > 2 ? 2 : 4;
         if (p.few) go(seq::attn_step_kernel<T, DT, NW>, NW, std::max(NW * 4 * tile, (size_t)NW * (DT * 4096 + 256)));
-        else if constexpr (sizeof(T) == 4) go(seq::attn_tile32_kernel<DT>, 4, 4 * tile);
+        else if constexpr (sizeof(T) == 4) {
+            if (DT <= 2 && p.longest <= 1024) go(seq::attn_tile32_kernel<DT, DT >= 3>, 4, 4 * tile);
+            else go(seq::attn_tile32_kernel<DT, true>, 4, 4 * tile);
+        }
         else if (k.key_mask) go(seq::attn_tile_kernel<T, DT, true>, 4, 8 * tile);
         else go(seq::attn_tile_kernel<T, DT, false>, 4, 8 * tile);
     });
