@@ -55,7 +55,8 @@ __device__ __forceinline__ LinearUnit linear_unit(const LinearArgs& a, uint32_t 
 
 // One row of each of n series.  Bound by reading and writing the states once, 8 bytes per element: a wave has 4 columns per
 // lane of as many state rows as fit side by side (64 lanes over dv / 4 quads), a workgroup all dk rows of a column block
-// of one series and head, and joins what the rows add to the output through LDS.
+// of one series and head, and joins what the rows add to the output through LDS.  64 series of 32 heads, 128 x 128: 54 us,
+// 4.9 TB/s.
 template <typename T>
 __global__ __launch_bounds__(256) void linear_step_kernel(LinearArgs a) {
     __shared__ float part[4 * 256];
@@ -123,14 +124,19 @@ __device__ __forceinline__ float into_range(float x, float& back) {
 
 // 16-bit types.  A wave keeps the state's columns of 32 value dimensions in registers, as the accumulator of the state's
 // product: rows of the key width along the registers, value dimension along the lanes.  Rounded to 16 bits it is, register
-// by register, the second operand of the product with q (the inner index may be taken in any order; q is read from LDS
-// in that order, and with it k for the scores).  Scores are computed transposed, which makes them the first operand of the
-// product with v.  k and v go through LDS once and are read as they are for the scores and transposed (ds_read_b64_tr_b16)
-// for the state.
+// by register, an operand of the product with q (the inner index may be taken in any order; q is read from LDS
+// in that order, and with it k for the scores).  Scores are computed transposed, keys along the registers, and so is the
+// output, value dimension along them: a row is a lane throughout, and its factors are one register.  k and v go through LDS
+// once and are read as they are for the scores and transposed (ds_read_b64_tr_b16) for the state.
 // Rounding: scores and the state's copy are rounded to the inputs' type (relative error eps/2, like the result's own);
 // the float32 state itself takes lam^(n-1-j) v_j as the sum of N parts of that type (24 bits of bfloat16 in three, 22 of
 // float16 in two), and loses nothing from call to call.  float16 has no range to spare: scores, state columns and
 // weighted values are scaled by powers of two before they are rounded.
+// Two series of 32,768 rows, 32 heads of 128 x 128, bfloat16, in 16 pieces: 710-745 us by card, 300 for the pieces' states (a
+// second reading of k and v), 12 to join them, the rest the outputs; 2.15 GB once are 457 us.  VALU 54 % busy, matrix pipe
+// 44 %.  24 ragged series, 16 heads of 64 x 128, float16: 155 us, as long as the longest series' 64 chunks take, two
+// workgroups to a CU; VALU 54 % (scales and splits), matrix pipe 16 %; 92 us at a copy's rate.  Eight waves of 16 columns
+// instead of four of 32: 852 us against 760 at the time.
 template <typename T, int KT, int NW, bool STATE>
 __global__ __launch_bounds__(NW * 64, STATE ? 3 : 2) void linear_chunk_kernel(LinearArgs a) {
     typedef typename Vec<T>::x8 x8;
@@ -425,7 +431,8 @@ __global__ __launch_bounds__(NW * 64, STATE ? 3 : 2) void linear_chunk_kernel(Li
 }
 
 // float32: the same on 32x32x2 products; a register of the state or of the scores is an operand as it is, and nothing is
-// rounded or split.
+// rounded or split.  Bound by the products, 3 us a chunk and wave at 64 x 64: 24 series of up to 2,048 rows of 16 heads, 64 x
+// 128: 575 us; one of 375 rows of 4 heads in 12 pieces: 20 us, of which its three launches take 6, 4 and 10.
 template <int KT, int NW, bool STATE>
 __global__ __launch_bounds__(NW * 64) void linear_chunk32_kernel(LinearArgs a) {
     constexpr int C = 32, THREADS = NW * 64;
@@ -586,7 +593,8 @@ __global__ __launch_bounds__(NW * 64) void linear_chunk32_kernel(LinearArgs a) {
             }
 }
 
-// The states before each piece: a unit holds what its predecessor added, from a state of 0.
+// The states before each piece: a unit holds what its predecessor added, from a state of 0.  Bound by reading and writing them
+// (2 x 16 pieces of 32 heads of 128 x 128: 12 us).
 static __global__ __launch_bounds__(256) void linear_scan_kernel(LinearArgs a) {
     const int slot = blockIdx.x, h = blockIdx.y;
     const int64_t size = (int64_t)a.dk * a.dv, e = ((int64_t)blockIdx.z * 256 + threadIdx.x) * 4;

