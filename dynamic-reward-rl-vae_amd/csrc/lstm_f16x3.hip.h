@@ -92,8 +92,11 @@ __device__ __forceinline__ void h128f_pointwise(const f32x16 (&acc)[4], float (&
         f16x4 hi, lo;
 #pragma unroll
         for (int qd = 0; qd < 4; ++qd) {
-            const float hv = lstm_cell(acc[tl][4 * qd], acc[tl][4 * qd + 1], acc[tl][4 * qd + 2],
-                                       acc[tl][4 * qd + 3], 0.0f, c[tl][qd]);
+            float hv = lstm_cell(acc[tl][4 * qd], acc[tl][4 * qd + 1], acc[tl][4 * qd + 2],
+                                 acc[tl][4 * qd + 3], 0.0f, c[tl][qd]);
+            // One rounded product for both parts: hi and the hi that lo is the rest of are otherwise made by different
+            // instructions (a conversion, and a fused multiply-add that rounds once), which differ at some ties.
+            asm("" : "+v"(hv));
             hi[qd] = (_Float16)hv;
             lo[qd] = (_Float16)(hv - (float)hi[qd]);
         }
