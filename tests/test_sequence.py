@@ -14,6 +14,7 @@ Tolerances.  u = eps/2 is half a step of a type relative to the value, U = 2^-24
 """
 import math
 import os
+import random
 import sys
 
 import pytest
@@ -394,7 +395,7 @@ def check_norm(sc, dt, x, groups, gamma, beta, o, layout, act, eps=1e-5, out=Non
     y = sc.group_norm(x, groups, gamma, beta, layout=layout, eps=eps, activation=act, out=out)
     torch.cuda.synchronize()
     want, size = orc.group_norm(src, groups, gamma, beta, o, eps=eps, activation=act)
-    n = max(b - a for a, b in zip(o, o[1:])) * (x.shape[1] // groups)
+    n = max([1] + [b - a for a, b in zip(o, o[1:])]) * (x.shape[1] // groups)
     within(y, want, 1.1 * (64 + n / 256) * U * size + half(dt) * want.abs() + torch.finfo(DT[dt]).tiny, act)
     return y
 
@@ -652,3 +653,117 @@ def test_norm_offsets_past_32_bits(sc, series):
     tol = 1.1 * (64 + n / 256) * U * size + half("bf16") * want.abs()
     within(y[-tail:], want, tol)
     within(y[:tail], want, tol)
+
+
+# ---- random cases, many series, the C interface ----------------------------------------------------------------------
+SEEDS = int(os.environ.get("DRLVAE_SWEEP_SEEDS", 24))
+
+
+def lengths_of(r, n, total):
+    return [r.choice([0, 1, 2, 31, 32, 33, 64, r.randint(1, total), r.randint(1, max(1, total // 4))]) for _ in range(n)]
+
+
+@pytest.mark.parametrize("seed", range(SEEDS))
+def test_attention_random(sc, seed):
+    r, g = random.Random(seed), torch.Generator().manual_seed(seed)
+    dt = r.choice(ALL)
+    G = r.choice([1, 1, 2, 3])
+    H, D = G * r.choice([1, 2, 3, 5, 8, 40]), 8 * r.randint(1, 16)
+    n = r.randint(1, 5)
+    qo = offs(lengths_of(r, n, 200 if H < 16 else 40), r.choice([0, 3]))
+    ko = qo if r.random() < 0.5 else offs(lengths_of(r, n, r.choice([100, 1500])), r.choice([0, 5]))
+    kr = ko[-1] + r.choice([0, 7])
+    q, k, v = normal(g, (qo[-1] + r.choice([0, 2]), H, D), dt, r.choice([0.3, 1.0, 3.0])), normal(g, (kr, G, D), dt), normal(g, (kr, G, D), dt)
+    mask = (torch.rand(kr, generator=g) < r.choice([0.1, 0.9])).cuda() if r.random() < 0.4 else None
+    k_len = torch.tensor([r.choice([0, 1, r.randint(0, 1600), 5000]) for _ in range(n)], dtype=torch.int32, device="cuda") if r.random() < 0.4 else None
+    check_attention(sc, dt, q, k, v, qo, ko, causal=r.random() < 0.7, window=r.choice([0, 0, 1, 20, 64, 300]), key_mask=mask, k_len=k_len)
+
+
+@pytest.mark.parametrize("seed", range(SEEDS))
+def test_linear_random(sc, seed):
+    r, g = random.Random(seed + 1000), torch.Generator().manual_seed(seed)
+    dt = r.choice(ALL)
+    G = r.choice([1, 2, 3])
+    H, dk, dv = G * r.choice([1, 2, 4]), 8 * r.randint(1, 16), 8 * r.randint(1, 32)
+    n = r.randint(1, 5)
+    o = offs(lengths_of(r, n, r.choice([60, 400])), r.choice([0, 3]))
+    q, k, v = normal(g, (o[-1], H, dk), dt), normal(g, (o[-1], G, dk), dt), normal(g, (o[-1], G, dv), dt, r.choice([0.01, 1.0]))
+    state = torch.randn(n, H, dk, dv, generator=g).cuda() if r.random() < 0.5 else None
+    check_linear(sc, dt, q, k, v, log_decay(g, H, r.choice(["memory", "ends"])), o, state=state)
+
+
+@pytest.mark.parametrize("seed", range(SEEDS))
+def test_norm_random(sc, seed):
+    r, g = random.Random(seed + 2000), torch.Generator().manual_seed(seed)
+    dt = r.choice(ALL)
+    G = r.choice([1, 2, 3, 8, 32])
+    C = G * r.choice([1, 2, 3, 7, 8, 12, 16, 64, 130])
+    n = r.randint(1, 6)
+    o = offs(lengths_of(r, n, r.choice([60, 3000 if C < 600 else 100])))
+    x = normal(g, (o[-1], C), dt, r.choice([0.1, 3.0])) + r.choice([0.0, 2.0])
+    gamma, beta = ((torch.rand(C, generator=g) + 0.5).cuda() if r.random() < 0.7 else None for _ in range(2))
+    if r.random() < 0.6:
+        check_norm(sc, dt, x, G, gamma, beta, o, sc.seq_layout(o), r.choice(["linear", "relu", "sigmoid", "silu"]))
+    else:
+        check_norm(sc, dt, x, G, gamma, beta, list(range(len(x) + 1)), None, r.choice(["linear", "relu", "sigmoid", "silu"]))
+
+
+def test_seventy_thousand_series(sc):
+    n, dt = 70000, "bf16"
+    g = torch.Generator().manual_seed(9)
+    lengths = torch.randint(0, 4, (n,), generator=g).tolist()
+    o = offs(lengths)
+    q, k, v = normal(g, (o[-1], 4, 16), dt), normal(g, (o[-1], 2, 16), dt), normal(g, (o[-1], 2, 16), dt)
+    ld, x = log_decay(g, 4), normal(g, (o[-1], 48), dt)
+    layout = sc.seq_layout(o)
+    a = sc.attention(q, k, v, layout)
+    b, state = sc.linear_attention(q, k, v, ld, layout)
+    c = sc.group_norm(x, 4, layout=layout)
+    for s in [0, 1, n // 2, n - 2, n - 1] + torch.randint(0, n, (60,), generator=g).tolist():
+        at, m = slice(o[s], o[s + 1]), [0, lengths[s]]
+        want, tol, _, _ = attention_bounds(dt, q[at], k[at], v[at], m, m, scale=0.25)
+        within(a[at], want, tol, s)
+        want, tol, S, stol = linear_bounds(dt, q[at], k[at], v[at], ld, m, 0.25)
+        within(b[at], want, tol, s)
+        within(state[s:s + 1], S, stol, s)
+        want, size = orc.group_norm(x[at], 4, None, None, m, eps=1e-5, activation="linear")
+        within(c[at], want, 1.1 * 65 * U * size + half(dt) * want.abs(), s)
+
+
+def test_the_c_interface_on_the_contexts_stream_and_its_workspaces(sc):
+    """Calls without a stream run on the context's; a workspace that is too small is refused before anything is written, one
+    of just the size is enough and nothing behind it is touched."""
+    import ctypes as C
+
+    from drlvae import _abi
+    g = torch.Generator().manual_seed(77)
+    rows, D = 6000, 64
+    q, k, v = (normal(g, (rows, 2, D), "bf16") for _ in range(3))
+    ld, x = log_decay(g, 2), normal(g, (rows, 64), "f32")
+    layout = sc.seq_layout([0, rows])
+    want = (sc.attention(q, k, v, layout), sc.linear_attention(q, k, v, ld, layout)[0], sc.group_norm(x, 1, layout=layout))
+    st = (2 * D, D) * 4
+    outs = [torch.full_like(w_, 7.0) for w_ in want]
+    final = torch.zeros(1, 2, D, D, device="cuda")
+    calls = [("attention", 2, (layout._h,), _abi.pack_attn(q.data_ptr(), k.data_ptr(), v.data_ptr(), outs[0].data_ptr(), 0, 0, 0, *st, 2, 2, D, 1, 0, D ** -0.5)),
+             ("linear_attention", 2, (layout._h,), _abi.pack_linear(q.data_ptr(), k.data_ptr(), v.data_ptr(), outs[1].data_ptr(), ld.data_ptr(), 0,
+                                                                    final.data_ptr(), *st, 2, 2, D, D, D ** -0.5, 0)),
+             ("group_norm", 0, (layout._h, rows), _abi.pack_norm(x.data_ptr(), outs[2].data_ptr(), 0, 0, 64, 64, 64, 1, 0, 1e-5))]
+    torch.cuda.synchronize()
+    for (name, code, head, args), out, exp in zip(calls, outs, want):
+        def pack(ws, size):
+            return _abi.pack_call(_abi.SEQ_CALL_SIZE, _abi.ABI_REVISION, code, 0, 0, ws, size)
+        need = C.c_int64(0)
+        assert getattr(sc._lib, f"drl_{name}_workspace")(sc._h, *head, pack(0, 0), args, C.byref(need)) == 0
+        assert need.value > 0, name
+        run = getattr(sc._lib, f"drl_{name}_dev")
+        ws = torch.full((need.value + 256,), 0xab, dtype=torch.uint8, device="cuda")
+        torch.cuda.synchronize()
+        for small in (pack(0, 0), pack(0, need.value), pack(ws.data_ptr(), need.value - 1)):
+            assert run(sc._h, *head, small, args) == -1, name
+        sc.synchronize()
+        assert torch.all(out == 7) and torch.all(ws == 0xab), name
+        assert run(sc._h, *head, pack(ws.data_ptr(), need.value), args) == 0, name
+        sc.synchronize()
+        assert torch.equal(out, exp), name
+        assert torch.all(ws[need.value:] == 0xab), name
