@@ -34,6 +34,9 @@ struct SegInfo {
 // A value that is the same in all lanes, into a scalar register.
 __device__ __forceinline__ float uniform(float x) { return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x))); }
 
+// What depends on x behind this stays in its branch; the compiler does without the branch otherwise, on every pass.
+__device__ __forceinline__ void rarely(int& x) { asm volatile("" : "+v"(x)); }
+
 // Lanes are joined without LDS: what lane l ^ M holds, where the lanes of each M hold the same (so that for 4 and 8 the
 // mirrored half row and row will do); 4 to 8 cycles each, where a shuffle through LDS takes a hundred.
 template <int M>

@@ -134,7 +134,7 @@ __device__ __forceinline__ float into_range(float x, float& back) {
 // weighted values are scaled by powers of two before they are rounded.
 // Two series of 32,768 rows, 32 heads of 128 x 128, bfloat16, in 16 pieces: 710-745 us by card, 300 for the pieces' states (a
 // second reading of k and v), 12 to join them, the rest the outputs; 2.15 GB once are 457 us.  VALU 54 % busy, matrix pipe
-// 44 %.  24 ragged series, 16 heads of 64 x 128, float16: 155 us, as long as the longest series' 64 chunks take, two
+// 44 %.  24 ragged series, 16 heads of 64 x 128, float16: 148 us, as long as the longest series' 64 chunks take, two
 // workgroups to a CU; VALU 54 % (scales and splits), matrix pipe 16 %; 92 us at a copy's rate.  Eight waves of 16 columns
 // instead of four of 32: 852 us against 760 at the time.
 template <typename T, int KT, int NW, bool STATE>
@@ -328,9 +328,11 @@ __global__ __launch_bounds__(NW * 64, STATE ? 3 : 2) void linear_chunk_kernel(Li
             if constexpr (F16)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) w[r] = fmaf(w[r], p_back, o[r]);
-            if (odd)
+            if (odd) {
+                rarely(bad);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) w[r] = col >= __shfl(bad, acc_row(r, half)) ? NAN : w[r];
+            }
             // Four columns of the lane's row are in four registers, the next four those of the lane 32 away: halves are
             // exchanged, and each lane writes eight.
             u32x4 out[2];
@@ -410,11 +412,13 @@ __global__ __launch_bounds__(NW * 64, STATE ? 3 : 2) void linear_chunk_kernel(Li
 #pragma unroll
             for (int r = 0; r < 16; ++r) S[kt][r] = F16 ? fmaf(acc[r], v_back, S[kt][r]) : acc[r];
         }
-        if (odd && bad < C)
+        if (odd) {
+            rarely(bad);
 #pragma unroll
             for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) S[kt][r] = NAN;
+                for (int r = 0; r < 16; ++r) S[kt][r] = bad < C ? NAN : S[kt][r];
+        }
     }
 
     float* to = nullptr;
