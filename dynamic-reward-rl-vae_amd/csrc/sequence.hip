@@ -128,6 +128,13 @@ void by_type(int dtype, F f) {
     else f((bf16*)nullptr);
 }
 
+// A kernel is a handle here, not a function that host code may call: launched through the runtime, not through the pointer.
+template <typename A>
+void launch(void (*kernel)(A), dim3 grid, dim3 block, size_t shmem, hipStream_t st, A args) {
+    void* p[] = {&args};
+    (void)hipLaunchKernel(reinterpret_cast<const void*>(kernel), grid, block, p, shmem, st);      // launched() says how it went
+}
+
 int launched(drl_ctx* c, const char* who) {
     const hipError_t err = hipGetLastError();
     return err == hipSuccess ? DRL_OK : hip_fail(c, who, err);
@@ -276,7 +283,7 @@ static void attn_tiles(const AttnPlan& p, const seq::AttnArgs& k, hipStream_t st
     const dim3 grid((unsigned)p.tiles, p.splits);
     auto go = [&](auto kernel, int waves, size_t shmem) {
         if (shmem > 64 * 1024) (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)shmem);
-        hipLaunchKernelGGL(kernel, grid, dim3(waves * 64), shmem, st, k);
+        launch(kernel, grid, dim3(waves * 64), shmem, st, k);
     };
     by_count(dt, [&](auto d) {
         constexpr int DT = decltype(d)::value;
@@ -291,7 +298,7 @@ static void attn_tiles(const AttnPlan& p, const seq::AttnArgs& k, hipStream_t st
     });
     if (p.splits > 1) {
         const dim3 jg((unsigned)((k.part_rows * k.heads + 3) / 4));
-        hipLaunchKernelGGL((seq::attn_join_kernel<T>), jg, dim3(256), 0, st, k);
+        launch((seq::attn_join_kernel<T>), jg, dim3(256), 0, st, k);
     }
 }
 
@@ -392,7 +399,7 @@ static void linear_chunks(const LinearPlan& p, const seq::LinearArgs& k, hipStre
     auto go = [&](auto kernel) {
         // more LDS than a kernel gets unasked
         if (stages * stage + table > 64 * 1024) (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, stages * stage + table);
-        hipLaunchKernelGGL(kernel, grid, dim3(NW * 64), stages * stage + table, st, k);
+        launch(kernel, grid, dim3(NW * 64), stages * stage + table, st, k);
     };
     if constexpr (sizeof(T) == 2) go(seq::linear_chunk_kernel<T, KT, NW, STATE>);
     else go(seq::linear_chunk32_kernel<KT, NW, STATE>);
@@ -414,7 +421,7 @@ static void linear_series(const LinearPlan& p, const seq::LinearArgs& k, hipStre
     if (k.states) {
         all(std::true_type());
         const dim3 grid(k.n_seg, k.heads, (k.dk * k.dv / 4 + 255) / 256);
-        hipLaunchKernelGGL(seq::linear_scan_kernel, grid, dim3(256), 0, st, k);
+        launch(seq::linear_scan_kernel, grid, dim3(256), 0, st, k);
     }
     all(std::false_type());
 }
@@ -455,7 +462,7 @@ int drl_linear_attention_step_dev(drl_ctx* c, int64_t n, const drl_seq_call* cal
     const seq::LinearArgs k = linear_args(a, nullptr, 0);
     by_type(call->dtype, [&](auto* t) {
         typedef std::remove_pointer_t<decltype(t)> T;
-        hipLaunchKernelGGL((seq::linear_step_kernel<T>), dim3((unsigned)(n * a->n_heads)), dim3(256), 0, stream_of(v, call), k);
+        launch((seq::linear_step_kernel<T>), dim3((unsigned)(n * a->n_heads)), dim3(256), 0, stream_of(v, call), k);
     });
     return launched(c, who);
 }
@@ -528,12 +535,12 @@ int drl_group_norm_workspace(drl_ctx* c, const drl_seq_layout* l, int64_t rows, 
 
 template <typename T, int V>
 static void norm_launch(const NormPlan& p, const seq::NormArgs& k, hipStream_t st) {
-    auto go = [&](auto kernel, dim3 grid) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, k); };
+    auto go = [&](auto kernel, dim3 grid) { launch(kernel, grid, dim3(256), 0, st, k); };
     if (p.share) {
         auto by = [&](auto r) {
             constexpr int R = decltype(r)::value;
             const dim3 grid((unsigned)((int64_t)((k.n_seg + 7) / 8) * 8 * k.groups));
-            auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(p.threads), 0, st, k); };
+            auto run = [&](auto kernel) { launch(kernel, grid, dim3(p.threads), 0, st, k); };
             if (p.threads == 1024) run(seq::norm_short_kernel<T, V, R, 1024>);
             else if constexpr (R <= 2) run(seq::norm_short_kernel<T, V, R, 256>);
         };
