@@ -767,3 +767,68 @@ def test_the_c_interface_on_the_contexts_stream_and_its_workspaces(sc):
         sc.synchronize()
         assert torch.equal(out, exp), name
         assert torch.all(ws[need.value:] == 0xab), name
+
+
+@pytest.mark.parametrize("dt", ALL)
+def test_broadcast_rows_and_heads(sc, dt):
+    """Strides of 0: one row of k for all, kv heads that share their memory, one row of q for all."""
+    g = torch.Generator().manual_seed(51)
+    n, D = 150, 40
+    q, k, v = normal(g, (n, 4, D), dt), normal(g, (n, 1, D), dt), normal(g, (n, 1, D), dt)
+    for a, b, c in ((q, k[:1].expand(n, 1, D), v), (q, k.expand(n, 2, D), v.expand(n, 2, D)), (q[:1].expand(n, 4, D), k, v[:1].expand(n, 1, D))):
+        check_attention(sc, dt, a, b, c, [0, 70, n], None)
+        check_linear(sc, dt, a, b, c, log_decay(g, 4), [0, 70, n])
+
+
+def test_layouts_outlive_their_scorer_and_serve_others(sc):
+    from drlvae.scorer import WindowScorer
+    g = torch.Generator().manual_seed(52)
+    q, k, v = (normal(g, (300, h, 32), "bf16") for h in (4, 2, 2))
+    o = [0, 120, 300]
+    other = WindowScorer(0)
+    theirs = other.seq_layout(o)
+    a = other.attention(q, k, v, theirs)
+    other.close()
+    assert torch.equal(sc.attention(q, k, v, theirs), a)
+    assert torch.equal(sc.attention(q, k, v, sc.seq_layout(o)), a)
+    theirs.close()
+    with pytest.raises(ValueError, match="closed"):
+        sc.attention(q, k, v, theirs)
+
+
+def test_threads_with_streams_and_layouts_of_their_own(sc):
+    import threading
+
+    from drlvae.scorer import WindowScorer
+    g = torch.Generator().manual_seed(53)
+    x = [[normal(g, (2000, h, 64), "f16") for h in (4, 2, 2)] for _ in range(4)]
+    ld = log_decay(g, 4)
+    cuts = [[0, 13 * i + 1, 700 + i, 2000] for i in range(4)]
+
+    def work(s, i):
+        layout = s.seq_layout(cuts[i])
+        a = s.attention(*x[i], layout, window=90)
+        b, _ = s.linear_attention(*x[i], ld, layout)
+        return a, b, s.group_norm(a.reshape(2000, 256), 4, layout=layout)
+
+    want = [work(sc, i) for i in range(4)]
+    torch.cuda.synchronize()
+    bad = []
+
+    def run(i):
+        try:
+            s, stream = WindowScorer(0), torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                got = [work(s, i) for _ in range(40)]
+            stream.synchronize()
+            bad.extend((i, r) for r, outs in enumerate(got) if not all(torch.equal(u, w) for u, w in zip(outs, want[i])))
+            s.close()
+        except Exception as e:                                 # a thread's failure is the test's
+            bad.append((i, repr(e)))
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad, bad[:3]
