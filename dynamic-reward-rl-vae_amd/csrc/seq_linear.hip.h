@@ -115,9 +115,11 @@ __global__ __launch_bounds__(256) void linear_step_kernel(LinearArgs a) {
     }
 }
 
-// 2^-e with |x| 2^-e in [2^13, 2^14), for scaling into float16's range; 1 for 0 and what is not finite.
+// 2^-e with |x| 2^-e in [2^13, 2^14), for scaling into float16's range; 1 for 0 and what is not finite.  e stops at -112: below,
+// the factor would pass float32's range, and a column that dies out would turn into infinities and, where it holds zeros,
+// NaN.  What is lost of smaller values, 2^-137, is below float32's own normal range.
 __device__ __forceinline__ float into_range(float x, float& back) {
-    const int e = x > 0.0f && x < INFINITY ? __builtin_amdgcn_frexp_expf(x) - 14 : 0;
+    const int e = x > 0.0f && x < INFINITY ? max(__builtin_amdgcn_frexp_expf(x) - 14, -112) : 0;
     back = __builtin_amdgcn_ldexpf(1.0f, e);
     return __builtin_amdgcn_ldexpf(1.0f, -e);
 }
@@ -131,7 +133,8 @@ __device__ __forceinline__ float into_range(float x, float& back) {
 // Rounding: scores and the state's copy are rounded to the inputs' type (relative error eps/2, like the result's own);
 // the float32 state itself takes lam^(n-1-j) v_j as the sum of N parts of that type (24 bits of bfloat16 in three, 22 of
 // float16 in two), and loses nothing from call to call.  float16 has no range to spare: scores, state columns and
-// weighted values are scaled by powers of two before they are rounded.
+// weighted values are scaled by powers of two before they are rounded, so that what is below 2^-38 of the largest score of a
+// row, or value of a column and chunk, is lost.
 // Two series of 32,768 rows, 32 heads of 128 x 128, bfloat16, in 16 pieces: 710-745 us by card, 300 for the pieces' states (a
 // second reading of k and v), 12 to join them, the rest the outputs; 2.15 GB once are 457 us.  VALU 54 % busy, matrix pipe
 // 44 %.  24 ragged series, 16 heads of 64 x 128, float16: 148 us, as long as the longest series' 64 chunks take, two

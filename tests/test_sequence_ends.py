@@ -1,0 +1,68 @@
+"""The sequence operators where values, alignments and callers are at their ends: columns that die out, the largest values,
+thousands of steps, tensors with tangents, errors that others left.  Bounds are those of test_sequence.py, with what is
+added named beside it."""
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from test_sequence import ALL, DT, U, half, linear_bounds, log_decay, normal, offs, within  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def sc():
+    from drlvae.scorer import WindowScorer
+    s = WindowScorer(0)
+    yield s
+    s.close()
+
+
+# ---- linear attention: values that die out ---------------------------------------------------------------------------
+def check_linear_tiny(sc, dt, q, k, v, ld, o, state=None):
+    """As check_linear; what lies below float32's normal range, 2^-126, may be taken as 0 in each of a chunk's 32 rows and
+    of the dk products of a state with q.  float16: a column x of weighted values is scaled so that its largest lies in [2^13,
+    2^14), and then rounded in two parts, the second one to a multiple of 2^-24: off by 2^-25, which is 2^-38 of the
+    largest at most; times |k|, over a chunk's 32 rows, and for all chunks before, decayed by lam^32 < 1/2 each where only
+    some rows are 0, a factor of 2 (a column of zeros loses nothing)."""
+    dk = q.shape[2]
+    out, final = sc.linear_attention(q, k, v, ld, sc.seq_layout(o), state=state)
+    want, tol, S, stol = linear_bounds(dt, q, k, v, ld, o, dk ** -0.5, state)
+    km, vm, qm = (float(x.abs().max()) for x in (k, v, q))
+    floor = 2.0 ** -126 + (2 * 2.0 ** -38 if dt == "f16" else 0)
+    within(final, S, stol + 32 * km * vm * floor, "final state")
+    within(out, want, tol + (dk + 32 * dk * km * vm) * qm * 2.0 ** -126, "out")
+
+
+@pytest.mark.parametrize("dt", ALL)
+@pytest.mark.parametrize("others", [0, 63])
+def test_linear_a_state_whose_columns_die_out(sc, dt, others):
+    """A few columns of v hold nothing: there the first state decays through the whole range of float32.  One series alone is
+    cut into pieces, one among 64 is not."""
+    g = torch.Generator().manual_seed(61)
+    o = offs([4200] + [1] * others)
+    q, k, v = normal(g, (o[-1], 4, 16), dt), normal(g, (o[-1], 4, 16), dt), normal(g, (o[-1], 4, 32), dt)
+    v[:, :, 3:7] = 0
+    ld = torch.log1p(-torch.exp2(-torch.tensor([5.0, 7.0, 9.0, 12.0], dtype=torch.float64))).float().cuda()
+    check_linear_tiny(sc, dt, q, k, v, ld, o, state=normal(g, (1 + others, 4, 16, 32), "f32", 3.0))
+
+
+@pytest.mark.parametrize("dt", ALL)
+@pytest.mark.parametrize("what", ["k", "v"])
+@pytest.mark.parametrize("d", [-2.0, -2.8, -3.0, -3.5])
+def test_linear_chunks_that_end_in_zeros(sc, dt, what, d):
+    """In each series the rows of a chunk behind the first so many are 0 in k or v: scores and weighted values of what is
+    left are powers of the decay from 1 down to nothing."""
+    g = torch.Generator().manual_seed(62)
+    first = [1, 2, 3, 4, 5, 6, 8, 12]
+    o = offs([96] * len(first))
+    q, k, v = normal(g, (o[-1], 2, 32), dt), normal(g, (o[-1], 2, 32), dt), normal(g, (o[-1], 2, 32), dt)
+    x = {"k": k, "v": v}[what]
+    for s, n in enumerate(first):
+        for c in range(3):
+            x[o[s] + 32 * c + n:o[s] + 32 * c + 32] = 0
+    ld = torch.tensor([d, d - 0.1], device="cuda")
+    check_linear_tiny(sc, dt, q, k, v, ld, o)
+    check_linear_tiny(sc, dt, q, k, v, ld, [0, 96], state=normal(g, (1, 2, 32, 32), "f32"))
