@@ -254,7 +254,7 @@ class SequenceOps:
         if layout is None:
             self._run("group_norm", x.dtype, x, (None, rows), args, None)
         else:
-            # the plan goes by what x and out are aligned to as well
+            # the plan goes by what x and out, and their rows, are aligned to as well
             self._run("group_norm", x.dtype, x, (layout._h, rows), args,
-                      (layout._plans, (2, x.dtype, c, groups, (xp | yp | xr * 16 | yr * 16) & 255)))
+                      (layout._plans, (2, x.dtype, c, groups, (xp | yp) & 15, (xr | yr) & 7)))
         return out

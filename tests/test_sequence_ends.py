@@ -66,3 +66,23 @@ def test_linear_chunks_that_end_in_zeros(sc, dt, what, d):
     ld = torch.tensor([d, d - 0.1], device="cuda")
     check_linear_tiny(sc, dt, q, k, v, ld, o)
     check_linear_tiny(sc, dt, q, k, v, ld, [0, 96], state=normal(g, (1, 2, 32, 32), "f32"))
+
+
+# ---- group norm: one layout, calls of several alignments -------------------------------------------------------------
+@pytest.mark.parametrize("dt,C,G,lengths,widths", [("bf16", 64, 8, [8000] * 4, (80, 81)), ("f32", 128, 8, [1461] * 67, (136, 138))])
+@pytest.mark.parametrize("turned", [False, True])
+def test_norm_of_one_layout_at_several_alignments(sc, dt, C, G, lengths, widths, turned):
+    """Column slices of parents of several widths, 16 or 32 bytes in: each call gets the scratch that it needs, whichever came
+    before; the same call with a layout of its own gives the same."""
+    g = torch.Generator().manual_seed(63)
+    o = offs(lengths)
+    layout = sc.seq_layout(o)
+    for width in widths[::-1] if turned else widths:
+        parent, results = normal(g, (o[-1], width), dt), [torch.zeros(o[-1], width, dtype=DT[dt], device="cuda") for _ in range(2)]
+        for at in (16 // parent.element_size(), 32 // parent.element_size()):
+            if at + C > width:
+                continue
+            x = parent[:, at:at + C]
+            assert torch.equal(sc.group_norm(x, G, layout=layout), sc.group_norm(x, G, layout=sc.seq_layout(o)))
+            a, b = (sc.group_norm(x, G, layout=use, out=r[:, at:at + C]) for use, r in zip((layout, sc.seq_layout(o)), results))
+            assert torch.equal(a, b)
