@@ -20,12 +20,14 @@ _dtypes = {}
 
 
 _stream = None
+_fw = None
 
 
 def _t():
-    global _torch, _stream
+    global _torch, _stream, _fw
     if _torch is None:
         import torch
+        import torch.autograd.forward_ad as _fw
         _dtypes.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
         _stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda d: torch.cuda.current_stream(d).cuda_stream)
         _torch = torch
@@ -86,6 +88,9 @@ class SequenceOps:
             raise ValueError(f"{name} is on {x.device}, the scorer on GPU {self.device}")
         if x.requires_grad and torch.is_grad_enabled():
             raise ValueError(f"{name} requires a gradient: the sequence operators are forward only (use torch.no_grad())")
+        # outside of a dual level (its number, -1 there, is cheaper to ask for) no tensor has a tangent
+        if getattr(_fw, "_current_level", 0) >= 0 and _fw.unpack_dual(x).tangent is not None:
+            raise ValueError(f"{name} has a forward-mode tangent: the sequence operators have no derivatives")
         return shape
 
     def _rows(self, name, x, dtype, rows, heads=None, dim=None):

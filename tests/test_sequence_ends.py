@@ -86,3 +86,29 @@ def test_norm_of_one_layout_at_several_alignments(sc, dt, C, G, lengths, widths,
             assert torch.equal(sc.group_norm(x, G, layout=layout), sc.group_norm(x, G, layout=sc.seq_layout(o)))
             a, b = (sc.group_norm(x, G, layout=use, out=r[:, at:at + C]) for use, r in zip((layout, sc.seq_layout(o)), results))
             assert torch.equal(a, b)
+
+
+# ---- tangents ----------------------------------------------------------------------------------------------------------
+def test_tensors_with_a_tangent_are_refused(sc):
+    """There is no forward-mode derivative: a call must not return a result without its tangent."""
+    import torch.autograd.forward_ad as fw
+    x, ld = torch.randn(4, 2, 32, device="cuda"), torch.zeros(2, device="cuda")
+    state, w, layout = torch.zeros(4, 2, 32, 32, device="cuda"), torch.ones(64, device="cuda"), sc.seq_layout([0, 4])
+    flat = x.view(4, 64)
+    with fw.dual_level():
+        dual = lambda t: fw.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for i in range(3):
+            a = [dual(x) if j == i else x for j in range(3)]
+            for f in (lambda: sc.attention(*a, layout), lambda: sc.linear_attention(*a, ld, layout), lambda: sc.linear_attention_step(*a, ld, state)):
+                with pytest.raises(ValueError, match="tangent"):
+                    f()
+        for f in (lambda: sc.linear_attention(x, x, x, dual(ld), layout), lambda: sc.linear_attention_step(x, x, x, ld, dual(state)),
+                  lambda: sc.linear_attention(x, x, x, ld, layout, state=dual(state[:1])),
+                  lambda: sc.group_norm(dual(flat), 2), lambda: sc.group_norm(flat, 2, dual(w)), lambda: sc.group_norm(flat, 2, w, dual(w)),
+                  lambda: sc.attention(x, x, x, layout, out=dual(x))):
+            with pytest.raises(ValueError, match="tangent"):
+                f()
+        want = sc.attention(x, x, x, layout)                     # a tensor without one is none the worse
+    with pytest.raises(ValueError, match="tangent"):
+        torch.func.jvp(lambda t: sc.group_norm(t, 2), (flat,), (flat,))
+    assert torch.equal(sc.attention(x, x, x, layout), want)
