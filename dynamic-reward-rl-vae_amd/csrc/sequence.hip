@@ -113,6 +113,7 @@ int fail(drl_ctx* c, const SeqError& e) { return drl_ctx_fail(c, e.code, e.msg);
 int hip_fail(drl_ctx* c, const char* who, hipError_t err) {
     SeqError e;
     e.set(DRL_ERR_HIP, "%s: %s", who, hipGetErrorString(err));
+    (void)hipGetLastError();               // reported here: not left for the caller's next question as well
     return fail(c, e);
 }
 
@@ -128,15 +129,28 @@ void by_type(int dtype, F f) {
     else f((bf16*)nullptr);
 }
 
+// How the launches of this thread's call went.  The runtime's own last error is no measure: it may be someone else's, and asking
+// for it takes it from them.
+thread_local hipError_t launch_error = hipSuccess;
+void keep_error(hipError_t err) {
+    if (launch_error == hipSuccess) launch_error = err;
+}
+
 // A kernel is a handle here, not a function that host code may call: launched through the runtime, not through the pointer.
 template <typename A>
 void launch(void (*kernel)(A), dim3 grid, dim3 block, size_t shmem, hipStream_t st, A args) {
     void* p[] = {&args};
-    (void)hipLaunchKernel(reinterpret_cast<const void*>(kernel), grid, block, p, shmem, st);      // launched() says how it went
+    keep_error(hipLaunchKernel(reinterpret_cast<const void*>(kernel), grid, block, p, shmem, st));
+}
+// More LDS than a kernel gets unasked.
+template <typename A>
+void allow_lds(void (*kernel)(A), size_t shmem) {
+    if (shmem > 64 * 1024) keep_error(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)shmem));
 }
 
 int launched(drl_ctx* c, const char* who) {
-    const hipError_t err = hipGetLastError();
+    const hipError_t err = launch_error;
+    launch_error = hipSuccess;
     return err == hipSuccess ? DRL_OK : hip_fail(c, who, err);
 }
 
@@ -282,7 +296,7 @@ static void attn_tiles(const AttnPlan& p, const seq::AttnArgs& k, hipStream_t st
     const size_t tile = 64 * sizeof(T) * (dt == 1 ? 1 : dt == 2 ? 2 : 4) * 16;    // 32 keys (or values)
     const dim3 grid((unsigned)p.tiles, p.splits);
     auto go = [&](auto kernel, int waves, size_t shmem) {
-        if (shmem > 64 * 1024) (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)shmem);
+        allow_lds(kernel, shmem);
         launch(kernel, grid, dim3(waves * 64), shmem, st, k);
     };
     by_count(dt, [&](auto d) {
@@ -397,8 +411,7 @@ static void linear_chunks(const LinearPlan& p, const seq::LinearArgs& k, hipStre
     constexpr int stage = 32 * sizeof(T) * ((STATE ? 1 : 2) * DP + 32 * NW), stages = sizeof(T) == 2 ? 3 : 2, table = sizeof(T) == 4 ? 0 : STATE ? 256 : 640 + 4096;
     const dim3 grid((unsigned)(p.units * k.heads * p.blocks));
     auto go = [&](auto kernel) {
-        // more LDS than a kernel gets unasked
-        if (stages * stage + table > 64 * 1024) (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, stages * stage + table);
+        allow_lds(kernel, stages * stage + table);
         launch(kernel, grid, dim3(NW * 64), stages * stage + table, st, k);
     };
     if constexpr (sizeof(T) == 2) go(seq::linear_chunk_kernel<T, KT, NW, STATE>);

@@ -112,3 +112,26 @@ def test_tensors_with_a_tangent_are_refused(sc):
     with pytest.raises(ValueError, match="tangent"):
         torch.func.jvp(lambda t: sc.group_norm(t, 2), (flat,), (flat,))
     assert torch.equal(sc.attention(x, x, x, layout), want)
+
+
+# ---- errors that others left -------------------------------------------------------------------------------------------
+def test_an_error_that_someone_else_left_is_not_taken_for_the_calls_own(sc):
+    """The runtime keeps the last error of a thread until it is asked for: a call that went well neither reports it nor clears it."""
+    import ctypes as C
+    with open("/proc/self/maps") as f:
+        hip = C.CDLL({line.split()[-1] for line in f if "libamdhip64" in line}.pop())
+    g = torch.Generator().manual_seed(64)
+    q, state, ld = normal(g, (3, 2, 32), "f32"), torch.zeros(3, 2, 32, 32, device="cuda"), log_decay(g, 2)
+    out, y = torch.empty_like(q), torch.empty(3, 64, device="cuda")
+    calls = [lambda: sc.linear_attention_step(q, q, q, ld, state, out=out), lambda: sc.group_norm(q.view(3, 64), 2, out=y)]
+    for call in calls:
+        call()
+        hip.hipGetLastError()
+        left = hip.hipSetDevice(1 << 20)                         # no such device: the runtime says so, nothing else happens
+        assert left != 0
+        try:
+            call()
+        finally:
+            kept = hip.hipGetLastError()
+        assert kept == left
+        assert hip.hipGetLastError() == 0
