@@ -76,7 +76,9 @@ __global__ __launch_bounds__(256) void linear_step_kernel(LinearArgs a) {
     if (on)
 #pragma unroll
         for (int e = 0; e < 4; ++e) vc[e] = (float)v[e];
-    const float lam = exp2_fast(decay_log(a, h) * LOG2E);
+    // lam - 1: lam itself, rounded, is off by the same 2^-25 in every step, which a long memory adds up (2,000 steps: 1e-4).  An
+    // infinite state, of which that would make a NaN, takes lam.
+    const float fall = expm1f(decay_log(a, h)), lam = 1.0f + fall;
     const int64_t sb = (row * a.heads + h) * (int64_t)a.dk * a.dv + x * 4;
     const float* in = a.state_in + sb;
     float* out = a.state_out + sb;
@@ -98,7 +100,8 @@ __global__ __launch_bounds__(256) void linear_step_kernel(LinearArgs a) {
                     const float kk = kq[0][r], qq = kq[1][r];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        S[u][e] = fmaf(kk, vc[e], lam * S[u][e]);
+                        const float kept = fabsf(S[u][e]) < INFINITY ? fmaf(S[u][e], fall, S[u][e]) : lam * S[u][e];
+                        S[u][e] = fmaf(kk, vc[e], kept);
                         acc[e] = fmaf(qq, S[u][e], acc[e]);
                     }
                     *(f32x4*)(out + (int64_t)r * a.dv) = S[u];

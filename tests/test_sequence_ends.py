@@ -135,3 +135,25 @@ def test_an_error_that_someone_else_left_is_not_taken_for_the_calls_own(sc):
             kept = hip.hipGetLastError()
         assert kept == left
         assert hip.hipGetLastError() == 0
+
+
+# ---- linear attention: thousands of steps ------------------------------------------------------------------------------
+def test_linear_steps_decay_as_much_as_the_series_do(sc):
+    """2,000 steps of nothing new: exp(d) must not be off by the same amount in each.  A step rounds the state once, by at most
+    U and to either side: the mean over 16,384 elements is sqrt(2000 / (3 x 16384)) U = 0.2 U off, 10 U at the very most; the
+    rate itself is known to 2 U of d a step."""
+    d = torch.tensor([-1e-3, -3.3e-4, -0.0101, -7e-5, 0.0, -0.0], device="cuda")
+    g = torch.Generator().manual_seed(65)
+    start = (1 + torch.rand(1, 6, 128, 128, generator=g)).cuda()
+    state, N = start.clone(), 2000
+    zero = torch.zeros(1, 6, 128, device="cuda")
+    for _ in range(N):
+        sc.linear_attention_step(zero, zero, zero, d, state)
+    want = torch.exp(d.double() * N)
+    off = ((state.double() / start.double()).mean((0, 2, 3)) / want - 1).abs()
+    assert torch.all(off <= 10 * U + 2 * U * N * d.double().abs()), off
+    assert torch.equal(state[:, 4:], start[:, 4:])
+    # a state that is not finite: as it was, decayed
+    state[0, :, 0, 0], state[0, :, 0, 1] = math.inf, math.nan
+    sc.linear_attention_step(zero, zero, zero, d, state)
+    assert torch.all(state[0, :, 0, 0] == math.inf) and torch.isnan(state[0, :, 0, 1]).all() and torch.isfinite(state[0, :, 1:]).all()
