@@ -76,6 +76,14 @@ __device__ constexpr float lift() { return __is_same(T, f16) ? 7.0f : 0.0f; }
 // m and l of a row to its log-sum; l = 0 where nothing was seen.
 __device__ __forceinline__ float log_sum(float m, float l) { return l == 0.0f ? -INFINITY : m + LN2 * __builtin_amdgcn_logf(l); }
 
+// A result in the inputs' type.  A mean of float16 values is inside the type's range; weights that are rounded up by up to 2^-11
+// could carry one of the largest values past it, to infinity.
+template <typename T>
+__device__ __forceinline__ T result(float x) {
+    if constexpr (__is_same(T, f16)) x = fabsf(x) < INFINITY ? __builtin_amdgcn_fmed3f(x, -65504.0f, 65504.0f) : x;
+    return (T)x;
+}
+
 // One row and head by one wave, straight from the definition, over the keys [from, to): a lane per key for the scores,
 // lanes over the width for the sum.  Touches nothing but the visible keys' rows.  Where a tile holds values that are
 // not finite and that some of its rows must not see, its rows are computed like this.
@@ -130,8 +138,8 @@ __device__ __forceinline__ void attn_row(const AttnArgs& a, const SegInfo& s, in
         return;
     }
     T* o = (T*)a.out + row * a.o_row + (int64_t)h * a.o_head;
-    if (lane < a.dim) o[lane] = (T)(o0 * inv);
-    if (lane + 64 < a.dim) o[lane + 64] = (T)(o1 * inv);
+    if (lane < a.dim) o[lane] = result<T>(o0 * inv);
+    if (lane + 64 < a.dim) o[lane + 64] = result<T>(o1 * inv);
     if (a.lse && lane == 0) a.lse[row * a.heads + h] = lse;
 }
 
@@ -191,7 +199,7 @@ __device__ __forceinline__ void attn_store(const AttnArgs& a, const AttnTile& t,
 #pragma unroll
         for (int r = 0; r < 16; r += 4) {
             const int d = (first + dt) * 32 + acc_row(r, half);
-            const Four w = {{(T)(o[dt][r] * inv), (T)(o[dt][r + 1] * inv), (T)(o[dt][r + 2] * inv), (T)(o[dt][r + 3] * inv)}};
+            const Four w = {{result<T>(o[dt][r] * inv), result<T>(o[dt][r + 1] * inv), result<T>(o[dt][r + 2] * inv), result<T>(o[dt][r + 3] * inv)}};
             if (d < a.dim) *(Four*)(out + d) = w;
         }
     if (a.lse && half == 0 && first == 0) a.lse[row * a.heads + h] = lse;
@@ -895,8 +903,8 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
     const int64_t row = a.row0 + id / a.heads;
     const int h = (int)(id % a.heads);
     T* out = (T*)a.out + row * a.o_row + (int64_t)h * a.o_head;
-    if (lane < a.dim) out[lane] = (T)(o0 * inv);
-    if (lane + 64 < a.dim) out[lane + 64] = (T)(o1 * inv);
+    if (lane < a.dim) out[lane] = result<T>(o0 * inv);
+    if (lane + 64 < a.dim) out[lane + 64] = result<T>(o1 * inv);
     if (a.lse && lane == 0) a.lse[row * a.heads + h] = log_sum(mm, l);
 }
 

@@ -157,3 +157,24 @@ def test_linear_steps_decay_as_much_as_the_series_do(sc):
     state[0, :, 0, 0], state[0, :, 0, 1] = math.inf, math.nan
     sc.linear_attention_step(zero, zero, zero, d, state)
     assert torch.all(state[0, :, 0, 0] == math.inf) and torch.isnan(state[0, :, 0, 1]).all() and torch.isfinite(state[0, :, 1:]).all()
+
+
+# ---- attention: the largest values of a type ---------------------------------------------------------------------------
+@pytest.mark.parametrize("nq,nk", [(64, 400), (64, 3000), (1, 400), (1, 30000)])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_attention_of_float16s_largest_values_stays_finite(sc, nq, nk, sign):
+    """A mean of values of 65504 is 65504; the weights here are all rounded up, by 3.5e-4, which would carry it past the type's
+    range.  A column that holds an infinity does not get a finite value."""
+    z = math.log(64.04 / 128)
+    hi = torch.tensor(z).half()
+    q, k, v = (torch.zeros(n, 1, 32, dtype=torch.float16) for n in (nq, nk, nk))
+    q[:, :, :2] = 1
+    k[1:, :, 0], k[1:, :, 1] = hi, (z - hi.double()).half()
+    v[:] = sign * 65504.0
+    v[:, :, 5] = 0
+    v[nk // 2, :, 5] = sign * math.inf
+    out = sc.attention(q.cuda(), k.cuda(), v.cuda(), sc.seq_layout([0, nq], [0, nk]), scale=1.0, causal=False)
+    keep = [d for d in range(32) if d != 5]
+    assert not torch.isfinite(out[..., 5]).any()
+    assert torch.isfinite(out[..., keep]).all()
+    assert float((out[..., keep].double().cpu() - sign * 65504.0).abs().max()) <= 65504 * 3 * half("f16")
