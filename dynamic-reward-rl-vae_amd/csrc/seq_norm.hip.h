@@ -23,10 +23,20 @@ struct NormArgs {
     float* part;              // [units][groups][2]: mean and squared deviation of a unit's rows (NULL: one unit per series)
 };
 
+// In float32 the exponent is taken in two parts, the second times ln 2 as a factor: one product's rounding alone, relative to
+// the exponent, would make the result's relative error grow with |x| (4e-6 at -40).  What is rounded to 16 bits does not show it.
+template <typename T>
 __device__ __forceinline__ float activate(float x, int act) {
     if (act == 1) return x < 0.0f ? 0.0f : x;                       // a NaN stays one
     if (act == 0) return x;
-    const float s = __builtin_amdgcn_rcpf(1.0f + exp2_fast(-LOG2E * x));
+    float e;
+    if constexpr (sizeof(T) == 4) {
+        constexpr float LOG2E_REST = 1.9259629911e-8f;              // log2(e) - LOG2E
+        const float t = -LOG2E * x;
+        e = exp2_fast(t);                                           // infinite, or nothing beside 1, from 128 on
+        e = fabsf(t) < 128.0f ? fmaf(e * LN2, fmaf(-LOG2E_REST, x, fmaf(-LOG2E, x, -t)), e) : e;
+    } else e = exp2_fast(-LOG2E * x);
+    const float s = __builtin_amdgcn_rcpf(1.0f + e);
     return act == 2 ? s : x * s;
 }
 
@@ -115,7 +125,7 @@ __global__ __launch_bounds__(256) void norm_rows_kernel(NormArgs a) {
             for (int n = 0; n < NV; ++n) {
                 P p;
 #pragma unroll
-                for (int e = 0; e < V; ++e) p.e[e] = (T)activate(fmaf(f[n][e] * rstd, ga[n][e], be[n][e]), a.act);
+                for (int e = 0; e < V; ++e) p.e[e] = (T)activate<T>(fmaf(f[n][e] * rstd, ga[n][e], be[n][e]), a.act);
                 if (on && sub + n * a.lanes < nv) *(P*)(y + (sub + n * a.lanes) * V) = p;
             }
         }
@@ -144,7 +154,7 @@ __global__ __launch_bounds__(256) void norm_rows_kernel(NormArgs a) {
 #pragma unroll
                     for (int e = 0; e < V; ++e) {
                         const int c = c0 + n * V + e;
-                        p.e[e] = (T)activate(fmaf(((float)p.e[e] - mean) * rstd, a.gamma ? a.gamma[c] : 1.0f, a.beta ? a.beta[c] : 0.0f), a.act);
+                        p.e[e] = (T)activate<T>(fmaf(((float)p.e[e] - mean) * rstd, a.gamma ? a.gamma[c] : 1.0f, a.beta ? a.beta[c] : 0.0f), a.act);
                     }
                     *(P*)(y + n * V) = p;
                 }
@@ -206,7 +216,7 @@ __global__ __launch_bounds__(THREADS) void norm_short_kernel(NormArgs a) {
 #pragma unroll
             for (int e = 0; e < V; ++e) {
                 const int c = c0 + pos[n] + e;
-                q.e[e] = (T)activate(fmaf(((float)p[n].e[e] - mean) * rstd, a.gamma ? a.gamma[c] : 1.0f, a.beta ? a.beta[c] : 0.0f), a.act);
+                q.e[e] = (T)activate<T>(fmaf(((float)p[n].e[e] - mean) * rstd, a.gamma ? a.gamma[c] : 1.0f, a.beta ? a.beta[c] : 0.0f), a.act);
             }
             *(P*)(y + (int64_t)row[n] * a.y_row + pos[n]) = q;
         }
@@ -322,7 +332,7 @@ __global__ __launch_bounds__(256) void norm_series_kernel(NormArgs a) {
         }
         auto put = [&](P p, int r) {
 #pragma unroll
-            for (int e = 0; e < V; ++e) p.e[e] = (T)activate(fmaf(((float)p.e[e] - mean) * rstd, ga[e], be[e]), a.act);
+            for (int e = 0; e < V; ++e) p.e[e] = (T)activate<T>(fmaf(((float)p.e[e] - mean) * rstd, ga[e], be[e]), a.act);
             *(P*)(y + (int64_t)r * a.y_row + v * V) = p;
         };
         int r = r0;

@@ -178,3 +178,20 @@ def test_attention_of_float16s_largest_values_stays_finite(sc, nq, nk, sign):
     assert not torch.isfinite(out[..., 5]).any()
     assert torch.isfinite(out[..., keep]).all()
     assert float((out[..., keep].double().cpu() - sign * 65504.0).abs().max()) <= 65504 * 3 * half("f16")
+
+
+# ---- group norm: the activations' far ends ------------------------------------------------------------------------------
+@pytest.mark.parametrize("act", ["sigmoid", "silu"])
+@pytest.mark.parametrize("rows,G,series", [(5, 16, False), (5, 1, False), (40, 16, True), (40, 1, True)])
+def test_norm_activations_keep_their_relative_error(sc, act, rows, G, series):
+    """gamma 0: y = act(beta), at beta from -80 to 80.  exp by a base of 2 within 2 U (its argument in two parts, the second
+    one's own rounding far below U), a sum U, a reciprocal 2 U, a product U; 2 U for what second orders there are: 8 U.  At
+    -200 the result, 1e-87, is none of float32's: 2^-126, where its normal range ends."""
+    beta = torch.linspace(-80, 80, 4096)
+    beta[7::512] = torch.tensor([math.inf, -math.inf, math.nan, 1e30, -1e30, 200.0, -200.0, 3e38])
+    g = torch.Generator().manual_seed(66)
+    x = normal(g, (rows, 4096), "f32")
+    y = sc.group_norm(x, G, torch.zeros(4096, device="cuda"), beta.cuda(), layout=sc.seq_layout([0, rows]) if series else None, activation=act)
+    b = beta.double()
+    want = (torch.sigmoid(b) if act == "sigmoid" else b * torch.sigmoid(b)).expand(rows, 4096)
+    within(y, want, 8 * U * want.abs() + 2.0 ** -126, act)
