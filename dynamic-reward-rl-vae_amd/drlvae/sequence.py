@@ -34,6 +34,17 @@ def _t():
     return _torch
 
 
+def _number(name, x):
+    """x as what a float32 argument can hold."""
+    if not -3.4e38 < x < 3.4e38:
+        raise ValueError(f"{name} {x} is not a float32 number")
+    return x
+
+
+def _scale(scale, dim):
+    return _number("scale", scale) if scale is not None else dim ** -0.5 if dim else 1.0
+
+
 class SeqLayout:
     """Which rows of packed tensors belong to which series: made once per batch layout with ``WindowScorer.seq_layout``
     and kept by the caller for as long as calls, or captured graphs, use it."""
@@ -171,15 +182,15 @@ class SequenceOps:
         if return_lse:
             lse = (q.new_empty if covered else q.new_zeros)((rows, heads), dtype=_torch.float32)
         if key_mask is not None:
+            mask = self._flat("key_mask", key_mask, None, k_rows)
             if key_mask.dtype not in (_torch.bool, _torch.uint8):
                 raise ValueError("key_mask must be bool or uint8")
-            mask = self._flat("key_mask", key_mask, None, k_rows)
         if k_len is not None:
             klen = self._flat("k_len", k_len, _torch.int32, layout.n_seg)
         window = max(-1, min(int(window), 0x7fffffff))             # more than any series has rows
         args = _abi.pack_attn(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(), mask, klen,
                               qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os_[0], os_[1], heads, kv, dim, 1 if causal else 0, window,
-                              dim ** -0.5 if scale is None else scale)
+                              _scale(scale, dim))
         self._run("attention", dtype, q, (layout._h,), args, (layout._plans, (0, dtype, heads, kv, dim, causal, window)))
         return out if lse is None else (out, lse)
 
@@ -211,7 +222,7 @@ class SequenceOps:
             last = self._state("final_state", final_state, shape)
         args = _abi.pack_linear(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), self._flat("log_decay", log_decay, _torch.float32, heads),
                                 first, last, qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os_[0], os_[1], heads, kv, dk, dv,
-                                dk ** -0.5 if scale is None else scale, 0)
+                                _scale(scale, dk), 0)
         self._run("linear_attention", dtype, q, (layout._h,), args, (layout._plans, (1, dtype, heads, kv, dk, dv)))
         return out, final_state
 
@@ -226,7 +237,7 @@ class SequenceOps:
         st = self._state("state", state, (n, heads, dk, dv))
         args = _abi.pack_linear(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), self._flat("log_decay", log_decay, _torch.float32, heads),
                                 st, st, qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os_[0], os_[1], heads, kv, dk, dv,
-                                dk ** -0.5 if scale is None else scale, 0)
+                                _scale(scale, dk), 0)
         self._run("linear_attention_step", dtype, q, (n,), args, None)
         return out
 
@@ -252,10 +263,11 @@ class SequenceOps:
         act = _ACTS.get(activation)
         if act is None:
             raise ValueError(f"activation {activation!r}: one of {', '.join(_ACTS)}")
+        groups = max(-1, min(int(groups), 0x7fffffff))             # more than any tensor has channels
         xp, yp = x.data_ptr(), out.data_ptr()
         xr, yr = (xs[0], ys[0]) if rows > 1 else (c, c)
         args = _abi.pack_norm(xp, yp, 0 if gamma is None else self._flat("gamma", gamma, _torch.float32, c),
-                              0 if beta is None else self._flat("beta", beta, _torch.float32, c), xr, yr, c, int(groups), act, eps)
+                              0 if beta is None else self._flat("beta", beta, _torch.float32, c), xr, yr, c, groups, act, _number("eps", eps))
         if layout is None:
             self._run("group_norm", x.dtype, x, (None, rows), args, None)
         else:

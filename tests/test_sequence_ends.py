@@ -195,3 +195,17 @@ def test_norm_activations_keep_their_relative_error(sc, act, rows, G, series):
     b = beta.double()
     want = (torch.sigmoid(b) if act == "sigmoid" else b * torch.sigmoid(b)).expand(rows, 4096)
     within(y, want, 8 * U * want.abs() + 2.0 ** -126, act)
+
+
+# ---- arguments that are something else -----------------------------------------------------------------------------------
+def test_arguments_of_another_kind_are_refused_by_name(sc):
+    x, ld, layout = torch.zeros(4, 2, 32, device="cuda"), torch.zeros(2, device="cuda"), sc.seq_layout([0, 4])
+    none = torch.zeros(4, 2, 0, device="cuda")
+    for f, match in ((lambda: sc.attention(x, x, x, layout, key_mask=[True] * 4), "key_mask"), (lambda: sc.attention(x, x, x, layout, k_len=[4]), "k_len"),
+                     (lambda: sc.attention(x, x, x, layout, scale=1e300), "scale"), (lambda: sc.linear_attention(x, x, x, ld, layout, scale=1e300), "scale"),
+                     (lambda: sc.linear_attention_step(x, x, x, ld, torch.zeros(4, 2, 32, 32, device="cuda"), scale=-1e39), "scale"),
+                     (lambda: sc.group_norm(x.view(4, 64), 2, eps=1e300), "eps"), (lambda: sc.group_norm(x.view(4, 64), 1 << 40), "groups"),
+                     (lambda: sc.attention(none, none, none, layout), "dim"), (lambda: sc.linear_attention(none, none, x, ld, layout), "dim"),
+                     (lambda: sc.linear_attention_step(none, none, x, ld, torch.zeros(4, 2, 0, 32, device="cuda")), "dim")):
+        with pytest.raises((ValueError, RuntimeError), match=match):
+            f()
