@@ -45,13 +45,20 @@ def _scale(scale, dim):
     return _number("scale", scale) if scale is not None else dim ** -0.5 if dim else 1.0
 
 
+def _whole(offsets):
+    a = np.asarray(offsets)
+    if a.size and a.dtype.kind not in "iu":
+        raise ValueError(f"offsets are whole numbers, not {a.dtype}")        # a fraction would be cut off without a word
+    return np.ascontiguousarray(a, dtype=np.int64)
+
+
 class SeqLayout:
     """Which rows of packed tensors belong to which series: made once per batch layout with ``WindowScorer.seq_layout``
     and kept by the caller for as long as calls, or captured graphs, use it."""
 
     def __init__(self, scorer, q_offsets: Sequence[int], k_offsets: Optional[Sequence[int]] = None):
-        q = np.ascontiguousarray(q_offsets, dtype=np.int64)
-        k = q if k_offsets is None else np.ascontiguousarray(k_offsets, dtype=np.int64)
+        q = _whole(q_offsets)
+        k = q if k_offsets is None else _whole(k_offsets)
         if q.ndim != 1 or k.ndim != 1 or len(q) < 1 or len(q) != len(k):
             raise ValueError("offsets are one-dimensional, n_seg + 1 entries, as many for k as for q")
         self._lib, self._h = scorer._lib, None

@@ -230,6 +230,20 @@ def test_python_refusals():
             s.seq_layout(q, k)
 
 
+def test_offsets_are_whole_numbers():
+    import numpy as np
+    import torch
+    s = _scorer()
+    for bad in ([0, 1.9], np.array([0.0, 4.0]), torch.tensor([0.0, 4.0]), [False, True], [0, 1 << 70]):
+        with pytest.raises(ValueError, match="whole numbers"):
+            s.seq_layout(bad)
+        with pytest.raises(ValueError, match="whole numbers"):
+            s.seq_layout([0, 4], bad)
+    for good in ([0, 4], range(0, 8, 4), np.array([0, 4], dtype=np.uint16), torch.tensor([0, 4]), (np.int32(0), 4)):
+        layout = s.seq_layout(good)
+        assert (layout.n_seg, layout.q_rows) == (1, 4)
+
+
 @pytest.mark.gpu
 def test_python_refusals_on_the_gpu():
     import torch
