@@ -138,6 +138,14 @@ int main() {
                     const double want = std::exp(std::min((double)ld.h[h], 0.0)) * st[at] + (double)k.h[(n * H + h) * D + d] * v.h[(n * H + h) * D + e];
                     EXPECT(near(st2[at], want, 10));
                 }
+    o = out.back();
+    for (int n = 0; n < 3; ++n)
+        for (int h = 0; h < H; ++h)
+            for (int e = 0; e < D; ++e) {
+                double want = 0;
+                for (int d = 0; d < D; ++d) want += 0.25 * st2[((n * H + h) * D + d) * D + e] * q.h[(n * H + h) * D + d];
+                EXPECT(near(o[(n * H + h) * D + e], want, 10));
+            }
     b.state_in = nullptr;
     EXPECT(drl_linear_attention_step_dev(ctx, 3, &call, &b) == DRL_ERR_ARG);
 
