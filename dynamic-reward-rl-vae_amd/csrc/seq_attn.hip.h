@@ -219,11 +219,9 @@ __device__ __forceinline__ void attn_store(const AttnArgs& a, const AttnTile& t,
 template <typename T, int DT, bool MASK>
 __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
     typedef typename Vec<T>::x8 x8;
-    typedef typename Vec<T>::x4 x4;
     constexpr int DP = DT <= 1 ? 32 : DT <= 2 ? 64 : 128;     // elements of a tile row in LDS
     constexpr int NC = DP / 8, KS = 2 * DT, BK = 64;
     constexpr int TILE = BK * DP * 2;                         // bytes of a tile of keys (or values)
-    constexpr int LOADS = BK * NC / 256;                      // 16-byte loads per thread and tile
     extern __shared__ char smem[];
     const uint32_t lds = lds_offset(smem);
     const AttnTile t = attn_tile(a, blockIdx.x);
@@ -456,7 +454,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
 template <int DT, bool LONG>
 __global__ __launch_bounds__(256, 2) void attn_tile32_kernel(AttnArgs a) {
     constexpr int DP = DT <= 1 ? 32 : DT <= 2 ? 64 : 128, NC = DP / 4, KS = 4 * DT, BK = 32;
-    constexpr int TILE = BK * DP * 4, LOADS = BK * NC / 256;
+    constexpr int TILE = BK * DP * 4;
     extern __shared__ char smem[];
     const uint32_t lds = lds_offset(smem);
     const AttnTile t = attn_tile(a, blockIdx.x);

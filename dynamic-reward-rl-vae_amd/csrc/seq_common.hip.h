@@ -151,7 +151,7 @@ struct TileLoad {
         if (width < NC * 16)
 #pragma unroll
             for (int n = 0; n < LOADS; ++n)
-                if (has(n) && chunk(n) >= width) *(__attribute__((address_space(3))) u32x4*)(tile + (n * THREADS + first) * 16) = u32x4{0, 0, 0, 0};
+                if (has(n) && chunk(n) >= width) *(__attribute__((address_space(3))) u32x4*)(uintptr_t)(tile + (n * THREADS + first) * 16) = u32x4{0, 0, 0, 0};
     }
     // The rows from `base` on, of which there are `rows`: behind them the last one again.  `tile`: where the wave's first
     // lane writes.
@@ -212,14 +212,14 @@ __device__ __forceinline__ bool not_finite(X... x) {
 }
 
 template <typename V>
-__device__ __forceinline__ V lds_read(uint32_t at) { return *(const __attribute__((address_space(3))) V*)at; }
+__device__ __forceinline__ V lds_read(uint32_t at) { return *(const __attribute__((address_space(3))) V*)(uintptr_t)at; }
 template <typename V>
-__device__ __forceinline__ void lds_write(uint32_t at, V x) { *(__attribute__((address_space(3))) V*)at = x; }
+__device__ __forceinline__ void lds_write(uint32_t at, V x) { *(__attribute__((address_space(3))) V*)(uintptr_t)at = x; }
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 // Lane i of a group of 16 names 8 bytes: row i / 4 of four, columns 4 (i % 4) ..; it gets column i of the four rows.
 __device__ __forceinline__ s16x4 lds_read_tr(uint32_t at) {
-    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at);
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(uintptr_t)at);
 }
 
 // x y, and 0 where one of them is 0, whatever the other holds (v_mul_legacy_f32).
