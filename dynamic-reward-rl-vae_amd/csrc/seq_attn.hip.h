@@ -30,9 +30,11 @@ struct AttnArgs {
     // heads of one kv head are cut into `blocks` runs of `rep_b`; a tile holds `per` rows of q of one run; every other
     // `turn` units go backwards
     int kv_blocks, blocks, rep_b, per, turn;
-    // the keys are cut into runs of `chunk` (splits > 1): partial results of run y, normalised, and their log-sums
+    // the keys are cut into runs of `chunk` (splits > 1): partial results of run y, normalised, and their references (in powers of
+    // two) and sums: a log-sum would be rounded to its own last place
     int splits, chunk;
-    float *part_o, *part_lse;      // [splits][rows][heads][dim], [splits][rows][heads], rows from the first series' first
+    float* part_o;                 // [splits][rows][heads][dim], rows from the first series' first
+    f32x2* part_ml;                // [splits][rows][heads]
     int64_t part_rows, row0;
 };
 
@@ -128,19 +130,19 @@ __device__ __forceinline__ void attn_row(const AttnArgs& a, const SegInfo& s, in
         }
     }
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;      // a NaN sum stays one
-    const float lse = log_sum(top == -INFINITY ? 0.0f : top, sum);
+    if (top == -INFINITY) top = 0.0f;
     if (a.splits > 1) {
         const int64_t at = ((int64_t)split * a.part_rows + row - a.row0) * a.heads + h;
         float* o = a.part_o + at * a.dim;
         if (lane < a.dim) o[lane] = o0 * inv;
         if (lane + 64 < a.dim) o[lane + 64] = o1 * inv;
-        if (lane == 0) a.part_lse[at] = lse;
+        if (lane == 0) a.part_ml[at] = f32x2{top * LOG2E, sum};
         return;
     }
     T* o = (T*)a.out + row * a.o_row + (int64_t)h * a.o_head;
     if (lane < a.dim) o[lane] = result<T>(o0 * inv);
     if (lane + 64 < a.dim) o[lane + 64] = result<T>(o1 * inv);
-    if (a.lse && lane == 0) a.lse[row * a.heads + h] = lse;
+    if (a.lse && lane == 0) a.lse[row * a.heads + h] = log_sum(top, sum);
 }
 
 // Which tile of which series a workgroup has: units of `per` rows, the longest series and the last rows (causal: the ones
@@ -173,11 +175,10 @@ __device__ __forceinline__ AttnTile attn_tile(const AttnArgs& a, uint32_t id) {
     return t;
 }
 
-// A wave's rows: o and l as they were summed, m the reference in natural units.
+// A wave's rows: o and l as they were summed, m the reference in powers of two.
 template <typename T, int DT>
 __device__ __forceinline__ void attn_store(const AttnArgs& a, const AttnTile& t, const f32x16 (&o)[DT], float l, float m, int i, int h, bool row_ok, int half, int first = 0) {
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;           // a NaN sum stays one
-    const float lse = log_sum(m, l);
     if (!row_ok) return;
     const int64_t row = t.s.q0 + i;
     if (a.splits > 1) {
@@ -189,7 +190,7 @@ __device__ __forceinline__ void attn_store(const AttnArgs& a, const AttnTile& t,
                 const int d = (first + dt) * 32 + acc_row(r, half);
                 if (d < a.dim) *(f32x4*)(a.part_o + at * a.dim + d) = f32x4{o[dt][r] * inv, o[dt][r + 1] * inv, o[dt][r + 2] * inv, o[dt][r + 3] * inv};
             }
-        if (half == 0 && first == 0) a.part_lse[at] = lse;
+        if (half == 0 && first == 0) a.part_ml[at] = f32x2{m, l};
         return;
     }
     T* out = (T*)a.out + row * a.o_row + (int64_t)h * a.o_head;
@@ -202,7 +203,7 @@ __device__ __forceinline__ void attn_store(const AttnArgs& a, const AttnTile& t,
             const Four w = {{result<T>(o[dt][r] * inv), result<T>(o[dt][r + 1] * inv), result<T>(o[dt][r + 2] * inv), result<T>(o[dt][r + 3] * inv)}};
             if (d < a.dim) *(Four*)(out + d) = w;
         }
-    if (a.lse && half == 0 && first == 0) a.lse[row * a.heads + h] = lse;
+    if (a.lse && half == 0 && first == 0) a.lse[row * a.heads + h] = log_sum(m * LN2, l);
 }
 
 // 16-bit types.  A workgroup of four waves has 128 rows, a wave 32 of them; keys and values go through LDS in tiles of 64
@@ -443,12 +444,12 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
         return;
     }
 
-    attn_store<T, DT>(a, t, o, pair_sum(l0 + l1), mc * LN2, i, h, row_ok, half);
+    attn_store<T, DT>(a, t, o, pair_sum(l0 + l1), mc, i, h, row_ok, half);
 }
 
 // float32.  The same on 32x32x2 products, with tiles of 32 keys: the matrix pipe is 16 times slower, and what it does takes
 // most of the time.  Here a score register is at once an operand of values^T x weights, and nothing is rounded.
-// 8 series of 1,000 rows of 8 heads, dim 128: 220 us, half of the float32 matrix peak; 67 series of 1,421 rows of 8 heads, dim
+// 8 series of 1,000 rows of 8 heads, dim 128: 224 us, matrix pipe 74 % busy; 67 series of 1,421 rows of 8 heads, dim
 // 32, windows of 50: 155 us, three tiles to a row of which two are edges, bound by how long one tile takes (matrix pipe 41 %
 // busy), with 82 us of reading and writing below it.
 template <int DT, bool LONG>
@@ -654,14 +655,16 @@ __global__ __launch_bounds__(256, 2) void attn_tile32_kernel(AttnArgs a) {
     for (int dt = 0; dt < ASIDE; ++dt)
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[dt][r] += aside[dt][r];
-    attn_store<float, DT>(a, t, o, pair_sum(l), mc * LN2, i, h, row_ok, half);
+    attn_store<float, DT>(a, t, o, pair_sum(l), mc, i, h, row_ok, half);
 }
 
-// At most 32 rows per kv head (steps).  Reading the cache is what takes the time: every wave has tiles of 32 keys of its own,
-// every NW-th, in two LDS buffers of its own, and waits for nothing but its own loads; at the end the waves' sums are
-// joined through LDS.  With 16-bit types, what the weights lose by rounding goes into a second product: it is free here.
-// 16 caches of up to 32,768 rows, 8 kv heads, dim 128, bfloat16: 256 us, 4.9 TB/s (a copy: 4.7); 4 of up to 384: 8.4 us in a
-// graph, of which the shortest launch is 5.4.
+// At most 32 rows per kv head (steps).  Reading the cache is what takes the time: every wave has tiles of 32 keys of its
+// own, every NW-th, in two LDS buffers of its own, and waits for nothing but its own loads (with a key mask, whose bytes are
+// asked for last, for those of the tile to come as well); at the end the waves' sums are joined through LDS.  With 16-bit
+// types, what the weights lose by rounding goes into a second product: it is free here. 16 caches of up to 32,768 rows, 8 kv
+// heads, dim 128, bfloat16: 256 us, 4.9 TB/s (a copy: 4.7), with a mask 292; 4 of up to 384: 8.4 us in a graph, of which the
+// shortest launch is 5.4.  In float32 the products bound it, of 32 rows where 4 are there: 16 caches of up to 16,384 rows,
+// 790 us, 1.9 TB/s.
 template <typename T, int DT, int NW>
 __global__ __launch_bounds__(NW * 64) void attn_step_kernel(AttnArgs a) {
     constexpr bool F32 = sizeof(T) == 4;
@@ -849,33 +852,31 @@ __global__ __launch_bounds__(NW * 64) void attn_step_kernel(AttnArgs a) {
 #pragma unroll
             for (int w = 0; w < NW; ++w) x[0][r] = fmaf(f[w], all[((w * DT + dt) * 16 + r) * 64 + lane], x[0][r]);
         }
-        attn_store<T, 1>(a, t, x, l, MM * LN2, i, h, row_ok, half, dt);
+        attn_store<T, 1>(a, t, x, l, MM, i, h, row_ok, half, dt);
     }
 }
 
-// Joins the runs of keys of a row and head: weights exp(lse_y - max), one wave each.  A run in which nothing is seen
-// (log-sum -inf) weighs nothing and its partial result is not read.  5 us for 16 rows of 32 heads: latency.
+// Joins the runs of keys of a row and head: weights l_y 2^(m_y - max), one wave each.  A run in which nothing is seen (l = 0)
+// weighs nothing and its partial result is not read.  5 us for 16 rows of 32 heads: latency.
 template <typename T>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
     const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (id >= a.part_rows * a.heads) return;
     const int lane = threadIdx.x & 63;
     const int64_t stride = a.part_rows * a.heads;
-    float m = -INFINITY, bad = 0.0f;
+    float m = -INFINITY;
     for (int y = lane; y < a.splits; y += 64) {
-        const float x = a.part_lse[y * stride + id];
-        m = fmaxf(m, x);
-        bad += x != x ? 1.0f : 0.0f;
+        const f32x2 x = a.part_ml[y * stride + id];
+        if (x[1] != 0.0f) m = fmaxf(m, x[0]);
     }
     m = wave_max(m);
-    if (wave_sum(bad) != 0.0f) m = NAN;
     const float mm = m == -INFINITY ? 0.0f : m;
     float l = 0.0f, o0 = 0.0f, o1 = 0.0f;
     for (int y0 = 0; y0 < a.splits; y0 += 64) {
-        const float x = y0 + lane < a.splits ? a.part_lse[(y0 + lane) * stride + id] : -INFINITY;
-        const float w = x == -INFINITY ? 0.0f : exp2_fast((x - mm) * LOG2E);
+        const f32x2 x = y0 + lane < a.splits ? a.part_ml[(y0 + lane) * stride + id] : f32x2{0.0f, 0.0f};
+        const float w = x[1] == 0.0f ? 0.0f : x[1] * exp2_fast(x[0] - mm);        // a NaN sum stays one
         l += w;
-        uint64_t todo = __ballot(x != -INFINITY);
+        uint64_t todo = __ballot(x[1] != 0.0f);
         while (todo) {
             int y[4];
             float wy[4], p0[4], p1[4];
@@ -903,7 +904,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
     T* out = (T*)a.out + row * a.o_row + (int64_t)h * a.o_head;
     if (lane < a.dim) out[lane] = result<T>(o0 * inv);
     if (lane + 64 < a.dim) out[lane + 64] = result<T>(o1 * inv);
-    if (a.lse && lane == 0) a.lse[row * a.heads + h] = log_sum(mm, l);
+    if (a.lse && lane == 0) a.lse[row * a.heads + h] = log_sum(mm * LN2, l);
 }
 
 }  // namespace seq

@@ -261,7 +261,7 @@ static AttnPlan attn_plan(const DrlCtxView& v, const drl_seq_layout* l, const dr
         p.chunk = (int)chunk;
     }
     p.longest = p.splits > 1 ? p.chunk : most;
-    if (p.splits > 1) p.workspace = (int64_t)p.splits * l->n_q * a->n_heads * (a->dim + 1) * 4;
+    if (p.splits > 1) p.workspace = (int64_t)p.splits * l->n_q * a->n_heads * (a->dim + 2) * 4;
     // Where all workgroups are resident at once, two per CU, each CU's second is taken from the other end of the order, so
     // that a long tile has a short one beside it (8,192 rows of 8 heads, dim 64: 124 -> 120 us, float32 834 -> 667; two
     // series of 4,096 84 -> 65, four of 2,048 45 -> 38).  Short ones would rather have the longest started first (eight
@@ -342,7 +342,7 @@ int drl_attention_dev(drl_ctx* c, const drl_seq_layout* l, const drl_seq_call* c
     k.part_rows = l->n_q; k.row0 = l->q_first;
     if (p.splits > 1) {
         k.part_o = (float*)call->workspace;
-        k.part_lse = k.part_o + (int64_t)p.splits * l->n_q * a->n_heads * a->dim;
+        k.part_ml = (seq::f32x2*)(k.part_o + (int64_t)p.splits * l->n_q * a->n_heads * a->dim);
     }
     const hipStream_t st = stream_of(v, call);
     by_type(call->dtype, [&](auto* t) { attn_tiles<std::remove_pointer_t<decltype(t)>>(p, k, st); });

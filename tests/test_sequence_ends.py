@@ -209,3 +209,21 @@ def test_arguments_of_another_kind_are_refused_by_name(sc):
                      (lambda: sc.linear_attention_step(none, none, x, ld, torch.zeros(4, 2, 0, 32, device="cuda")), "dim")):
         with pytest.raises((ValueError, RuntimeError), match=match):
             f()
+
+
+# ---- attention: runs of keys ------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dt", ALL)
+@pytest.mark.parametrize("nq,nk", [(1, 400), (1, 700), (9, 1500), (64, 1500)])
+def test_attention_joins_runs_of_keys_by_what_they_hold(sc, dt, nq, nk):
+    """Scores of 1.875 x 2^18 that float32 holds exactly, of a few keys, and others far below: the mean of the tied keys' values, to
+    the roundings of the weights, the sum and the result.  A log-sum of 491,520 is itself rounded to 1/32, which would weigh runs that hold
+    one and three of the keys alike to 3 %."""
+    g = torch.Generator().manual_seed(69)
+    a, b = 1.25 * 2.0 ** 7, 1.5 * 2.0 ** 6
+    q, k, v = torch.full((nq, 1, 32), a), torch.full((nk, 1, 32), b / 4), normal(g, (nk, 1, 32), dt)
+    at = torch.tensor([0, 1, 2, nk - 1])                      # three in the first run, one in the last
+    k[at] = b
+    out = sc.attention(q.to(DT[dt]).cuda(), k.to(DT[dt]).cuda(), v, sc.seq_layout([0, nq], [0, nk]), scale=1.0, causal=False)
+    want = v[at.cuda()].double().cpu().mean(0).expand(nq, 1, 32)
+    size = v[at.cuda()].double().cpu().abs().mean(0).expand(nq, 1, 32)
+    within(out, want, half(dt) * (want.abs() + size) + (nk + 64) * U * size, "ties")
