@@ -75,6 +75,31 @@ __device__ __forceinline__ uint64_t have_keys(int asked, int base, int end) {
 template <typename T>
 __device__ constexpr float lift() { return __is_same(T, f16) ? 7.0f : 0.0f; }
 
+// Beyond this the reference in powers of two, ref c1, has an error that an exponent shows: z c1 - mc is then up to half of mc's
+// last place for z = ref itself, not 0, and from 2^24 on weights pass float16's range, from 2^31 on float32's.  Where a row of the
+// wave is there, the reference is subtracted from the scores before the product; elsewhere a branch per tile (ragged batch
+// 132.3 -> 133.9 us, the other cases 0 to 1.3 % slower).
+constexpr float FAR = 0x1p20f;
+
+// The factor for what was summed with the reference `ref` (mc), when that becomes `now` (mcn).
+__device__ __forceinline__ float rescale(float ref, float mc, float now, float mcn, float c1) {
+    return ref == -INFINITY ? 0.0f : exp2_fast(fabsf(mcn) > FAR ? (ref - now) * c1 : mc - mcn);
+}
+
+// Whether a row of the wave is there; mz is what is subtracted from the product with c1, of scores or of what is left of them.
+__device__ __forceinline__ int far_away(float ref, float mc, float c1, float lift, float& mz) {
+    const int far = __builtin_amdgcn_readfirstlane(__any(fabsf(mc) > FAR));
+    mz = mc;
+    if (far) mz = fabsf(mc) > FAR ? -lift : ref == -INFINITY ? 0.0f : -fmaf(ref, c1, -mc);
+    return far;
+}
+__device__ __forceinline__ void from_reference(f32x16& z, float ref) {
+    float base = ref == -INFINITY ? 0.0f : ref;
+    asm volatile("" : "+v"(base));                           // this stays in its branch
+#pragma unroll
+    for (int r = 0; r < 16; ++r) z[r] -= base;
+}
+
 // m and l of a row to its log-sum; l = 0 where nothing was seen.
 __device__ __forceinline__ float log_sum(float m, float l) { return l == 0.0f ? -INFINITY : m + LN2 * __builtin_amdgcn_logf(l); }
 
@@ -294,6 +319,8 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
     constexpr bool F16 = __is_same(T, f16);
     const bool by_product = !F16 || c1 * 6.8e10f > 1000.0f;
     float ref = -INFINITY, mc = 0.0f;        // the reference, in units of the raw score; mc = ref * c1 - LIFT, 0 while there is none
+    float mz = 0.0f;
+    int far = 0;
     float l0 = 0.0f, l1 = 0.0f;
     f32x16 o[DT];
 #pragma unroll
@@ -394,9 +421,10 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
         if (__any((m - ref) * c1 > 8.0f)) {
             const float now = fmaxf(m, ref);
             const float mcn = now == -INFINITY ? 0.0f : now * c1 - LIFT;
-            const float f = ref == -INFINITY ? 0.0f : exp2_fast(mc - mcn);
+            const float f = rescale(ref, mc, now, mcn, c1);
             ref = now;
             mc = mcn;
+            far = far_away(ref, mc, c1, LIFT, mz);
             l0 *= f;
             l1 *= f;
 #pragma unroll
@@ -404,12 +432,16 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) o[dt][r] *= f;
         }
+        if (far) {
+            from_reference(z[0], ref);
+            from_reference(z[1], ref);
+        }
         x8 p[4];
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
             for (int r = 0; r < 16; r += 2) {
-                const float w0 = exp2_fast(fmaf(z[kt][r], c1, -mc)), w1 = exp2_fast(fmaf(z[kt][r + 1], c1, -mc));
+                const float w0 = exp2_fast(fmaf(z[kt][r], c1, -mz)), w1 = exp2_fast(fmaf(z[kt][r + 1], c1, -mz));
                 l0 += w0;                     // the sum takes the weights as they are: the log-sum is float32
                 l1 += w1;
                 const int g = 2 * kt + (r >> 3);
@@ -511,6 +543,8 @@ __global__ __launch_bounds__(256, 2) void attn_tile32_kernel(AttnArgs a) {
     };
     const float c1 = a.scale * LOG2E;
     float ref = -INFINITY, mc = 0.0f, l = 0.0f;
+    float mz = 0.0f;
+    int far = 0;
     constexpr int ASIDE = DT > 2 || !LONG ? 0 : DT;
     f32x16 o[DT], aside[ASIDE + 1];
 #pragma unroll
@@ -582,9 +616,10 @@ __global__ __launch_bounds__(256, 2) void attn_tile32_kernel(AttnArgs a) {
         if (__any((m - ref) * c1 > 8.0f)) {
             const float now = fmaxf(m, ref);
             const float mcn = now == -INFINITY ? 0.0f : now * c1;
-            const float f = ref == -INFINITY ? 0.0f : exp2_fast(mc - mcn);
+            const float f = rescale(ref, mc, now, mcn, c1);
             ref = now;
             mc = mcn;
+            far = far_away(ref, mc, c1, 0.0f, mz);
             l *= f;
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt)
@@ -594,9 +629,10 @@ __global__ __launch_bounds__(256, 2) void attn_tile32_kernel(AttnArgs a) {
                     if (dt < ASIDE) aside[dt][r] *= f;
                 }
         }
+        if (far) from_reference(z, ref);
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            z[r] = exp2_fast(fmaf(z[r], c1, -mc));
+            z[r] = exp2_fast(fmaf(z[r], c1, -mz));
             l += z[r];
         }
         // Short chains of sums: added to the running sum, each key would be rounded to its last place (the last of 16,000 rows:
@@ -712,6 +748,8 @@ __global__ __launch_bounds__(NW * 64) void attn_step_kernel(AttnArgs a) {
     const float c1 = a.scale * LOG2E;
     constexpr float LIFT = lift<T>();
     float ref = -INFINITY, mc = 0.0f, l = 0.0f;
+    float mz = 0.0f;
+    int far = 0;
     f32x16 o[DT];
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
@@ -759,18 +797,20 @@ __global__ __launch_bounds__(NW * 64) void attn_step_kernel(AttnArgs a) {
         if (__any((m - ref) * c1 > 8.0f)) {
             const float now = fmaxf(m, ref);
             const float mcn = now == -INFINITY ? 0.0f : now * c1 - LIFT;
-            const float f = ref == -INFINITY ? 0.0f : exp2_fast(mc - mcn);
+            const float f = rescale(ref, mc, now, mcn, c1);
             ref = now;
             mc = mcn;
+            far = far_away(ref, mc, c1, LIFT, mz);
             l *= f;
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) o[dt][r] *= f;
         }
+        if (far) from_reference(z, ref);
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            z[r] = exp2_fast(fmaf(z[r], c1, -mc));
+            z[r] = exp2_fast(fmaf(z[r], c1, -mz));
             l += z[r];
         }
         if constexpr (F32) {

@@ -227,3 +227,47 @@ def test_attention_joins_runs_of_keys_by_what_they_hold(sc, dt, nq, nk):
     want = v[at.cuda()].double().cpu().mean(0).expand(nq, 1, 32)
     size = v[at.cuda()].double().cpu().abs().mean(0).expand(nq, 1, 32)
     within(out, want, half(dt) * (want.abs() + size) + (nk + 64) * U * size, "ties")
+
+
+# ---- attention: enormous scores ----------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dt", ALL)
+@pytest.mark.parametrize("nq,nk", [(64, 400), (64, 3000), (1, 400), (1, 30000), (3, 700)])
+@pytest.mark.parametrize("std", [300.0, 3000.0, 16000.0])
+def test_attention_of_enormous_scores_stays_a_mean(sc, dt, nq, nk, std):
+    """float32 says nothing about which key wins where scores of 1e6 to 1e11 are closer than their roundings; but the result is a
+    mean of the values, 1 where these are all 1 (rounded weights: 2 u), and the log-sum is near the largest score: the
+    dot product's 64 roundings of U, and one each for scale, product with log2 e and back."""
+    g = torch.Generator().manual_seed(67)
+    q, k, v = ((torch.randn(n, 2, 64, generator=g) * s).clamp(-60000, 60000).to(DT[dt]).cuda() for n, s in ((nq, std), (nk, std), (nk, 1.0)))
+    v[..., :8] = 1
+    for kw in ({}, {"key_mask": (torch.rand(nk, generator=g) < 0.5).cuda()}):
+        out, lse = sc.attention(q, k, v, sc.seq_layout([0, nq], [0, nk]), scale=0.125, causal=False, return_lse=True, **kw)
+        z = torch.einsum("ihd,jhd->ihj", q.double().cpu(), k.double().cpu()) * 0.125
+        size = torch.einsum("ihd,jhd->ihj", q.double().cpu().abs(), k.double().cpu().abs()) * 0.125
+        if kw:
+            z[..., ~kw["key_mask"].cpu()] = -math.inf
+        want = torch.logsumexp(z, 2)
+        within(out[..., :8], torch.ones(nq, 2, 8), 3 * half(dt) + (nk + 64) * U, "mean of ones")
+        within(lse, want, (64 + 8) * U * size.amax(2) + math.log(nk), "lse")
+        assert float(out.abs().max()) <= float(v.abs().max()) * (1 + 3 * half(dt) + 1e-5)
+
+
+@pytest.mark.parametrize("dt", ALL)
+@pytest.mark.parametrize("nq,nk,ties", [(64, 400, 5), (64, 3000, 7), (1, 400, 5), (1, 30000, 300), (3, 200, 7), (9, 30000, 1)])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_attention_of_enormous_scores_that_are_exact(sc, dt, nq, nk, ties, sign):
+    """Scores of 1.875 x 2^33 that float32 holds exactly, and others far below, or far below 0: the mean of the tied keys' values,
+    to the roundings of the sum and of the result."""
+    g = torch.Generator().manual_seed(68)
+    a, b = 1.25 * 2.0 ** 14, 1.5 * 2.0 ** 14
+    q, k, v = torch.full((nq, 1, 32), a), torch.full((nk, 1, 32), b if sign < 0 else b * (1 - 2.0 ** -6)), normal(g, (nk, 1, 32), dt)
+    at = torch.randperm(nk, generator=g)[:ties]
+    k[::3] /= 4
+    if sign < 0:
+        k *= -2
+    k[at] = -b / 4 if sign < 0 else b
+    at = at if sign > 0 else (k[:, 0, 0] == k.max()).nonzero()[:, 0]
+    out = sc.attention(q.to(DT[dt]).cuda(), k.to(DT[dt]).cuda(), v, sc.seq_layout([0, nq], [0, nk]), scale=1.0, causal=False)
+    want = v[at.cuda()].double().cpu().mean(0).expand(nq, 1, 32)
+    size = v[at.cuda()].double().cpu().abs().mean(0).expand(nq, 1, 32)
+    within(out, want, half(dt) * want.abs() + (nk + 64) * U * size, "ties")
