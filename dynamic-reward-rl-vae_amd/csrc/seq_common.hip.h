@@ -106,6 +106,7 @@ __device__ __forceinline__ int find_seg(const SegInfo* segs, int n_seg, uint32_t
 // A tile row holds NC chunks of 16 bytes; chunk c of row r lies at place c ^ swz<NC>(r).  With it neither the reads of one
 // chunk of 16 consecutive rows (ds_read_b128, an MFMA operand's rows) nor the transposing reads of four consecutive
 // rows by 64 bytes (ds_read_b64_tr_b16) meet on a bank: LDS has 64 banks of 4 bytes, so 256 bytes go at once.
+// Reads of 8 bytes of 32 rows (linear attention's, in the order of its accumulators) do: rows 16 apart lie alike.
 template <int NC>
 __device__ __forceinline__ int swz(int r) {
     if constexpr (NC == 4) return (r >> 2) & 3;

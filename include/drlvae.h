@@ -270,8 +270,12 @@ typedef struct drl_seq_call {
  *   out_i = sum_j softmax_j(scale q_i.k_j) v_j,   lse_i = log sum_j exp(scale q_i.k_j)     over the visible keys j.
  * In a series of nq rows and nk keys, row i sees key j when j <= i + nk - nq (causal), j > i + nk - nq - window
  * (window > 0), and key_mask[j] != 0.  A row that sees nothing gets out = 0, lse = -inf.  What q, k or v hold behind
- * masked keys, infinities and NaN included, has no influence.  nq = 1 is the step of a live series against its cache:
- * k_offsets then name the cache's slots, and k_len how many of each are filled (nk above). */
+ * masked keys, infinities and NaN included, has no influence.  Of what a row does see, a value that is not finite makes its
+ * column of the result infinite or NaN, a score that is +infinity or NaN the row.  Sums are float32, with weights of up to
+ * 2^8: in float32 and bfloat16 |v| times the number of keys has to stay below 2^119.  With 16-bit types and more than 32
+ * (row, head) pairs to a series and kv head the weights are rounded to the type for their product with v, as the result is.
+ * nq = 1 is the step of a live series against its cache: k_offsets then name the cache's slots, and k_len how many of each
+ * are filled (nk above). */
 typedef struct drl_attn_args {
     const void* q;            /* rows x n_heads x dim */
     const void* k;            /* rows x n_kv_heads x dim */
@@ -296,7 +300,9 @@ int drl_attention_dev(drl_ctx* ctx, const drl_seq_layout* layout, const drl_seq_
  *   S <- exp(d_h) S + k_t v_t^T,   out_t = scale S^T q_t,      d_h = min(log_decay[h], 0)
  * The states S are float32 [n_seg, n_heads, dim_k, dim_v]; state_in NULL: they start at 0; state_out NULL: the last
  * ones are not kept; state_out may be state_in.  A series without rows hands its state on.  k_offsets of the layout are
- * not used: k and v have q's rows.  A value that is not finite makes its column of the outputs and of the state not finite
+ * not used: k and v have q's rows.  With 16-bit types the series form rounds scores and, for the product with q, the state
+ * to the type, as the result is; the state itself is float32 throughout (float16: what a row adds is lost below 2^-38 of
+ * the most that one of 32 rows adds to the column).  A value that is not finite makes its column of the outputs and of the state not finite
  * (NaN, but for steps) from its row on, and reaches nothing before it.
  * drl_linear_attention_step_dev: n series with one row each, state_in and state_out required. */
 typedef struct drl_linear_args {
@@ -323,7 +329,7 @@ int drl_linear_attention_step_dev(drl_ctx* ctx, int64_t n, const drl_seq_call* c
 /* Group normalisation with an activation, channels last: channels are cut into `groups` equal groups, and over each
  * group's channels, in all rows of a series (layout NULL: in each of `rows` rows by itself),
  *   y = act((x - mean) / sqrt(var + eps) * gamma + beta)          (var: the mean squared deviation)
- * y may be x (with the same row stride). */
+ * y may be x (with the same row stride), and overlaps it in no other way. */
 typedef struct drl_norm_args {
     const void* x;            /* rows x channels */
     void* y;
