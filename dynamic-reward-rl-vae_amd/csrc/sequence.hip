@@ -30,7 +30,8 @@ using seq::f16;
 
 // Device memory of the layouts' tables.  Small ones come out of slabs: a layout is made for every new batch, and asking the
 // runtime for memory takes longer than the rest of it.  A table given back may still be read by work under way, on any
-// stream: it waits among the retired until the device has been waited for once, which happens when many have gathered.
+// stream: it waits among the retired until the device has been waited for once, which happens when many have gathered.  Slabs are kept
+// until the process ends.
 class TablePool {
     static constexpr size_t SLAB = 256 << 10, LARGEST = 32 << 10, MOST_RETIRED = 64;
     std::mutex mu;

@@ -329,7 +329,8 @@ int drl_linear_attention_step_dev(drl_ctx* ctx, int64_t n, const drl_seq_call* c
 /* Group normalisation with an activation, channels last: channels are cut into `groups` equal groups, and over each
  * group's channels, in all rows of a series (layout NULL: in each of `rows` rows by itself),
  *   y = act((x - mean) / sqrt(var + eps) * gamma + beta)          (var: the mean squared deviation)
- * y may be x (with the same row stride), and overlaps it in no other way. */
+ * y may be x (with the same row stride), and overlaps it in no other way.  Sums are float32: a group's squared deviations have
+ * to stay in its range (|x - mean| below 1e19 / sqrt(the group's values)). */
 typedef struct drl_norm_args {
     const void* x;            /* rows x channels */
     void* y;
