@@ -271,3 +271,35 @@ def test_attention_of_enormous_scores_that_are_exact(sc, dt, nq, nk, ties, sign)
     want = v[at.cuda()].double().cpu().mean(0).expand(nq, 1, 32)
     size = v[at.cuda()].double().cpu().abs().mean(0).expand(nq, 1, 32)
     within(out, want, half(dt) * want.abs() + (nk + 64) * U * size, "ties")
+
+
+@pytest.mark.parametrize("seed", range(36))
+def test_attention_random_cases_of_scores_that_are_exact(sc, seed):
+    """Whole numbers times 2^e: every score is exact in float32, and scores that are not tied differ by 4^e, 64 at least: each row
+    is the mean of its largest keys' values, whatever the lengths, masks, windows and runs."""
+    import random
+
+    from oracle import sequence as orc
+    from test_sequence import lengths_of
+    r, g = random.Random(seed), torch.Generator().manual_seed(seed)
+    dt = ALL[seed % 3]
+    G, D = r.choice([1, 2]), 8 * r.randint(1, 16)
+    H = G * r.choice([1, 2, 5, 8])
+    n = r.randint(1, 4)
+    qo = offs(lengths_of(r, n, r.choice([3, 200])))
+    ko = qo if r.random() < 0.4 else offs(lengths_of(r, n, r.choice([100, 2500])))
+    e = r.choice([3, 7, 10, 12])
+    whole = lambda rows, heads: (torch.randint(-3, 4, (rows, heads, D), generator=g) * 2.0 ** e).to(DT[dt]).cuda()  # noqa: E731
+    q, k, v = whole(qo[-1], H), whole(ko[-1], G), normal(g, (ko[-1], G, D), dt)
+    if r.random() < 0.3:
+        q, k = q.abs(), -k.abs()                                # all scores below 0
+    mask = (torch.rand(ko[-1], generator=g) < r.choice([0.2, 0.9])).cuda() if r.random() < 0.5 else None
+    kw = dict(scale=1.0, causal=r.random() < 0.6, window=r.choice([0, 0, 7, 64, 300]), key_mask=mask)
+    out, lse = sc.attention(q, k, v, sc.seq_layout(qo, ko), return_lse=True, **kw)
+    want, wl, weight, _ = orc.attention(q, k, v, qo, ko, **kw)
+    nk = max([1] + [b - a for a, b in zip(ko, ko[1:])])
+    # references past 2^10 are rounded, by U times themselves, which all weights of a row share; two tiles' differ by that
+    top = torch.where(torch.isinf(wl), 0.0, wl.abs())
+    E = (nk + 64) * U + torch.where(top * 1.45 > 2.0 ** 20, 0.0, 4 * U * top)
+    within(out, want, (half(dt) + E[..., None]) * weight + half(dt) * want.abs() + torch.finfo(DT[dt]).tiny, "out")
+    within(lse, wl, 4 * U * top + (nk + 64) * U + torch.where(top > 2.0 ** 20, math.log(nk) + 5, 0.0), "lse")
