@@ -240,8 +240,8 @@ __device__ __forceinline__ void attn_store(const AttnArgs& a, const AttnTile& t,
 // order of the keys inside the product is free, and the values are read with ds_read_b64_tr_b16 in the weights' order.
 // Bound by issue: one series of 8,192 rows, 32 heads over 8, dim 128, bfloat16: 525-565 us by card, 0.97-1.05 PFLOP/s (one
 // library product of 8,192^3: 1.17), matrix pipe 53 % busy and VALU 50 %, each waiting for the other's results.  24 ragged
-// series of up to 2,048 rows, 16 heads over 4, dim 64, float16, a tenth of the keys masked: 135 us, VALU 69 %, matrix pipe
-// 33 %: the exponentials and their sums are the same for half the products.
+// series of up to 2,048 rows, 16 heads over 4, dim 64, float16, a tenth of the keys masked: 134-143 us by card, VALU 71 %,
+// matrix pipe 33 %: the exponentials and their sums are the same for half the products.
 template <typename T, int DT, bool MASK>
 __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
     typedef typename Vec<T>::x8 x8;
@@ -698,7 +698,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile32_kernel(AttnArgs a) {
 // own, every NW-th, in two LDS buffers of its own, and waits for nothing but its own loads (with a key mask, whose bytes are
 // asked for last, for those of the tile to come as well); at the end the waves' sums are joined through LDS.  With 16-bit
 // types, what the weights lose by rounding goes into a second product: it is free here. 16 caches of up to 32,768 rows, 8 kv
-// heads, dim 128, bfloat16: 256 us, 4.9 TB/s (a copy: 4.7), with a mask 292; 4 of up to 384: 8.4 us in a graph, of which the
+// heads, dim 128, bfloat16: 256 us, 4.9 TB/s (a copy: 4.7), with a mask 288; 4 of up to 384: 8.6 us in a graph, of which the
 // shortest launch is 5.4.  In float32 the products bound it, of 32 rows where 4 are there: 16 caches of up to 16,384 rows,
 // 790 us, 1.9 TB/s.
 template <typename T, int DT, int NW>

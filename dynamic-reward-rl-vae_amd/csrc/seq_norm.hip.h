@@ -70,7 +70,7 @@ __device__ __forceinline__ Moments join_lanes(Moments m, int lanes) {
 // Rows by themselves.  `lanes` lanes hold a group of a row, NV packs of V channels each (NV = 0: it does not fit, and is
 // read twice more from the caches); a wave has 64 / lanes neighbouring groups and goes down the rows with them, so that
 // gamma and beta stay in registers.  65,536 rows of 4,096 channels in 32 groups, bfloat16: 241 us, 4.5 TB/s (a copy: 4.7); 4
-// rows of 1,024: 7.9 us, a launch.
+// rows of 1,024: 7.0 us, a launch.
 template <typename T, int V, int NV>
 __global__ __launch_bounds__(256) void norm_rows_kernel(NormArgs a) {
     typedef Pack<T, V> P;

@@ -47,8 +47,15 @@ def _scale(scale, dim):
 
 def _whole(offsets):
     a = np.asarray(offsets)
-    if a.size and a.dtype.kind not in "iu":
-        raise ValueError(f"offsets are whole numbers, not {a.dtype}")        # a fraction would be cut off without a word
+    if a.dtype.kind != "i":
+        try:
+            with np.errstate(invalid="ignore"):
+                whole = a.astype(np.int64)
+        except (OverflowError, TypeError, ValueError):
+            whole = None
+        if whole is None or not np.array_equal(whole, a):        # a fraction would be cut off without a word
+            raise ValueError(f"offsets are whole numbers of 64 bits, not {offsets!r:.200}")
+        a = whole
     return np.ascontiguousarray(a, dtype=np.int64)
 
 

@@ -1,6 +1,7 @@
 """CPU-only: the argument checks of the sequence operators (csrc/seq_check.h compiled on its own), the structs' layout on
 both sides of the ABI, and the refusals of the Python layer."""
 import ctypes as C
+import math
 import os
 import subprocess
 
@@ -234,12 +235,12 @@ def test_offsets_are_whole_numbers():
     import numpy as np
     import torch
     s = _scorer()
-    for bad in ([0, 1.9], np.array([0.0, 4.0]), torch.tensor([0.0, 4.0]), [False, True], [0, 1 << 70]):
+    for bad in ([0, 1.9], np.array([0.0, math.nan]), torch.tensor([0.0, 3.5]), [0, 1 << 70], [0, 1e30], np.array([0, (1 << 64) - 1], dtype=np.uint64), ["a", "b"], [0, None]):
         with pytest.raises(ValueError, match="whole numbers"):
             s.seq_layout(bad)
         with pytest.raises(ValueError, match="whole numbers"):
             s.seq_layout([0, 4], bad)
-    for good in ([0, 4], range(0, 8, 4), np.array([0, 4], dtype=np.uint16), torch.tensor([0, 4]), (np.int32(0), 4)):
+    for good in ([0, 4], [0.0, 4.0], torch.tensor([0.0, 4.0]), range(0, 8, 4), np.array([0, 4], dtype=np.uint16), torch.tensor([0, 4]), (np.int32(0), 4)):
         layout = s.seq_layout(good)
         assert (layout.n_seg, layout.q_rows) == (1, 4)
 
