@@ -33,6 +33,36 @@ __device__ __forceinline__ float decay_log(const LinearArgs& a, int h) {
 }
 __device__ __forceinline__ float power(float ld2, int n) { return n == 0 ? 1.0f : exp2_fast(ld2 * (float)n); }
 
+// A state over n rows: S + (lam^n - 1) S where lam^n is above 1/2, since lam^n itself, rounded, would drift over many times; where
+// it is below, lam^n S, since 1 + (lam^n - 1) would keep an error of the old state's last place: all of a state that dies out.
+struct Decay {
+    float f;
+    bool most;
+    __device__ __forceinline__ float operator()(float S) const { return fmaf(S, f, most ? S : 0.0f); }
+};
+__device__ __forceinline__ Decay decay_of(const LinearArgs& a, int h, int n) {
+    const float less = expm1f(decay_log(a, h) * (float)n);
+    const bool most = !(less < -0.5f);                         // a NaN stays one
+    return {most ? less : power(decay_log(a, h) * LOG2E, n), most};
+}
+// The same over chunk after chunk with one product: lam^n in its two roundings, in such turns that their product is never further
+// than 2^-24 from lam's power (none of this below 1/2, where nothing is left to drift).
+struct ChunkDecay {
+    float f, rest, owed;
+    __device__ __forceinline__ ChunkDecay(const LinearArgs& a, int h, int n) {
+        const Decay d = decay_of(a, h, n);
+        f = uniform(d.most ? 1.0f + d.f : d.f);
+        rest = uniform(d.most ? d.f - (f - 1.0f) : 0.0f);
+        owed = 0.0f;
+    }
+    __device__ __forceinline__ float next() {
+        owed += rest;
+        const float more = owed > 0x1p-25f ? 0x1p-24f : owed < -0x1p-25f ? -0x1p-24f : 0.0f;      // a last place of [1/2, 1)
+        owed -= more;
+        return f + more;
+    }
+};
+
 struct LinearUnit {
     SegInfo s;
     int64_t u;
@@ -76,9 +106,7 @@ __global__ __launch_bounds__(256) void linear_step_kernel(LinearArgs a) {
     if (on)
 #pragma unroll
         for (int e = 0; e < 4; ++e) vc[e] = (float)v[e];
-    // lam - 1: lam itself, rounded, is off by the same 2^-25 in every step, which a long memory adds up (2,000 steps: 1e-4).  An
-    // infinite state, of which that would make a NaN, takes lam.
-    const float fall = expm1f(decay_log(a, h)), lam = 1.0f + fall;
+    const Decay decay = decay_of(a, h, 1);
     const int64_t sb = (row * a.heads + h) * (int64_t)a.dk * a.dv + x * 4;
     const float* in = a.state_in + sb;
     float* out = a.state_out + sb;
@@ -100,7 +128,8 @@ __global__ __launch_bounds__(256) void linear_step_kernel(LinearArgs a) {
                     const float kk = kq[0][r], qq = kq[1][r];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const float kept = fabsf(S[u][e]) < INFINITY ? fmaf(S[u][e], fall, S[u][e]) : lam * S[u][e];
+                        // an infinite state stays one
+                        const float kept = fabsf(S[u][e]) < INFINITY ? decay(S[u][e]) : S[u][e] * (decay.most ? 1.0f + decay.f : decay.f);
                         S[u][e] = fmaf(kk, vc[e], kept);
                         acc[e] = fmaf(qq, S[u][e], acc[e]);
                     }
@@ -235,7 +264,8 @@ __global__ __launch_bounds__(NW * 64, STATE ? 3 : 2) void linear_chunk_kernel(Li
             if (!STATE) lds_write<f32x4>(inner_at + r * 256, inner);
         }
     const float grown = a.scale * power(ld2, col + 1);         // of this lane's row from the chunk's start
-    float fall = expm1f(decay_log(a, h) * (float)C);           // lam^n - 1: lam^n itself, rounded, would drift over many chunks
+    ChunkDecay decay(a, h, C);
+    const float lam_rest = ChunkDecay(a, h, t.rows % C).f;     // of a chunk that is not full
 
     T* op = (T*)a.out + row0 * a.o_row + (int64_t)h * a.o_head + c0;
     // the state has arrived: no wait for it inside the loop, where it would be one for the chunks to come
@@ -255,7 +285,7 @@ __global__ __launch_bounds__(NW * 64, STATE ? 3 : 2) void linear_chunk_kernel(Li
         __syncthreads();
         if (base + 2 * C < t.rows) stage(base + 2 * C, far);
         if (c0 >= a.dv) continue;                              // a wave behind the values' width only loads
-        if (n < C) fall = expm1f(decay_log(a, h) * (float)n);
+        const float lam_n = n < C ? lam_rest : decay.next();
         const uint32_t kb = lds + buf * STAGE, qb = kb + QK + VB;
 
         x8 v[2];
@@ -407,7 +437,7 @@ __global__ __launch_bounds__(NW * 64, STATE ? 3 : 2) void linear_chunk_kernel(Li
             f32x16 acc;
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                S[kt][r] = fmaf(S[kt][r], fall, S[kt][r]);
+                S[kt][r] *= lam_n;
                 acc[r] = F16 ? 0.0f : S[kt][r];
             }
 #pragma unroll
@@ -506,7 +536,8 @@ __global__ __launch_bounds__(NW * 64) void linear_chunk32_kernel(LinearArgs a) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) up[r] = uniform(power(ld2, acc_row(r, 0)));
     const float lane_up = a.scale * power(ld2, 4 * half + 1), lane_left = power(ld2, 4 - 4 * half);
-    float fall = expm1f(decay_log(a, h) * (float)C);
+    ChunkDecay decay(a, h, C);
+    const float lam_rest = ChunkDecay(a, h, t.rows % C).f;     // of a chunk that is not full
     float* op = (float*)a.out + row0 * a.o_row + (int64_t)h * a.o_head;
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt) asm volatile("" : "+v"(S[kt]));        // arrived
@@ -517,7 +548,7 @@ __global__ __launch_bounds__(NW * 64) void linear_chunk32_kernel(LinearArgs a) {
         __syncthreads();
         if (base + C < t.rows) stage(base + C, buf ^ 1);
         if (c0 >= a.dv) continue;
-        if (n < C) fall = expm1f(decay_log(a, h) * (float)n);
+        const float lam_n = n < C ? lam_rest : decay.next();
         const uint32_t at = buf * STAGE;
         float v[16];
         bool odd = false;
@@ -584,7 +615,7 @@ __global__ __launch_bounds__(NW * 64) void linear_chunk32_kernel(LinearArgs a) {
                 sum = mfma(lds_read<float>(k), v[r], sum);
             }
 #pragma unroll
-            for (int r = 0; r < 16; ++r) S[kt][r] = fmaf(S[kt][r], fall, S[kt][r]) + sum[r];
+            for (int r = 0; r < 16; ++r) S[kt][r] = fmaf(S[kt][r], lam_n, sum[r]);
         }
         if (odd && bad < C)
 #pragma unroll
@@ -613,7 +644,7 @@ static __global__ __launch_bounds__(256) void linear_scan_kernel(LinearArgs a) {
     if (e >= size) return;
     const SegInfo s = a.segs[slot];
     const int n = max(1, (int)(((uint32_t)s.nq + a.piece - 1) / (uint32_t)a.piece));
-    const float fall = expm1f(decay_log(a, h) * (float)a.piece);
+    const Decay decay = decay_of(a, h, a.piece);
     f32x4 S = {0.0f, 0.0f, 0.0f, 0.0f};
     if (a.state_in) S = *(const f32x4*)(a.state_in + ((int64_t)s.seg * a.heads + h) * size + e);
     float* at = a.states + ((int64_t)(s.cum / (uint32_t)a.piece + slot) * a.heads + h) * size + e;
@@ -629,7 +660,7 @@ static __global__ __launch_bounds__(256) void linear_scan_kernel(LinearArgs a) {
             if (k + u >= n) break;
             at += next;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) S[c] = fmaf(S[c], fall, S[c]) + add[u][c];
+            for (int c = 0; c < 4; ++c) S[c] = decay(S[c]) + add[u][c];
             *(f32x4*)at = S;
         }
     }

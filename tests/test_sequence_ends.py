@@ -303,3 +303,56 @@ def test_attention_random_cases_of_scores_that_are_exact(sc, seed):
     E = (nk + 64) * U + torch.where(top * 1.45 > 2.0 ** 20, 0.0, 4 * U * top)
     within(out, want, (half(dt) + E[..., None]) * weight + half(dt) * want.abs() + torch.finfo(DT[dt]).tiny, "out")
     within(lse, wl, 4 * U * top + (nk + 64) * U + torch.where(top > 2.0 ** 20, math.log(nk) + 5, 0.0), "lse")
+
+
+# ---- linear attention: silence ------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dt", ALL)
+@pytest.mark.parametrize("others", [0, 63])
+@pytest.mark.parametrize("silent", [24, 64, 107])
+def test_linear_states_keep_their_relative_error_in_silence(sc, dt, others, silent):
+    """40 rows and then nothing: what is left of the state, 1e-2 to 1e-19 of it, is off by its own roundings, not by those of what
+    it was.  float16: the last rows' chunk loses 2^-38 of its largest weighted value (times k, 32 rows), which decays as the
+    state does."""
+    g = torch.Generator().manual_seed(70)
+    o = offs([40 + silent] + [1] * others)
+    q, k, v = normal(g, (o[-1], 4, 32), dt), normal(g, (o[-1], 4, 32), dt), normal(g, (o[-1], 4, 64), dt)
+    for x in (k, v):
+        x[40:40 + silent] = 0
+    ld = torch.tensor([-0.02, -0.1, -0.2, -0.4], device="cuda")
+    state = normal(g, (1 + others, 4, 32, 64), "f32", 3.0)
+    out, final = sc.linear_attention(q, k, v, ld, sc.seq_layout(o), state=state)
+    want, tol, S, stol = linear_bounds(dt, q, k, v, ld, o, 32 ** -0.5, state)
+    left = torch.exp(ld.double().cpu() * silent)[None, :, None, None]
+    floor = 32 * float(k.abs().max()) * float(v.abs().max()) * 2.0 ** -38 if dt == "f16" else 0.0
+    within(final, S, stol + floor * left, "final state")
+    within(out, want, tol, "out")
+
+
+def test_linear_steps_keep_their_relative_error_in_silence(sc):
+    """A state alone for 12 steps at rates from -1e-4 to -6: each step rounds twice at most, and knows exp(d) to 4 U and 2 U of |d|."""
+    d = torch.tensor([-1e-4, -0.1, -0.5, -0.69, -0.7, -2.0, -6.0, -math.inf], device="cuda")
+    g = torch.Generator().manual_seed(71)
+    start = (1 + torch.rand(1, 8, 32, 32, generator=g)).cuda()
+    state, zero, N = start.clone(), torch.zeros(1, 8, 32, device="cuda"), 12
+    for _ in range(N):
+        sc.linear_attention_step(zero, zero, zero, d, state)
+    want = start.double() * torch.exp(d.double() * N)[None, :, None, None]
+    within(state, want.cpu(), want.cpu() * (N * 2 * U * (3 + d[:7].abs().max().item())), "state")
+
+
+def test_linear_states_of_a_long_series_do_not_drift(sc):
+    """100,000 rows of which only the first holds anything, at memories of 20,000 rows to ever: lam^32, rounded, is off by up to 2^-25
+    in each of 3,125 chunks (one series among many) or lam^n in each of a few hundred pieces: together less than 2^-22 and the
+    states' own roundings, U each to either side: 8 sqrt(3125) U at the very most over their mean, 2 U of the rate."""
+    T = 100_000
+    d = torch.tensor([-5e-5, -1.7e-5, -3.1e-6, 0.0], device="cuda")
+    for dt in ("f32", "bf16"):
+        for others in (0, 63):
+            o = offs([T] + [1] * others)
+            q, k, v = (torch.zeros(o[-1], 4, 32, dtype=DT[dt], device="cuda") for _ in range(3))
+            g = torch.Generator().manual_seed(72)
+            state = (1 + torch.rand(1 + others, 4, 32, 32, generator=g)).cuda()
+            _, final = sc.linear_attention(q, k, v, d, sc.seq_layout(o), state=state)
+            want = torch.exp(d.double() * T)
+            off = ((final[0].double() / state[0].double()).mean((1, 2)) / want - 1).abs()
+            assert torch.all(off <= 4 * U + 8 * math.sqrt(3125 / 3 / 1024) * U + 2 * U * T * d.double().abs()), (dt, others, off)
