@@ -45,23 +45,32 @@ __device__ __forceinline__ Decay decay_of(const LinearArgs& a, int h, int n) {
     const bool most = !(less < -0.5f);                         // a NaN stays one
     return {most ? less : power(decay_log(a, h) * LOG2E, n), most};
 }
-// The same over chunk after chunk with one product: lam^n in its two roundings, in such turns that their product is never further
-// than 2^-24 from lam's power (none of this below 1/2, where nothing is left to drift).
-struct ChunkDecay {
-    float f, rest, owed;
-    __device__ __forceinline__ ChunkDecay(const LinearArgs& a, int h, int n) {
+// lam^n in its two roundings, f and the one beside it, by turns: the same over chunk after chunk with one product, which would drift
+// with f alone.  `owed` is what the factors so far are short of; a column begins with what its state's bits make of it, from -2^-25
+// to 2^-25, so that calls that hand a state on do not all round alike either.  (None of this below 1/2: nothing is left to drift.)
+struct Factor {
+    float f, rest;                // the same in all lanes
+    __device__ __forceinline__ Factor(const LinearArgs& a, int h, int n) {
         const Decay d = decay_of(a, h, n);
         f = uniform(d.most ? 1.0f + d.f : d.f);
         rest = uniform(d.most ? d.f - (f - 1.0f) : 0.0f);
-        owed = 0.0f;
     }
-    __device__ __forceinline__ float next() {
+    __device__ __forceinline__ float operator()(float& owed) const {
         owed += rest;
         const float more = owed > 0x1p-25f ? 0x1p-24f : owed < -0x1p-25f ? -0x1p-24f : 0.0f;      // a last place of [1/2, 1)
         owed -= more;
         return f + more;
     }
 };
+template <int KT>
+__device__ __forceinline__ float owed_at_first(const f32x16 (&S)[KT]) {
+    uint32_t bits = 0;
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) bits = bits * 5 + __builtin_bit_cast(uint32_t, S[kt][r]);
+    return ((float)(bits * 0x9e3779b1u >> 9) - 0x1p22f) * 0x1p-47f;
+}
 
 struct LinearUnit {
     SegInfo s;
@@ -264,8 +273,8 @@ __global__ __launch_bounds__(NW * 64, STATE ? 3 : 2) void linear_chunk_kernel(Li
             if (!STATE) lds_write<f32x4>(inner_at + r * 256, inner);
         }
     const float grown = a.scale * power(ld2, col + 1);         // of this lane's row from the chunk's start
-    ChunkDecay decay(a, h, C);
-    const float lam_rest = ChunkDecay(a, h, t.rows % C).f;     // of a chunk that is not full
+    const Factor whole(a, h, C), part(a, h, t.rows % C);       // over a chunk, and over one that is not full
+    float owed = owed_at_first<KT>(S);
 
     T* op = (T*)a.out + row0 * a.o_row + (int64_t)h * a.o_head + c0;
     // the state has arrived: no wait for it inside the loop, where it would be one for the chunks to come
@@ -285,7 +294,7 @@ __global__ __launch_bounds__(NW * 64, STATE ? 3 : 2) void linear_chunk_kernel(Li
         __syncthreads();
         if (base + 2 * C < t.rows) stage(base + 2 * C, far);
         if (c0 >= a.dv) continue;                              // a wave behind the values' width only loads
-        const float lam_n = n < C ? lam_rest : decay.next();
+        const float lam_n = (n < C ? part : whole)(owed);
         const uint32_t kb = lds + buf * STAGE, qb = kb + QK + VB;
 
         x8 v[2];
@@ -472,7 +481,7 @@ __global__ __launch_bounds__(NW * 64, STATE ? 3 : 2) void linear_chunk_kernel(Li
 }
 
 // float32: the same on 32x32x2 products; a register of the state or of the scores is an operand as it is, and nothing is
-// rounded or split.  24 series of up to 2,048 rows of 16 heads, 64 x 128: 570 us, matrix pipe 60 % busy (112 products of 64
+// rounded or split.  24 series of up to 2,048 rows of 16 heads, 64 x 128: 580 us, matrix pipe 60 % busy (112 products of 64
 // cycles a chunk and wave, of which 32 are scores that each of a workgroup's waves makes for itself), with the loads one chunk
 // ahead; one of 375 rows of 4 heads in 12 pieces: 20 us, of which its three launches take 6, 4 and 10.
 template <int KT, int NW, bool STATE>
@@ -536,8 +545,8 @@ __global__ __launch_bounds__(NW * 64) void linear_chunk32_kernel(LinearArgs a) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) up[r] = uniform(power(ld2, acc_row(r, 0)));
     const float lane_up = a.scale * power(ld2, 4 * half + 1), lane_left = power(ld2, 4 - 4 * half);
-    ChunkDecay decay(a, h, C);
-    const float lam_rest = ChunkDecay(a, h, t.rows % C).f;     // of a chunk that is not full
+    const Factor whole(a, h, C), part(a, h, t.rows % C);       // over a chunk, and over one that is not full
+    float owed = owed_at_first<KT>(S);
     float* op = (float*)a.out + row0 * a.o_row + (int64_t)h * a.o_head;
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt) asm volatile("" : "+v"(S[kt]));        // arrived
@@ -548,7 +557,7 @@ __global__ __launch_bounds__(NW * 64) void linear_chunk32_kernel(LinearArgs a) {
         __syncthreads();
         if (base + C < t.rows) stage(base + C, buf ^ 1);
         if (c0 >= a.dv) continue;
-        const float lam_n = n < C ? lam_rest : decay.next();
+        const float lam_n = (n < C ? part : whole)(owed);
         const uint32_t at = buf * STAGE;
         float v[16];
         bool odd = false;

@@ -356,3 +356,24 @@ def test_linear_states_of_a_long_series_do_not_drift(sc):
             want = torch.exp(d.double() * T)
             off = ((final[0].double() / state[0].double()).mean((1, 2)) / want - 1).abs()
             assert torch.all(off <= 4 * U + 8 * math.sqrt(3125 / 3 / 1024) * U + 2 * U * T * d.double().abs()), (dt, others, off)
+
+
+@pytest.mark.parametrize("rows", [32, 50])
+def test_linear_states_that_are_handed_on_do_not_drift(sc, rows):
+    """3,000 calls of a chunk or two that hold nothing new: a call must not take the same rounding of lam^n each time.  Per call
+    and column the factor is off by at most U to either side, the state's rounding by U: 8 sqrt(3000 / 3 / 32) U at the
+    very most over the mean of 32 columns, 2 U of the rate."""
+    N = 3000
+    d = torch.tensor([-1e-4, -3.3e-5, -7.1e-6, -2e-4], device="cuda")          # at most e^-30: float32's normal range
+    for dt, others in (("f32", 0), ("bf16", 0), ("f16", 63)):
+        o = offs([rows] + [1] * others)
+        layout = sc.seq_layout(o)
+        q, k, v = (torch.zeros(o[-1], 4, 32, dtype=DT[dt], device="cuda") for _ in range(3))
+        g = torch.Generator().manual_seed(73)
+        state = (1 + torch.rand(1 + others, 4, 32, 32, generator=g)).cuda()
+        start = state.clone()
+        for _ in range(N):
+            sc.linear_attention(q, k, v, d, layout, state=state, final_state=state)
+        want = torch.exp(d.double() * (N * rows))
+        off = ((state[0].double() / start[0].double()).mean((1, 2)) / want - 1).abs()
+        assert torch.all(off <= 8 * math.sqrt(N / 3 / 32) * U + 2 * U * N * rows * d.double().abs()), (dt, off)
