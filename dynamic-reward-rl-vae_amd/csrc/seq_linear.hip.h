@@ -177,9 +177,9 @@ __device__ __forceinline__ float into_range(float x, float& back) {
 // weighted values are scaled by powers of two before they are rounded, so that what is below 2^-38 of the largest score of a
 // row, or value of a column and chunk, is lost.
 // Two series of 32,768 rows, 32 heads of 128 x 128, bfloat16, in 16 pieces: 710-745 us by card, 300 for the pieces' states
-// (a second reading of k and v), 12 to join them, the rest the outputs; 2.15 GB once are 457 us.  VALU 53 % busy, matrix
-// pipe 44 %; LDS 26 % of the time, a third of it rows that meet on a bank.  24 ragged series, 16 heads of 64 x 128, float16:
-// 148 us, as long as the longest series' 64 chunks take, two workgroups to a CU; VALU 54 % (scales and splits), matrix pipe
+// (a second reading of k and v), 12 to join them, the rest the outputs; 2.15 GB once are 457 us.  VALU 51 % busy, matrix
+// pipe 42 %; LDS 25 % of the time, a third of it rows that meet on a bank.  24 ragged series, 16 heads of 64 x 128, float16:
+// 148 us, as long as the longest series' 64 chunks take, two workgroups to a CU; VALU 55 % (scales and splits), matrix pipe
 // 17 %, LDS 16 % (a quarter of it rows that meet); 92 us at a copy's rate.  Eight waves of 16 columns instead of four of 32:
 // 852 us against 760 at the time.
 template <typename T, int KT, int NW, bool STATE>
@@ -481,7 +481,7 @@ __global__ __launch_bounds__(NW * 64, STATE ? 3 : 2) void linear_chunk_kernel(Li
 }
 
 // float32: the same on 32x32x2 products; a register of the state or of the scores is an operand as it is, and nothing is
-// rounded or split.  24 series of up to 2,048 rows of 16 heads, 64 x 128: 580 us, matrix pipe 60 % busy (112 products of 64
+// rounded or split.  24 series of up to 2,048 rows of 16 heads, 64 x 128: 580 us, matrix pipe 58 % busy (112 products of 64
 // cycles a chunk and wave, of which 32 are scores that each of a workgroup's waves makes for itself), with the loads one chunk
 // ahead; one of 375 rows of 4 heads in 12 pieces: 20 us, of which its three launches take 6, 4 and 10.
 template <int KT, int NW, bool STATE>
